@@ -331,6 +331,91 @@ int envg_linear_rmsnorm(float* dst, const float* x, const float* weight, envg_we
 int envg_linear_noalloc(float* dst, const float* x, envg_weight W, const float* bias, int64_t M,
                         int64_t K, int64_t N, int epilogue, const float* gate, int flags);
 
+/* ---- language-model decode operators --------------------------------------------------------
+ * What a Qwen3-style layer runs from token to token around its norms: linears over 4-bit weights,
+ * the per-head norm of queries and keys with their position rotation, a paged key/value cache in
+ * 4 bits, and attention over it.  The reference runs these steps on whole prompts with 16-bit
+ * weights (quicknn_qwen3.pas:712-789); the 4-bit forms are new with this library.  All of them
+ * follow the conventions above (fp32 rows, status codes, host or device pointers by `flags`), take
+ * a row stride for every matrix and allocate nothing with device pointers.  Arguments that only
+ * the device can read (a page table, lengths, positions) are checked there: a value out of range
+ * reads and writes nothing out of bounds, and the next synchronising call returns ENVG_ERR_ARG. */
+
+/* Opaque device-resident 4-bit weight. */
+typedef struct envg_q4weight_s* envg_q4weight;
+
+/* Rounds W[N, K] to 4-bit codes on the host (needs no GPU): for each group of `group` (32, 64 or
+ * 128) columns of a row, s = (max - min) / 15 over its values and 0, z = rint(-min / s),
+ * c = clamp(rint(w / s) + z, 0, 15), so that w is held as (c - z) s.  codes: [N, ceil(K / 2)]
+ * bytes, even column in the low nibble; scales fp32 and zeros uint8: [N, ceil(K / group)]. */
+int envg_quantize_q4(const uint16_t* w_bf16, const float* w_f32, int64_t N, int64_t K, int group,
+                     uint8_t* codes, float* scales, uint8_t* zeros);
+
+/* Uploads a 4-bit weight W[n][k] = (c - z) s in the form envg_quantize_q4 writes; zeros may be
+ * NULL (z = 8 throughout), its entries are 0..15.  codes, scales and zeros are host or device
+ * pointers by `flags`; they may be freed after the call.  layout_flags: ENVG_LAYOUT_PLAIN or
+ * ENVG_LAYOUT_GATE_UP.  The codes are re-laid out once, here, for the kernels. */
+int envg_weight_upload_q4(const uint8_t* codes, const float* scales, const uint8_t* zeros, int64_t N,
+                          int64_t K, int group, int layout_flags, int flags, envg_q4weight* out);
+int envg_q4weight_free(envg_q4weight w);
+
+/* dst = epilogue(x . W^T) for a 4-bit weight, epilogues as envg_linear; x [M, K] of row stride
+ * ldx, dst [M, N] (N / 2 for ENVG_EPI_SILU_GATE) of row stride ldd.  The product is an fp32 one:
+ * codes are exact in the tensor cores' 16-bit operands, x is carried as two of them, scales are
+ * applied to the fp32 sums of their groups (about 1e-7 relative).  Made for few rows (M up to
+ * about 64); 0 <= M <= 65535.  A row of x that holds an infinity or a NaN gives non-finite
+ * outputs in that row.  dst must not overlap x. */
+int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4weight W, const float* bias,
+                   int64_t M, int64_t K, int64_t N, int epilogue, const float* gate, int flags);
+
+/* For every token t and head h of q (heads) and k (kv_heads):
+ *   y = rot(x * weight / sqrt(mean(x^2) + eps), position of t)
+ * (QNNRMSNormRows per head, then the rotation, of the Qwen3 layer).  rot turns each pair (a, b) of
+ * channels into (a cos - b sin, b cos + a sin); a pair is (i, i + head_dim / 2), or (2i, 2i + 1)
+ * when `interleaved`.  cos_table / sin_table: [table_rows, head_dim / 2], both NULL for the norm
+ * alone; the position of token t is positions[t] (int32), or pos0 + t when positions is NULL.
+ * q_weight / k_weight: [head_dim] or NULL.  Head h starts at column h * head_dim of its row.  One of
+ * heads and kv_heads may be 0 (its operands are then not read).  q_dst may be q and k_dst may be k
+ * (with the same stride).  head_dim: a multiple of 8 up to 256. */
+int envg_qk_norm_rope(float* q_dst, int64_t ldqd, float* k_dst, int64_t ldkd, const float* q, int64_t ldq,
+                      const float* k, int64_t ldk, const float* q_weight, const float* k_weight,
+                      const float* cos_table, const float* sin_table, int64_t table_rows,
+                      const int32_t* positions, int64_t pos0, int64_t tokens, int heads, int kv_heads,
+                      int head_dim, float eps, int interleaved, int flags);
+
+/* A key/value cache in 4 bits: `pages` pages of `page_size` (a multiple of 16 up to 1024) tokens,
+ * kv_heads heads of head_dim (64 or 128) channels.  For each token, head and group of 64 channels
+ * it holds m = fp16(min x), s = fp16((max x - min x) / 15) (both limited to fp16's range) and codes
+ * c = clamp(rint((x - m) / s), 0, 15), rounded to nearest even; the value is m + s c.  A group with
+ * a NaN holds NaN.  Created empty (all zeros). */
+typedef struct envg_kv4_s* envg_kv4;
+int envg_kv4_create(int64_t pages, int page_size, int kv_heads, int head_dim, envg_kv4* out);
+int envg_kv4_free(envg_kv4 c);
+
+/* Writes the newest q_len tokens of `batch` sequences to the cache.  Row b * q_len + i of k and v
+ * ([batch * q_len, kv_heads * head_dim], row strides ldk / ldv) is token ctx_lens[b] - q_len + i of
+ * sequence b (rows that would come before its first token are left out): ctx_lens counts the new
+ * tokens.  Token p stands in page table[b * table_stride + p / page_size] at p % page_size.  Pages
+ * may be shared between sequences as long as one call does not write a token twice. */
+int envg_kv4_append(envg_kv4 cache, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                    const int32_t* table, int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len,
+                    int flags);
+
+/* The values the cache holds for the same tokens (zeros for rows before a sequence's first token). */
+int envg_kv4_read(envg_kv4 cache, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table,
+                  int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int flags);
+
+/* Attention of the newest q_len tokens of each sequence over the cache (which holds them too):
+ * row b * q_len + i of q and dst ([batch * q_len, heads * head_dim]) stands at position
+ * p = ctx_lens[b] - q_len + i and sees the cached tokens j <= p; with window > 0 only those with
+ * j > p - window or j < sinks (the first tokens stay visible).  Head h reads kv head
+ * h / (heads / kv_heads).  dst = softmax(scale * q . k) . v in fp32 (about 1e-6 relative); a row
+ * that sees nothing is zeros.  max_ctx is the largest of ctx_lens where the caller knows it, or 0:
+ * it only plans how the work is split.  dst must not overlap q. */
+int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, envg_kv4 cache,
+                       const int32_t* table, int64_t table_stride, const int32_t* ctx_lens, int batch,
+                       int q_len, int max_ctx, int heads, int window, int sinks, float scale, int flags);
+
 /* cblas_sgemm-compatible fp32 GEMM on host pointers: the signature of the function-pointer
  * slot TQNNSingleOPS.cblas_sgemm (quicknncpu.pas:102-109; enums quicknn_common.pas:54-58:
  * RowMajor = 101, NoTrans = 111, Trans = 112).  Re-pointing that slot to this entry moves

@@ -30,6 +30,8 @@
 #include "../../include/envgemm.h"
 #include "attention.cuh"
 #include "kernels.cuh"
+#include "kv4.cuh"
+#include "q4.cuh"
 #include "safetensors.hpp"
 
 using namespace envg;
@@ -87,6 +89,7 @@ struct Dev {
   Buf x, y, xb, wb, part, cnt, bias, gate, act, col, b32, xbatch, ada, xn;
   Buf gn, c1, vec;  // GroupNorm statistics + affine, ResBlock conv1 output, small parameter vectors
   Buf fa, fain;     // attention operands (bf16 Q / K / V^T + key bits), host-call staging
+  Buf lm;           // host-call staging of the language-model decode operators
   cudaStream_t aux = nullptr;              // second stream of envg_linear_batch
   cudaStream_t h2d = nullptr, d2h = nullptr;  // copy streams of pipelined host-pointer calls
   std::vector<cudaEvent_t> pipe_events;    // reused event pool of the pipelined host calls
@@ -116,7 +119,7 @@ struct Dev {
   size_t ws_bytes() const {
     return x.bytes + y.bytes + xb.bytes + wb.bytes + part.bytes + cnt.bytes + sched.bytes + bias.bytes + gate.bytes + act.bytes +
            col.bytes + b32.bytes + xbatch.bytes + ada.bytes + xn.bytes + gn.bytes + c1.bytes + vec.bytes +
-           fa.bytes + fain.bytes + hb.bytes;
+           fa.bytes + fain.bytes + hb.bytes + lm.bytes;
   }
 };
 
@@ -128,7 +131,8 @@ int g_cur = -1;
 enum KernelId {
   KID_K1 = 0, KID_K1_SILU_GATE, KID_K1_CONV, KID_K2, KID_GEMV, KID_CAST, KID_ADALN, KID_TRANSPOSE, KID_IM2COL,
   KID_SELFTEST, KID_GN_STATS, KID_GN_AFFINE, KID_GN_APPLY, KID_ATTN, KID_CAST_HEADS, KID_KEY_BITS, KID_ABSMAX,
-  KID_SPLIT_REDUCE, KID_SKINNY_REDUCE, KID_RMSNORM, KID_CAST_X3, KID_COUNT
+  KID_SPLIT_REDUCE, KID_SKINNY_REDUCE, KID_RMSNORM, KID_CAST_X3, KID_Q4, KID_NORM_ROPE, KID_KV4_APPEND,
+  KID_KV4_READ, KID_KV4_ATTN, KID_COUNT
 };
 // Profile names are per family: "k1_gemm*" counts k1_gemm and k1_gemm_pair launches (plain,
 // SiLU-gate, conv), "k2_set" counts k2_set and the no-alloc path's k2_skinny.
@@ -138,7 +142,9 @@ const char* const kKernelNames[KID_COUNT] = {"k1_gemm",     "k1_gemm_silu_gate",
                                              "k_wait_selftest", "k_group_stats",     "k_group_affine",
                                              "k_group_apply",   "k_attention",       "k_cast_heads",
                                              "k_key_bits",      "k_absmax_heads",    "k_split_reduce",
-                                             "k_skinny_reduce", "k_rmsnorm",      "k_cast_x3"};
+                                             "k_skinny_reduce", "k_rmsnorm",      "k_cast_x3",
+                                             "k_q4",            "k_qk_norm_rope", "k_kv4_append",
+                                             "k_kv4_read",      "k_kv4_attn"};
 struct KAcc {
   uint64_t launches = 0;
   double ms = 0, flops = 0, bytes = 0;
@@ -487,6 +493,12 @@ int check_status(Dev* d) {
     if (d->cnt.p) cudaMemsetAsync(d->cnt.p, 0, d->cnt.bytes, stream_of(d));  // re-arm split-K counters
     if (d->sched.p) cudaMemsetAsync(d->sched.p, 0, d->sched.bytes, stream_of(d));  // and the schedules
     d->st.last_status = st;
+    if (st == ENVG_ERR_ARG)
+      return fail(st, "a device-side argument was out of range: %s",
+                  site == SITE_KV_PAGE    ? "the page table names no page of the cache (its tokens were left out)"
+                  : site == SITE_KV_LEN   ? "a context length does not fit its row of the page table"
+                  : site == SITE_ROPE_POS ? "a position lies outside the cos / sin tables"
+                                          : "a zero point of a 4-bit weight is above 15");
     return fail(st, "device-side wait exceeded its bound (site %d); pipeline abandoned", site);
   }
   return ENVG_OK;
@@ -1560,7 +1572,7 @@ int envg_shutdown(void) {
   cudaStreamSynchronize(stream_of(d));
   Buf* bufs[] = {&d->x,    &d->y,   &d->xb,  &d->wb,  &d->part,  &d->cnt,
                  &d->bias, &d->gate, &d->act, &d->col, &d->b32, &d->xbatch, &d->ada, &d->xn,
-                 &d->gn,   &d->c1,   &d->vec,  &d->fa,  &d->fain, &d->sched, &d->hb};
+                 &d->gn,   &d->c1,   &d->vec,  &d->fa,  &d->fain, &d->sched, &d->hb,   &d->lm};
   for (Buf* b : bufs) {
     if (b->p) cudaFree(b->p);
     *b = Buf{};
@@ -3380,3 +3392,5 @@ int envg_selftest_wait_timeout(uint64_t cap_ns) {
 }
 
 }  // extern "C"
+
+#include "lm_ops.hpp"

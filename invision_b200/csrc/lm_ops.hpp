@@ -1,0 +1,559 @@
+// lm_ops.hpp -- host side of the language-model decode operators (4-bit linears, q/k norm +
+// rotation, the paged 4-bit cache and its attention).  Part of envgemm.cu's translation unit: it
+// uses its device registry, error and launch helpers.
+#pragma once
+
+namespace {
+constexpr uint32_t Q4_MAGIC = 0xE17A9E44u;
+constexpr uint32_t KV4_MAGIC = 0xE17A9E4Cu;
+}  // namespace
+
+struct envg_q4weight_s {
+  uint32_t magic;
+  int dev;
+  uint8_t* d;
+  size_t bytes;
+  int layout;
+  Q4View v;
+};
+
+struct envg_kv4_s {
+  uint32_t magic;
+  int dev;
+  uint8_t* d;
+  size_t bytes;
+  int64_t pages;
+  int page_size, kv_heads, head_dim;
+};
+
+namespace {
+
+int lm_dev(Dev** d) {
+  *d = cur();
+  if (!*d) return fail(ENVG_ERR_STATE, "envg_init has not been called");
+  return ENVG_OK;
+}
+
+int check_q4(Dev* d, envg_q4weight w) {
+  if (!w || w->magic != Q4_MAGIC) return fail(ENVG_ERR_STATE, "invalid or freed 4-bit weight handle");
+  if (w->dev != d->id) return fail(ENVG_ERR_STATE, "weight lives on device %d, current device is %d", w->dev, d->id);
+  return ENVG_OK;
+}
+
+int check_kv4(Dev* d, envg_kv4 c) {
+  if (!c || c->magic != KV4_MAGIC) return fail(ENVG_ERR_STATE, "invalid or freed cache handle");
+  if (c->dev != d->id) return fail(ENVG_ERR_STATE, "cache lives on device %d, current device is %d", c->dev, d->id);
+  return ENVG_OK;
+}
+
+bool f4_ok(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
+
+// Device copies of a host-pointer call's operands, packed into one grow-only buffer.
+class LmStage {
+ public:
+  explicit LmStage(Dev* d) : d_(d) {}
+  // Reserves `bytes` and returns the piece's number; p() gives its address after commit().
+  int add(size_t bytes) {
+    at_.push_back(total_);
+    total_ += (size_t)rup((int64_t)std::max<size_t>(bytes, 16), 256);
+    return (int)at_.size() - 1;
+  }
+  int commit() { return ensure(d_, d_->lm, total_); }
+  template <typename T>
+  T* p(int i) const {
+    return reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(d_->lm.p) + at_[i]);
+  }
+  // rows x cols floats (or 4-byte integers) of row stride ld, packed
+  int in(int i, const void* src, int64_t ld, int64_t rows, int64_t cols) {
+    if (rows == 0 || cols == 0) return ENVG_OK;
+    ENVG_CUDA(cudaMemcpy2DAsync(p<uint8_t>(i), cols * 4, src, ld * 4, cols * 4, rows, cudaMemcpyHostToDevice, stream_of(d_)));
+    d_->st.h2d_bytes += 4.0 * rows * cols;
+    return ENVG_OK;
+  }
+  int out(int i, void* dst, int64_t ld, int64_t rows, int64_t cols) {
+    if (rows == 0 || cols == 0) return ENVG_OK;
+    ENVG_CUDA(cudaMemcpy2DAsync(dst, ld * 4, p<uint8_t>(i), cols * 4, cols * 4, rows, cudaMemcpyDeviceToHost, stream_of(d_)));
+    d_->st.d2h_bytes += 4.0 * rows * cols;
+    return ENVG_OK;
+  }
+
+ private:
+  Dev* d_;
+  size_t total_ = 0;
+  std::vector<size_t> at_;
+};
+
+int finish_call(Dev* d, int flags) {
+  d->st.calls++;
+  if (!(flags & ENVG_DEVICE_PTRS) || !(flags & ENVG_ASYNC)) return sync_and_check(d);
+  return ENVG_OK;
+}
+
+int launch_q4(Dev* d, const Q4Args& a) {
+  const double bytes = (double)a.w.tiles * a.w.kblocks * q4_block_bytes(a.w.group) + 4.0 * a.M * a.w.K + 4.0 * a.M * a.w.N;
+  ProfScope ps(stream_of(d), KID_Q4, 2.0 * a.M * (double)a.w.N * (double)a.w.K, bytes);
+  ENVG_TRY(launch_pdl(d, k_q4_simple, dim3((unsigned)cdiv(a.w.tiles, 4), (unsigned)a.M), dim3(128), 0, a));
+  d->st.kernel_launches++;
+  return ENVG_OK;
+}
+
+int launch_norm_rope(Dev* d, const NormRopeArgs& a) {
+  const int all = a.heads + a.kv_heads;
+  int lanes = 1;
+  while (lanes * 8 < a.hd) lanes *= 2;
+  const int64_t blocks = cdiv(a.tokens * all * lanes, 256);
+  if (blocks > INT32_MAX) return fail(ENVG_ERR_ARG, "qk_norm_rope: %lld tokens are too many", (long long)a.tokens);
+  ProfScope ps(stream_of(d), KID_NORM_ROPE, 0.0, 8.0 * (double)a.tokens * all * a.hd + 4.0 * (double)a.tokens * a.hd);
+  const dim3 g((unsigned)blocks), b(256);
+  switch (lanes) {
+    case 1: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<1>, g, b, 0, a)); break;
+    case 2: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<2>, g, b, 0, a)); break;
+    case 4: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<4>, g, b, 0, a)); break;
+    case 8: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<8>, g, b, 0, a)); break;
+    case 16: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<16>, g, b, 0, a)); break;
+    default: ENVG_TRY(launch_pdl(d, k_qk_norm_rope<32>, g, b, 0, a)); break;
+  }
+  d->st.kernel_launches++;
+  return ENVG_OK;
+}
+
+// Checks shared by the calls that name tokens of a cache through a page table.  The call touches
+// the new tokens, the `before` tokens in front of them and the first `sinks`: only the pages of
+// those have to exist.
+int check_kv_call(Dev* d, envg_kv4 c, const int32_t* table, int64_t table_stride, const int32_t* ctx_lens, int batch,
+                  int q_len, int64_t before, int sinks, int flags, const char* what) {
+  ENVG_TRY(check_kv4(d, c));
+  if (batch < 0 || q_len < 0 || table_stride < 0) return fail(ENVG_ERR_ARG, "%s: batch %d, q_len %d, table stride %lld", what, batch, q_len, (long long)table_stride);
+  if (table_stride * c->page_size > INT32_MAX)
+    return fail(ENVG_ERR_ARG, "%s: a table row names %lld tokens (at most 2^31 - 1)", what, (long long)(table_stride * c->page_size));
+  if (batch == 0 || q_len == 0) return ENVG_OK;
+  if (!table || !ctx_lens) return fail(ENVG_ERR_ARG, "%s: table or ctx_lens is NULL", what);
+  if ((int64_t)batch * q_len > INT32_MAX) return fail(ENVG_ERR_ARG, "%s: batch x q_len is too large", what);
+  if (!(flags & ENVG_DEVICE_PTRS)) {
+    for (int b = 0; b < batch; ++b) {
+      const int64_t n = ctx_lens[b];
+      if (n < 0 || n > table_stride * c->page_size)
+        return fail(ENVG_ERR_ARG, "%s: ctx_lens[%d] = %lld does not fit the table (%lld pages of %d)", what, b, (long long)n,
+                    (long long)table_stride, c->page_size);
+      const int64_t first = std::max<int64_t>(0, n - q_len - before) / c->page_size;
+      for (int64_t i = 0; i < cdiv(n, c->page_size); ++i) {
+        if (i < first && i >= cdiv(sinks, c->page_size)) continue;
+        const int32_t page = table[b * table_stride + i];
+        if (page < 0 || page >= c->pages)
+          return fail(ENVG_ERR_ARG, "%s: table[%d][%lld] = %d names no page (%lld pages)", what, b, (long long)i, page, (long long)c->pages);
+      }
+    }
+  }
+  return ENVG_OK;
+}
+
+Kv4View kv_view(Dev* d, envg_kv4 c, const int32_t* table, int64_t stride, const int32_t* lens) {
+  Kv4View v{};
+  v.base = c->d;
+  v.pages = c->pages;
+  v.page_size = c->page_size;
+  v.kv_heads = c->kv_heads;
+  v.table = table;
+  v.table_stride = stride;
+  v.ctx_lens = lens;
+  v.status = d->d_status;
+  return v;
+}
+
+// Append (k, v are read) or read back (k, v are written) the last q_len tokens of each sequence.
+int kv4_rows(envg_kv4 c, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table, int64_t stride,
+             const int32_t* lens, int batch, int q_len, int flags, bool read) {
+  const char* what = read ? "kv4_read" : "kv4_append";
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  ENVG_TRY(check_kv_call(d, c, table, stride, lens, batch, q_len, 0, 0, flags, what));
+  const int64_t rows = (int64_t)batch * q_len, width = (int64_t)c->kv_heads * c->head_dim;
+  if (rows == 0) return ENVG_OK;
+  if (!k || !v) return fail(ENVG_ERR_ARG, "%s: k or v is NULL", what);
+  if (ldk < width || ldv < width) return fail(ENVG_ERR_ARG, "%s: a row stride is shorter than kv_heads x head_dim", what);
+  if (read && k == v) return fail(ENVG_ERR_ARG, "kv4_read: k and v are the same buffer");
+  LmStage st(d);
+  const bool devp = (flags & ENVG_DEVICE_PTRS) != 0;
+  float *dk = k, *dv = v;
+  int64_t lk = ldk, lv = ldv;
+  int ik = 0, iv = 0;
+  if (!devp) {
+    ik = st.add(rows * width * 4), iv = st.add(rows * width * 4);
+    const int it = st.add(batch * stride * 4), il = st.add((size_t)batch * 4);
+    ENVG_TRY(st.commit());
+    if (!read) {
+      ENVG_TRY(st.in(ik, k, ldk, rows, width));
+      ENVG_TRY(st.in(iv, v, ldv, rows, width));
+    }
+    ENVG_TRY(st.in(it, table, stride, batch, stride));
+    ENVG_TRY(st.in(il, lens, batch, 1, batch));
+    dk = st.p<float>(ik), dv = st.p<float>(iv), lk = lv = width;
+    table = st.p<int32_t>(it), lens = st.p<int32_t>(il);
+  }
+  KvRowsArgs a{};
+  a.c = kv_view(d, c, table, stride, lens);
+  a.k = dk, a.v = dv, a.ldk = lk, a.ldv = lv;
+  a.hd = c->head_dim, a.batch = batch, a.q_len = q_len;
+  a.items = rows * c->kv_heads * 2 * (c->head_dim / KV_GROUP);
+  a.vec = f4_ok(dk, lk) && f4_ok(dv, lv);
+  const int64_t blocks = cdiv(a.items * 8, 256);
+  if (blocks > INT32_MAX) return fail(ENVG_ERR_ARG, "%s: too many rows", what);
+  {
+    ProfScope ps(stream_of(d), read ? KID_KV4_READ : KID_KV4_APPEND, 0.0,
+                 (double)rows * c->kv_heads * (8.0 * c->head_dim + c->head_dim + 8 * (c->head_dim / KV_GROUP)));
+    if (read) ENVG_TRY(launch_pdl(d, k_kv4_rows<true>, dim3((unsigned)blocks), dim3(256), 0, a));
+    else ENVG_TRY(launch_pdl(d, k_kv4_rows<false>, dim3((unsigned)blocks), dim3(256), 0, a));
+    d->st.kernel_launches++;
+  }
+  if (!devp && read) {
+    ENVG_TRY(st.out(ik, k, ldk, rows, width));
+    ENVG_TRY(st.out(iv, v, ldv, rows, width));
+  }
+  return finish_call(d, flags);
+}
+
+int launch_kv4_attn(Dev* d, const KvAttnArgs& a, int max_ctx) {
+  const int64_t items = (int64_t)a.batch * a.q_len * a.heads;
+  const double tok = (double)a.batch * max_ctx;
+  ProfScope ps(stream_of(d), KID_KV4_ATTN, 4.0 * a.hd * a.heads * (double)a.q_len * tok,
+               tok * a.c.kv_heads * (a.hd + 8 * (a.hd / KV_GROUP)) + 8.0 * (double)a.batch * a.q_len * a.heads * a.hd);
+  ENVG_TRY(launch_pdl(d, k_kv4_attn_simple, dim3((unsigned)cdiv(items, 4)), dim3(128), 0, a));
+  d->st.kernel_launches++;
+  return ENVG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int envg_quantize_q4(const uint16_t* w_bf16, const float* w_f32, int64_t N, int64_t K, int group, uint8_t* codes,
+                     float* scales, uint8_t* zeros) {
+  if ((w_bf16 == nullptr) == (w_f32 == nullptr)) return fail(ENVG_ERR_ARG, "exactly one of w_bf16 / w_f32 must be set");
+  if (N < 0 || K <= 0) return fail(ENVG_ERR_ARG, "quantize_q4: N=%lld K=%lld", (long long)N, (long long)K);
+  if (group != 32 && group != 64 && group != 128) return fail(ENVG_ERR_ARG, "quantize_q4: group %d (32, 64 or 128)", group);
+  if (N > 0 && (!codes || !scales || !zeros)) return fail(ENVG_ERR_ARG, "quantize_q4: NULL output");
+  const WSrc src{w_bf16, w_f32, K};
+  const int64_t ldc = (K + 1) / 2, ng = cdiv(K, group);
+  for (int64_t n = 0; n < N; ++n)
+    for (int64_t g = 0; g < ng; ++g) {
+      const int64_t k0 = g * group, k1 = std::min<int64_t>(K, k0 + group);
+      float lo = 0.0f, hi = 0.0f;  // the range always holds 0, so that 0 stays 0
+      for (int64_t k = k0; k < k1; ++k) {
+        const float v = src.value(n, k);
+        if (!std::isfinite(v)) return fail(ENVG_ERR_ARG, "quantize_q4: W[%lld][%lld] is not finite", (long long)n, (long long)k);
+        lo = std::min(lo, v), hi = std::max(hi, v);
+      }
+      const float s = std::isfinite(hi - lo) ? (hi - lo) / 15.0f : hi / 15.0f - lo / 15.0f;
+      const int z = s > 0.0f ? (int)std::nearbyint(std::min(15.0f, std::max(0.0f, -lo / s))) : 8;
+      scales[n * ng + g] = s;
+      zeros[n * ng + g] = (uint8_t)z;
+      for (int64_t k = k0; k < k1; ++k) {
+        const float c = s > 0.0f ? std::nearbyint(src.value(n, k) / s) + z : 8.0f;
+        const uint8_t q = (uint8_t)std::min(15.0f, std::max(0.0f, c));
+        uint8_t& b = codes[n * ldc + (k >> 1)];
+        b = (k & 1) ? (uint8_t)((b & 15) | (q << 4)) : q;
+      }
+    }
+  return ENVG_OK;
+}
+
+int envg_weight_upload_q4(const uint8_t* codes, const float* scales, const uint8_t* zeros, int64_t N, int64_t K,
+                          int group, int layout_flags, int flags, envg_q4weight* out) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!out) return fail(ENVG_ERR_ARG, "out handle pointer is NULL");
+  *out = nullptr;
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  if (!codes || !scales) return fail(ENVG_ERR_ARG, "weight_upload_q4: codes or scales is NULL");
+  if (N <= 0 || K <= 0 || N > INT32_MAX / 2 || K > INT32_MAX / 2)
+    return fail(ENVG_ERR_ARG, "weight_upload_q4: N=%lld K=%lld", (long long)N, (long long)K);
+  if (group != 32 && group != 64 && group != 128)
+    return fail(ENVG_ERR_ARG, "weight_upload_q4: group %d (32, 64 or 128)", group);
+  if (layout_flags != ENVG_LAYOUT_PLAIN && layout_flags != ENVG_LAYOUT_GATE_UP)
+    return fail(ENVG_ERR_ARG, "weight_upload_q4: layout %d (PLAIN or GATE_UP)", layout_flags);
+  const bool gu = layout_flags == ENVG_LAYOUT_GATE_UP;
+  if (gu && N % 2) return fail(ENVG_ERR_ARG, "weight_upload_q4: a GATE_UP weight has an even number of rows");
+  Q4View v{};
+  v.tiles = (int)(gu ? cdiv(N / 2, 8) : cdiv(N, 16));
+  v.kblocks = (int)cdiv(K, Q4_COLS);
+  v.group = group, v.gate_up = gu ? 1 : 0, v.N = N, v.K = K;
+  const int64_t blocks = (int64_t)v.tiles * v.kblocks;
+  if (blocks > INT32_MAX) return fail(ENVG_ERR_ARG, "weight_upload_q4: N=%lld K=%lld is too large", (long long)N, (long long)K);
+  const size_t bytes = (size_t)blocks * q4_block_bytes(group);
+  const size_t cb = (size_t)N * ((K + 1) / 2), ng = (size_t)N * cdiv(K, group);
+  uint8_t *dst = nullptr, *raw = nullptr;
+  if (cudaMalloc(reinterpret_cast<void**>(&dst), bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ENVG_ERR_OOM, "4-bit weight allocation of %zu bytes failed", bytes);
+  }
+  cudaStream_t s = stream_of(d);
+  int rc = ENVG_OK;
+  if (!(flags & ENVG_DEVICE_PTRS)) {
+    const size_t so = (cb + 255) & ~size_t(255), zo = so + ng * 4;
+    if (cudaMalloc(reinterpret_cast<void**>(&raw), zo + ng) != cudaSuccess) {
+      cudaGetLastError();
+      cudaFree(dst);
+      return fail(ENVG_ERR_OOM, "4-bit weight staging of %zu bytes failed", zo + ng);
+    }
+    cudaError_t e = cudaMemcpyAsync(raw, codes, cb, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(raw + so, scales, ng * 4, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess && zeros) e = cudaMemcpyAsync(raw + zo, zeros, ng, cudaMemcpyHostToDevice, s);
+    if (e != cudaSuccess) rc = fail(ENVG_ERR_CUDA, "weight_upload_q4: copy failed: %s", cudaGetErrorString(e));
+    d->st.h2d_bytes += (double)cb + 4.0 * ng + (zeros ? (double)ng : 0.0);
+    codes = raw, scales = reinterpret_cast<const float*>(raw + so), zeros = zeros ? raw + zo : nullptr;
+  }
+  if (rc == ENVG_OK) {
+    k_q4_pack<<<(unsigned)blocks, 256, 0, s>>>(v, dst, codes, scales, zeros, d->d_status);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) rc = fail(ENVG_ERR_CUDA, "k_q4_pack launch failed: %s", cudaGetErrorString(e));
+    d->st.kernel_launches++;
+  }
+  const int rs = sync_and_check(d);
+  if (rc == ENVG_OK) rc = rs;
+  if (raw) cudaFree(raw);
+  if (rc != ENVG_OK) {
+    cudaFree(dst);
+    return rc;
+  }
+  v.base = dst;
+  envg_q4weight w = new envg_q4weight_s{};
+  w->magic = Q4_MAGIC, w->dev = d->id, w->d = dst, w->bytes = bytes, w->layout = layout_flags, w->v = v;
+  d->st.weight_bytes += bytes;
+  *out = w;
+  return ENVG_OK;
+}
+
+int envg_q4weight_free(envg_q4weight w) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!w || w->magic != Q4_MAGIC) return fail(ENVG_ERR_STATE, "invalid or already freed 4-bit weight handle");
+  Dev* d = (w->dev >= 0 && w->dev < 64 && g_dev[w->dev].ready) ? &g_dev[w->dev] : nullptr;
+  if (d) cudaStreamSynchronize(stream_of(d));
+  cudaFree(w->d);  // waits for work on other streams that still reads it
+  if (d) d->st.weight_bytes -= std::min<uint64_t>(d->st.weight_bytes, w->bytes);
+  w->magic = 0;
+  delete w;
+  return ENVG_OK;
+}
+
+int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4weight W, const float* bias, int64_t M,
+                   int64_t K, int64_t N, int epilogue, const float* gate, int flags) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  ENVG_TRY(check_q4(d, W));
+  if (K != W->v.K || N != W->v.N)
+    return fail(ENVG_ERR_ARG, "linear_q4: [K=%lld, N=%lld] does not match the weight [N=%lld, K=%lld]", (long long)K,
+                (long long)N, (long long)W->v.N, (long long)W->v.K);
+  const bool gu = W->layout == ENVG_LAYOUT_GATE_UP;
+  if ((epilogue == ENVG_EPI_SILU_GATE) != gu)
+    return fail(ENVG_ERR_ARG, "linear_q4: SILU_GATE goes with (and only with) a GATE_UP weight");
+  if (epilogue != ENVG_EPI_NONE && epilogue != ENVG_EPI_BIAS && epilogue != ENVG_EPI_SILU_GATE &&
+      epilogue != ENVG_EPI_GATED_RESIDUAL)
+    return fail(ENVG_ERR_ARG, "linear_q4: epilogue %d not valid for a linear", epilogue);
+  if (epilogue == ENVG_EPI_BIAS && !bias) return fail(ENVG_ERR_ARG, "linear_q4: BIAS epilogue without bias");
+  if (epilogue == ENVG_EPI_GATED_RESIDUAL && !gate) return fail(ENVG_ERR_ARG, "linear_q4: GATED_RESIDUAL without gate");
+  if (M < 0 || M > 65535) return fail(ENVG_ERR_ARG, "linear_q4: M=%lld outside [0, 65535]", (long long)M);
+  const int64_t n_out = gu ? N / 2 : N;
+  if (M == 0) return ENVG_OK;
+  if (ldx < K || ldd < n_out) return fail(ENVG_ERR_ARG, "linear_q4: a row stride is shorter than its row");
+  if (!dst || !x) return fail(ENVG_ERR_ARG, "linear_q4: dst or x is NULL");
+  if ((const void*)dst == (const void*)x) return fail(ENVG_ERR_ARG, "linear_q4: dst aliases x");
+  Q4Args a{};
+  a.w = W->v;
+  a.x = x, a.dst = dst, a.ldx = ldx, a.ldd = ldd, a.M = (int)M;
+  a.mode = gu ? Q4_SILU_GATE : epilogue == ENVG_EPI_GATED_RESIDUAL ? Q4_GATED_RES : Q4_PLAIN;
+  a.bias = bias;
+  a.gate = a.mode == Q4_GATED_RES ? gate : nullptr;
+  LmStage st(d);
+  const bool devp = (flags & ENVG_DEVICE_PTRS) != 0;
+  int iy = 0;
+  if (!devp) {
+    const int ix = st.add(M * K * 4);
+    iy = st.add(M * n_out * 4);
+    const int ib = st.add(N * 4), ig = st.add(N * 4);
+    ENVG_TRY(st.commit());
+    ENVG_TRY(st.in(ix, x, ldx, M, K));
+    if (a.mode == Q4_GATED_RES) ENVG_TRY(st.in(iy, dst, ldd, M, n_out));
+    if (bias) ENVG_TRY(st.in(ib, bias, N, 1, N));
+    if (a.gate) ENVG_TRY(st.in(ig, gate, N, 1, N));
+    a.x = st.p<float>(ix), a.dst = st.p<float>(iy), a.ldx = K, a.ldd = n_out;
+    a.bias = bias ? st.p<float>(ib) : nullptr;
+    a.gate = a.gate ? st.p<float>(ig) : nullptr;
+  }
+  ENVG_TRY(launch_q4(d, a));
+  d->st.flops += 2.0 * (double)M * (double)N * (double)K;
+  if (!devp) ENVG_TRY(st.out(iy, dst, ldd, M, n_out));
+  return finish_call(d, flags);
+}
+
+int envg_qk_norm_rope(float* q_dst, int64_t ldqd, float* k_dst, int64_t ldkd, const float* q, int64_t ldq,
+                      const float* k, int64_t ldk, const float* q_weight, const float* k_weight, const float* cos_table,
+                      const float* sin_table, int64_t table_rows, const int32_t* positions, int64_t pos0, int64_t tokens,
+                      int heads, int kv_heads, int head_dim, float eps, int interleaved, int flags) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  if (head_dim < 8 || head_dim > 256 || head_dim % 8)
+    return fail(ENVG_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d (a multiple of 8 up to 256)", head_dim);
+  if (tokens < 0 || heads < 0 || kv_heads < 0 || heads > 65535 || kv_heads > 65535)
+    return fail(ENVG_ERR_ARG, "qk_norm_rope: %lld tokens, %d + %d heads", (long long)tokens, heads, kv_heads);
+  if (!(eps >= 0.0f)) return fail(ENVG_ERR_ARG, "qk_norm_rope: eps must not be negative");
+  if ((cos_table == nullptr) != (sin_table == nullptr)) return fail(ENVG_ERR_ARG, "qk_norm_rope: cos and sin go together");
+  if (tokens == 0 || heads + kv_heads == 0) return ENVG_OK;
+  if (tokens > INT32_MAX) return fail(ENVG_ERR_ARG, "qk_norm_rope: %lld tokens are too many", (long long)tokens);
+  const int64_t wq = (int64_t)heads * head_dim, wk = (int64_t)kv_heads * head_dim;
+  if ((heads && (!q || !q_dst)) || (kv_heads && (!k || !k_dst))) return fail(ENVG_ERR_ARG, "qk_norm_rope: NULL operand");
+  if ((heads && (ldq < wq || ldqd < wq)) || (kv_heads && (ldk < wk || ldkd < wk)))
+    return fail(ENVG_ERR_ARG, "qk_norm_rope: a row stride is shorter than its heads x head_dim");
+  if (cos_table) {
+    if (table_rows <= 0) return fail(ENVG_ERR_ARG, "qk_norm_rope: empty position table");
+    if (!positions && (pos0 < 0 || pos0 + tokens > table_rows))
+      return fail(ENVG_ERR_ARG, "qk_norm_rope: positions %lld..%lld outside the table's %lld rows", (long long)pos0,
+                  (long long)(pos0 + tokens - 1), (long long)table_rows);
+    if (positions && !(flags & ENVG_DEVICE_PTRS))
+      for (int64_t i = 0; i < tokens; ++i)
+        if (positions[i] < 0 || positions[i] >= table_rows)
+          return fail(ENVG_ERR_ARG, "qk_norm_rope: positions[%lld] = %d outside the table's %lld rows", (long long)i,
+                      positions[i], (long long)table_rows);
+  }
+  NormRopeArgs a{};
+  a.qd = q_dst, a.kd = k_dst, a.q = q, a.k = k, a.ldqd = ldqd, a.ldkd = ldkd, a.ldq = ldq, a.ldk = ldk;
+  a.wq = q_weight, a.wk = k_weight, a.cos = cos_table, a.sin = sin_table, a.table_rows = table_rows;
+  a.positions = positions, a.pos0 = pos0, a.tokens = tokens;
+  a.heads = heads, a.kv_heads = kv_heads, a.hd = head_dim, a.eps = eps, a.interleaved = interleaved ? 1 : 0;
+  a.status = d->d_status;
+  LmStage st(d);
+  const bool devp = (flags & ENVG_DEVICE_PTRS) != 0;
+  int iq = 0, ik = 0;
+  if (!devp) {
+    const int64_t half = head_dim / 2;
+    // with pos0 only its rows of the tables travel
+    const int64_t r0 = positions ? 0 : pos0, rows = positions ? table_rows : tokens;
+    iq = st.add(tokens * wq * 4), ik = st.add(tokens * wk * 4);
+    const int iwq = st.add(head_dim * 4), iwk = st.add(head_dim * 4);
+    const int ic = st.add(cos_table ? rows * half * 4 : 0), is = st.add(cos_table ? rows * half * 4 : 0);
+    const int ip = st.add(positions ? tokens * 4 : 0);
+    ENVG_TRY(st.commit());
+    if (heads) ENVG_TRY(st.in(iq, q, ldq, tokens, wq));
+    if (kv_heads) ENVG_TRY(st.in(ik, k, ldk, tokens, wk));
+    if (q_weight) ENVG_TRY(st.in(iwq, q_weight, head_dim, 1, head_dim));
+    if (k_weight) ENVG_TRY(st.in(iwk, k_weight, head_dim, 1, head_dim));
+    if (cos_table) {
+      ENVG_TRY(st.in(ic, cos_table + r0 * half, half, rows, half));
+      ENVG_TRY(st.in(is, sin_table + r0 * half, half, rows, half));
+      a.cos = st.p<float>(ic), a.sin = st.p<float>(is), a.table_rows = rows, a.pos0 = 0;
+    }
+    if (positions) ENVG_TRY(st.in(ip, positions, tokens, 1, tokens));
+    a.q = a.qd = st.p<float>(iq), a.k = a.kd = st.p<float>(ik);
+    a.ldq = a.ldqd = wq, a.ldk = a.ldkd = wk;
+    a.wq = q_weight ? st.p<float>(iwq) : nullptr, a.wk = k_weight ? st.p<float>(iwk) : nullptr;
+    a.positions = positions ? st.p<int32_t>(ip) : nullptr;
+  }
+  a.vec = (!heads || (f4_ok(a.q, a.ldq) && f4_ok(a.qd, a.ldqd))) && (!kv_heads || (f4_ok(a.k, a.ldk) && f4_ok(a.kd, a.ldkd))) &&
+          f4_ok(a.wq, 0) && f4_ok(a.wk, 0) && f4_ok(a.cos, 0) && f4_ok(a.sin, 0);
+  ENVG_TRY(launch_norm_rope(d, a));
+  if (!devp) {
+    if (heads) ENVG_TRY(st.out(iq, q_dst, ldqd, tokens, wq));
+    if (kv_heads) ENVG_TRY(st.out(ik, k_dst, ldkd, tokens, wk));
+  }
+  return finish_call(d, flags);
+}
+
+int envg_kv4_create(int64_t pages, int page_size, int kv_heads, int head_dim, envg_kv4* out) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!out) return fail(ENVG_ERR_ARG, "out handle pointer is NULL");
+  *out = nullptr;
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  if (head_dim != 64 && head_dim != 128) return fail(ENVG_ERR_UNSUPPORTED, "kv4_create: head_dim %d (64 or 128)", head_dim);
+  if (pages <= 0 || pages > INT32_MAX || kv_heads <= 0 || kv_heads > 1024)
+    return fail(ENVG_ERR_ARG, "kv4_create: %lld pages, %d kv heads", (long long)pages, kv_heads);
+  if (page_size < KV_TILE || page_size > 1024 || page_size % KV_TILE)
+    return fail(ENVG_ERR_ARG, "kv4_create: page_size %d (a multiple of %d up to 1024)", page_size, KV_TILE);
+  const size_t bytes = (size_t)pages * kv_heads * (page_size / KV_TILE) * kv_tile_bytes(head_dim);
+  uint8_t* p = nullptr;
+  if (cudaMalloc(reinterpret_cast<void**>(&p), bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ENVG_ERR_OOM, "cache allocation of %zu bytes failed", bytes);
+  }
+  cudaError_t e = cudaMemsetAsync(p, 0, bytes, stream_of(d));
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream_of(d));
+  if (e != cudaSuccess) {
+    cudaFree(p);
+    return fail(ENVG_ERR_CUDA, "kv4_create: clearing the cache failed: %s", cudaGetErrorString(e));
+  }
+  envg_kv4 c = new envg_kv4_s{};
+  c->magic = KV4_MAGIC, c->dev = d->id, c->d = p, c->bytes = bytes;
+  c->pages = pages, c->page_size = page_size, c->kv_heads = kv_heads, c->head_dim = head_dim;
+  *out = c;
+  return ENVG_OK;
+}
+
+int envg_kv4_free(envg_kv4 c) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!c || c->magic != KV4_MAGIC) return fail(ENVG_ERR_STATE, "invalid or already freed cache handle");
+  Dev* d = (c->dev >= 0 && c->dev < 64 && g_dev[c->dev].ready) ? &g_dev[c->dev] : nullptr;
+  if (d) cudaStreamSynchronize(stream_of(d));
+  cudaFree(c->d);  // waits for work on other streams that still uses it
+  c->magic = 0;
+  delete c;
+  return ENVG_OK;
+}
+
+int envg_kv4_append(envg_kv4 cache, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* table,
+                    int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int flags) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  return kv4_rows(cache, const_cast<float*>(k), ldk, const_cast<float*>(v), ldv, table, table_stride, ctx_lens, batch, q_len,
+                  flags, false);
+}
+
+int envg_kv4_read(envg_kv4 cache, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table, int64_t table_stride,
+                  const int32_t* ctx_lens, int batch, int q_len, int flags) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  return kv4_rows(cache, k, ldk, v, ldv, table, table_stride, ctx_lens, batch, q_len, flags, true);
+}
+
+int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, envg_kv4 cache, const int32_t* table,
+                       int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int max_ctx, int heads,
+                       int window, int sinks, float scale, int flags) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  Dev* d;
+  ENVG_TRY(lm_dev(&d));
+  if (window < 0 || sinks < 0) return fail(ENVG_ERR_ARG, "attention_kv4: window %d, sinks %d", window, sinks);
+  ENVG_TRY(check_kv_call(d, cache, table, table_stride, ctx_lens, batch, q_len, window > 0 ? window - 1 : INT32_MAX,
+                         window > 0 ? sinks : 0, flags, "attention_kv4"));
+  if (heads <= 0 || heads % cache->kv_heads || heads > 65535)
+    return fail(ENVG_ERR_ARG, "attention_kv4: %d heads over %d kv heads", heads, cache->kv_heads);
+  if (max_ctx < 0) return fail(ENVG_ERR_ARG, "attention_kv4: max_ctx %d", max_ctx);
+  if (!(scale > 0.0f)) return fail(ENVG_ERR_ARG, "attention_kv4: scale must be positive");
+  const int64_t rows = (int64_t)batch * q_len, width = (int64_t)heads * cache->head_dim;
+  if (rows == 0) return ENVG_OK;
+  if (!dst || !q) return fail(ENVG_ERR_ARG, "attention_kv4: dst or q is NULL");
+  if (ldo < width || ldq < width) return fail(ENVG_ERR_ARG, "attention_kv4: a row stride is shorter than heads x head_dim");
+  if ((const void*)dst == (const void*)q) return fail(ENVG_ERR_ARG, "attention_kv4: dst aliases q");
+  LmStage st(d);
+  const bool devp = (flags & ENVG_DEVICE_PTRS) != 0;
+  KvAttnArgs a{};
+  a.q = q, a.out = dst, a.ldq = ldq, a.ldo = ldo;
+  int io = 0;
+  if (!devp) {
+    const int iq = st.add(rows * width * 4), it = st.add(batch * table_stride * 4), il = st.add((size_t)batch * 4);
+    io = st.add(rows * width * 4);
+    ENVG_TRY(st.commit());
+    ENVG_TRY(st.in(iq, q, ldq, rows, width));
+    ENVG_TRY(st.in(it, table, table_stride, batch, table_stride));
+    ENVG_TRY(st.in(il, ctx_lens, batch, 1, batch));
+    a.q = st.p<float>(iq), a.out = st.p<float>(io), a.ldq = a.ldo = width;
+    table = st.p<int32_t>(it), ctx_lens = st.p<int32_t>(il);
+  }
+  a.c = kv_view(d, cache, table, table_stride, ctx_lens);
+  a.batch = batch, a.q_len = q_len, a.heads = heads, a.hd = cache->head_dim;
+  a.window = window, a.sinks = sinks;
+  a.sl2 = scale * 1.4426950408889634f;
+  const int64_t most = table_stride * cache->page_size;
+  ENVG_TRY(launch_kv4_attn(d, a, (int)(max_ctx > 0 ? std::min<int64_t>(max_ctx, most) : most)));
+  if (!devp) ENVG_TRY(st.out(io, dst, ldo, rows, width));
+  return finish_call(d, flags);
+}
+
+}  // extern "C"

@@ -112,6 +112,18 @@ def lib():
         L.envg_vae_resblock.argtypes = [_vp, _vp, ctypes.POINTER(ResBlockDesc), _ci, _ci, _ci, _ci, _ci]
         L.envg_sgemm.argtypes = [_ci, _ci, _ci, _i64, _i64, _i64, ctypes.c_float, _vp, _i64, _vp, _i64,
                                  ctypes.c_float, _vp, _i64]
+        L.envg_quantize_q4.argtypes = [_vp, _vp, _i64, _i64, _ci, _vp, _vp, _vp]
+        L.envg_weight_upload_q4.argtypes = [_vp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, ctypes.POINTER(_vp)]
+        L.envg_q4weight_free.argtypes = [_vp]
+        L.envg_linear_q4.argtypes = [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _vp, _ci]
+        L.envg_qk_norm_rope.argtypes = [_vp, _i64] * 4 + [_vp] * 4 + [_i64, _vp, _i64, _i64, _ci, _ci, _ci,
+                                                                      ctypes.c_float, _ci, _ci]
+        L.envg_kv4_create.argtypes = [_i64, _ci, _ci, _ci, ctypes.POINTER(_vp)]
+        L.envg_kv4_free.argtypes = [_vp]
+        L.envg_kv4_append.argtypes = [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _ci, _ci, _ci]
+        L.envg_kv4_read.argtypes = [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _ci, _ci, _ci]
+        L.envg_attention_kv4.argtypes = [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _ci, _ci, _ci, _ci, _ci, _ci,
+                                         ctypes.c_float, _ci]
         L.envg_set_stream.argtypes = [_vp]
         L.envg_get_stats.argtypes = [ctypes.POINTER(Stats)]
         L.envg_set_wait_cap_ns.argtypes = [ctypes.c_uint64]
@@ -558,6 +570,237 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
         _host_f32(a, "sgemm operand")
     return _check(lib().envg_sgemm(order, transA, transB, M, N, K, alpha, A.ctypes.data, lda, B.ctypes.data, ldb,
                                    beta, C.ctypes.data, ldc))
+
+
+# ---------------------------------------------------------------------------------------------
+# Language-model decode operators: 4-bit linears, q/k norm + rotation, the paged 4-bit cache and
+# its attention.  Matrices may be row-strided views (columns adjacent): a slice of a fused
+# projection's output is passed as it is.
+# ---------------------------------------------------------------------------------------------
+
+def _device_of(arrays):
+    """DEVICE_PTRS (and the library put on torch's current stream) for CUDA tensors, HOST_PTRS for
+    numpy arrays; never mixed."""
+    torch_side = None
+    for a in arrays:
+        if a is None:
+            continue
+        t = not isinstance(a, np.ndarray)
+        if torch_side is None:
+            torch_side = t
+        elif torch_side != t:
+            raise TypeError("operands must be all numpy (host) or all torch CUDA tensors (device)")
+    if not torch_side:
+        return HOST_PTRS
+    import torch
+
+    for a in arrays:
+        if a is not None and not (isinstance(a, torch.Tensor) and a.is_cuda):
+            raise TypeError("device operands must be CUDA tensors")
+    if _follow_torch_stream:
+        h = torch.cuda.current_stream().cuda_stream
+        lib().envg_set_stream(h if h else CUDA_STREAM_LEGACY)
+    return DEVICE_PTRS
+
+
+_DTYPE_NAMES = {"float32": ("float32", "torch.float32"), "int32": ("int32", "torch.int32"),
+                "uint8": ("uint8", "torch.uint8")}
+
+
+def _typed(a, dtype, name):
+    if str(a.dtype) not in _DTYPE_NAMES[dtype]:
+        raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
+
+
+def _matrix(a, rows, cols, name, dtype="float32"):
+    """(pointer, row stride in elements) of a 2-D array [rows, >= cols] whose columns are adjacent."""
+    if a is None:
+        return None, 0
+    _typed(a, dtype, name)
+    if a.ndim != 2 or a.shape[0] != rows or a.shape[1] < cols:
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(a.shape)}")
+    if isinstance(a, np.ndarray):
+        st, ptr = [s // a.itemsize for s in a.strides], a.ctypes.data
+    else:
+        st, ptr = a.stride(), a.data_ptr()
+    if a.shape[1] > 1 and st[1] != 1:
+        raise TypeError(f"{name}: columns must be adjacent")
+    ld = st[0] if rows > 1 else max(a.shape[1], 1)
+    if ld < cols:
+        raise TypeError(f"{name}: rows overlap")
+    return ptr, ld
+
+
+def _vector(a, n, name, dtype="float32"):
+    if a is None:
+        return None
+    _typed(a, dtype, name)
+    if a.ndim != 1 or a.shape[0] != n:
+        raise ValueError(f"{name}: expected [{n}], got {list(a.shape)}")
+    if isinstance(a, np.ndarray):
+        if n > 1 and a.strides[0] != a.itemsize:
+            raise TypeError(f"{name}: must be contiguous")
+        return a.ctypes.data
+    if n > 1 and a.stride(0) != 1:
+        raise TypeError(f"{name}: must be contiguous")
+    return a.data_ptr()
+
+
+def _flags(mode, sync):
+    return mode | ASYNC if mode == DEVICE_PTRS and not sync else mode
+
+
+def quantize_q4(w, group=128):
+    """(codes, scales, zeros) of W[N, K] (float32, or uint16 bf16 bits) in 4 bits: envg_quantize_q4."""
+    w = np.ascontiguousarray(w)
+    if w.ndim != 2 or w.dtype not in (np.dtype(np.uint16), np.dtype(np.float32)):
+        raise TypeError("weight must be a 2-D array of uint16 (bf16 bits) or float32")
+    N, K = w.shape
+    codes = np.zeros((N, (K + 1) // 2), np.uint8)
+    groups = -(-K // group) if group > 0 else 0
+    scales, zeros = np.zeros((N, groups), np.float32), np.zeros((N, groups), np.uint8)
+    bits = w.dtype == np.uint16
+    _check(lib().envg_quantize_q4(w.ctypes.data if bits else None, None if bits else w.ctypes.data, N, K, group,
+                                  codes.ctypes.data, scales.ctypes.data, zeros.ctypes.data))
+    return codes, scales, zeros
+
+
+class Q4Weight:
+    """A device-resident 4-bit weight: W[n, k] = (c - z) s per group of ``group`` columns.
+
+    ``codes`` [N, ceil(K / 2)] uint8 (even column in the low nibble), ``scales`` float32 and ``zeros``
+    uint8 (or None: 8) [N, ceil(K / group)], all numpy or all CUDA tensors; ``quantize_q4`` makes them
+    from a bf16 or float32 weight."""
+
+    def __init__(self, codes, scales, zeros=None, K=None, group=128, layout=LAYOUT_PLAIN):
+        self.h = None
+        mode = _device_of((codes, scales, zeros))
+        self.N = codes.shape[0]
+        self.K = 2 * codes.shape[1] if K is None else int(K)
+        if codes.ndim != 2 or codes.shape[1] != (self.K + 1) // 2:
+            raise ValueError(f"codes: expected [N, {(self.K + 1) // 2}], got {list(codes.shape)}")
+        if group not in (32, 64, 128):
+            raise ValueError(f"group {group}: 32, 64 or 128")
+        groups = -(-self.K // group)
+        ptrs = []
+        for a, n, dt, what in ((codes, codes.shape[1], "uint8", "codes"), (scales, groups, "float32", "scales"),
+                               (zeros, groups, "uint8", "zeros")):
+            p, ld = _matrix(a, self.N, n, what, dt)
+            if a is not None and (a.shape[1] != n or ld != n):
+                raise ValueError(f"{what}: expected a contiguous [{self.N}, {n}], got {list(a.shape)}")
+            ptrs.append(p)
+        h = _vp()
+        _check(lib().envg_weight_upload_q4(*ptrs, self.N, self.K, group, layout, mode, ctypes.byref(h)))
+        self.group, self.layout, self.h = group, layout, h
+
+    def free(self):
+        if self.h is not None and self.h.value:
+            _check(lib().envg_q4weight_free(self.h))
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def linear_q4(dst, x, W, bias=None, epilogue=None, gate=None, sync=True):
+    """dst = epilogue(x . W^T) for a Q4Weight: envg_linear_q4.  x [M, K]; dst [M, N] (N/2 for SILU_GATE)."""
+    if epilogue is None:
+        epilogue = EPI_SILU_GATE if W.layout == LAYOUT_GATE_UP else (EPI_BIAS if bias is not None else EPI_NONE)
+    mode = _device_of((dst, x, bias, gate))
+    M, N = x.shape[0], W.N
+    px, ldx = _matrix(x, M, W.K, "x")
+    if x.shape[1] != W.K:
+        raise ValueError(f"x: expected {W.K} columns, got {x.shape[1]}")
+    py, ldd = _matrix(dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, "dst")
+    return _check(lib().envg_linear_q4(py, ldd, px, ldx, W.h, _vector(bias, N, "bias"), M, W.K, N, epilogue,
+                                       _vector(gate, N, "gate"), _flags(mode, sync)))
+
+
+def qk_norm_rope(q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, heads, kv_heads, head_dim=128, positions=None,
+                 pos0=0, eps=1e-6, interleaved=False, sync=True):
+    """RMS norm of every query and key head, then the position rotation: envg_qk_norm_rope.
+
+    q [T, heads * hd], k [T, kv_heads * hd] (either may be None with 0 heads); cos / sin
+    [P, hd / 2] or None (the norm alone); positions int32 [T], or None for pos0 + t."""
+    mode = _device_of((q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, positions))
+    T = q.shape[0] if q is not None else k.shape[0]
+    (pqd, lqd), (pq, lq) = _matrix(q_dst, T, heads * head_dim, "q_dst"), _matrix(q, T, heads * head_dim, "q")
+    (pkd, lkd), (pk, lk) = _matrix(k_dst, T, kv_heads * head_dim, "k_dst"), _matrix(k, T, kv_heads * head_dim, "k")
+    rows = cos.shape[0] if cos is not None else 0
+    tables = []
+    for a, what in ((cos, "cos"), (sin, "sin")):
+        p, ld = _matrix(a, rows, head_dim // 2, what)
+        if a is not None and (a.shape[1] != head_dim // 2 or ld != head_dim // 2):
+            raise ValueError(f"{what}: expected a contiguous [{rows}, {head_dim // 2}], got {list(a.shape)}")
+        tables.append(p)
+    return _check(lib().envg_qk_norm_rope(pqd, lqd, pkd, lkd, pq, lq, pk, lk, _vector(q_weight, head_dim, "q_weight"),
+                                          _vector(k_weight, head_dim, "k_weight"), *tables, rows,
+                                          _vector(positions, T, "positions", "int32"), pos0, T, heads, kv_heads,
+                                          head_dim, eps, 1 if interleaved else 0, _flags(mode, sync)))
+
+
+def _table(table, ctx_lens, batch):
+    p, ld = _matrix(table, batch, 0, "table", "int32")
+    if batch > 1 and ld != table.shape[1]:
+        raise TypeError("table: must be contiguous")
+    return p, table.shape[1], _vector(ctx_lens, batch, "ctx_lens", "int32")
+
+
+class KV4Cache:
+    """A paged key/value cache in 4 bits: envg_kv4_create (``pages`` pages of ``page_size`` tokens).
+
+    ``table`` [B, P] int32 names the pages of each sequence in order, ``ctx_lens`` [B] int32 its
+    tokens, the ``q_len`` newest among them."""
+
+    def __init__(self, pages, page_size, kv_heads, head_dim=128):
+        self.h = None
+        h = _vp()
+        _check(lib().envg_kv4_create(pages, page_size, kv_heads, head_dim, ctypes.byref(h)))
+        self.pages, self.page_size, self.kv_heads, self.head_dim, self.h = pages, page_size, kv_heads, head_dim, h
+
+    def _rows(self, call, k, v, table, ctx_lens, q_len, sync):
+        mode = _device_of((k, v, table, ctx_lens))
+        B, width = ctx_lens.shape[0], self.kv_heads * self.head_dim
+        (pk, lk), (pv, lv) = _matrix(k, B * q_len, width, "k"), _matrix(v, B * q_len, width, "v")
+        pt, stride, pl = _table(table, ctx_lens, B)
+        return _check(call(self.h, pk, lk, pv, lv, pt, stride, pl, B, q_len, _flags(mode, sync)))
+
+    def append(self, k, v, table, ctx_lens, q_len=1, sync=True):
+        """Write the newest ``q_len`` tokens of each sequence; k, v [B * q_len, kv_heads * hd]: envg_kv4_append."""
+        return self._rows(lib().envg_kv4_append, k, v, table, ctx_lens, q_len, sync)
+
+    def read(self, k, v, table, ctx_lens, q_len=1, sync=True):
+        """The values held for the newest ``q_len`` tokens of each sequence, into k and v: envg_kv4_read."""
+        return self._rows(lib().envg_kv4_read, k, v, table, ctx_lens, q_len, sync)
+
+    def free(self):
+        if self.h is not None and self.h.value:
+            _check(lib().envg_kv4_free(self.h))
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def attention_kv4(dst, q, cache, table, ctx_lens, heads, q_len=1, max_ctx=0, window=0, sinks=0, scale=None, sync=True):
+    """Attention of the newest ``q_len`` tokens of each sequence over a KV4Cache: envg_attention_kv4.
+
+    q, dst [B * q_len, heads * hd]; causal, with ``window`` > 0 only the last ``window`` tokens and the
+    first ``sinks``; ``max_ctx`` (0: unknown) is the largest of ctx_lens and only plans the launch."""
+    mode = _device_of((dst, q, table, ctx_lens))
+    B, width = ctx_lens.shape[0], heads * cache.head_dim
+    (po, lo), (pq, lq) = _matrix(dst, B * q_len, width, "dst"), _matrix(q, B * q_len, width, "q")
+    pt, stride, pl = _table(table, ctx_lens, B)
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    return _check(lib().envg_attention_kv4(po, lo, pq, lq, cache.h, pt, stride, pl, B, q_len, max_ctx, heads, window,
+                                           sinks, scale, _flags(mode, sync)))
 
 
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,86 @@
+"""CPU: the host side of the language-model decode operators: 4-bit rounding of weights, argument
+checks of the binding, status codes before envg_init."""
+import numpy as np
+import pytest
+
+from invision_b200 import envg
+from oracle import oracle as O
+from tests import lm_ref as R
+
+
+@pytest.mark.parametrize("N,K,group", [(1, 1, 32), (5, 63, 64), (3, 300, 128), (7, 257, 32)])
+def test_quantize_q4_within_half_a_step(N, K, group):
+    rng = np.random.default_rng(K)
+    w = (0.05 * rng.standard_normal((N, K)) + 0.02).astype(np.float32)
+    w[0, : K // 3] = 0.0
+    codes, scales, zeros = envg.quantize_q4(w, group)
+    held = R.q4_weight(codes, scales, zeros, K, group)
+    step = scales[:, np.arange(K) // group]
+    # half a step, and half a step of the zero point's own rounding where a value would leave 0..15
+    assert (np.abs(held - w) <= step * (1.0 + 1e-5)).all()
+    assert np.abs(held - w).mean() <= 0.3 * step.mean()
+    assert (held[w == 0] == 0).all() and zeros.max() <= 15
+    bits = O.f32_to_bf16_rne(w)
+    c2, s2, z2 = envg.quantize_q4(bits, group)
+    c3, s3, z3 = envg.quantize_q4((bits.astype(np.uint32) << 16).view(np.float32), group)
+    assert np.array_equal(c2, c3) and np.array_equal(s2, s3) and np.array_equal(z2, z3)
+
+
+def test_quantize_q4_edges():
+    codes, scales, zeros = envg.quantize_q4(np.zeros((2, 40), np.float32), 32)
+    assert (R.q4_weight(codes, scales, zeros, 40, 32) == 0).all()
+    w = np.array([[3e38, -3e38, 1.0]], np.float32)  # a span beyond fp32
+    codes, scales, zeros = envg.quantize_q4(w, 32)
+    assert np.isfinite(scales).all() and np.abs(R.q4_weight(codes, scales, zeros, 3, 32) - w).max() <= scales.max()
+    for bad in (np.nan, np.inf):
+        with pytest.raises(envg.EnvgError, match="not finite"):
+            envg.quantize_q4(np.full((1, 3), bad, np.float32), 32)
+    with pytest.raises(envg.EnvgError, match="group"):
+        envg.quantize_q4(np.zeros((1, 3), np.float32), 16)
+    with pytest.raises(TypeError):
+        envg.quantize_q4(np.zeros((1, 3), np.float64))
+
+
+def test_held_values_stay_near():
+    """The cache's rounding as the tests state it: within half a step plus fp16 of the minimum."""
+    rng = np.random.default_rng(0)
+    x = (rng.standard_normal((50, 128)) * 3 + 1).astype(np.float32)
+    y = R.kv_hold(x)
+    g = x.reshape(50, 2, 64)
+    step = (g.max(-1) - g.min(-1)) / 15
+    assert (np.abs(y.reshape(g.shape) - g) <= step[..., None] * 0.51 + np.abs(g).max() * 2.0 ** -10).all()
+
+
+def test_binding_refuses_before_any_call():
+    f = np.zeros((2, 128), np.float32)
+    with pytest.raises(ValueError, match="codes"):
+        envg.Q4Weight(np.zeros((4, 10), np.uint8), np.zeros((4, 1), np.float32), K=64)
+    with pytest.raises(ValueError, match="group"):
+        envg.Q4Weight(np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.float32), group=256)
+    with pytest.raises(TypeError, match="scales"):
+        envg.Q4Weight(np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.float64), group=64)
+    with pytest.raises(TypeError, match="adjacent"):
+        envg._matrix(f[:, ::2], 2, 64, "x")
+    with pytest.raises(TypeError, match="overlap"):
+        envg._matrix(np.lib.stride_tricks.as_strided(f, (2, 64), (4, 4)), 2, 64, "x")
+    assert envg._matrix(f[:, 3:60], 2, 57, "x")[1] == 128
+
+
+def test_calls_before_init_return_state_error():
+    try:
+        import torch
+
+        if torch.cuda.is_available():
+            pytest.skip("checks the uninitialised state")
+    except ImportError:
+        pass
+    L = envg.lib()
+    assert L.envg_linear_q4(None, 0, None, 0, None, None, 1, 1, 1, 0, None, 0) == envg.ERR_STATE
+    assert L.envg_qk_norm_rope(*([None, 0] * 4), None, None, None, None, 0, None, 0, 1, 1, 0, 128, 1e-6, 0, 0) == envg.ERR_STATE
+    for go in (lambda: envg.KV4Cache(4, 16, 1, 128),
+               lambda: envg.Q4Weight(np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.float32), group=64)):
+        with pytest.raises(envg.EnvgError) as e:
+            go()
+        assert e.value.code == envg.ERR_STATE
+    assert L.envg_kv4_free(None) == envg.ERR_STATE and L.envg_q4weight_free(None) == envg.ERR_STATE
+    assert L.envg_weight_upload_q4(None, None, None, 1, 1, 32, 0, 0, None) == envg.ERR_ARG
