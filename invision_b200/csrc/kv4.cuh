@@ -6,10 +6,12 @@
 // group holds m = fp16(min x), s = fp16((max x - min x) / 15) and codes
 // c = clamp(rint((x - m) / s), 0, 15); it stands for the values m + s c.  The codes of 16 tokens
 // lie together in one tile, tiles of a (page, kv head) follow one another:
-//   tile = K codes [16][hd / 2 bytes] | V codes [16][hd / 2 bytes] | scales [16][2][hd / 64] half2 (s, m)
+//   tile = K codes [16][hd / 2 bytes] | V codes [16][hd / 2 bytes] | scales [16][K s.., K m.., V s.., V m..] fp16
 // A 32-bit word holds 8 consecutive channels 64 gi + 8 r + j (nibble j, r = 0..7).  In a K row,
 // word (gi, r) stands at byte (r / 2) * hd / 8 + (2 gi + r % 2) * 4, so that lane t of a quad
 // finds the words of its 16-channel pieces side by side; in a V row at byte r * hd / 16 + 4 gi.
+// Token 8 a + 4 b + c of a tile takes K row 8 a + 2 c + b: the scores that lane t of a quad then
+// gets are those of tokens t, t + 4, t + 8, t + 12, whose V rows four lanes read side by side.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -156,9 +158,17 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(const NormRopeArgs a) {
 // Eight threads hold one group of 64 channels, eight consecutive channels (one word of codes)
 // each; the group's minimum and maximum are one shuffle tree.  Every rounding is IEEE (no
 // contraction), so equal inputs give equal codes on any path that uses the formula.
-ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) { return tok * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4; }
+ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) {
+  const int row = (tok & 8) + 2 * (tok & 3) + ((tok >> 2) & 1);
+  return row * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4;
+}
 ENVG_DEV uint32_t kv_v_word(int hd, int tok, int gi, int r) { return KV_TILE * (hd / 2) + tok * (hd / 2) + r * (hd / 16) + 4 * gi; }
-ENVG_DEV uint32_t kv_scale_at(int hd, int tok, int v, int gi) { return KV_TILE * hd + (tok * 2 + v) * (hd / KV_GROUP) * 4 + gi * 4; }
+// Byte offset of the scale of (token, K or V, group); its minimum stands hd / 64 halves further.
+ENVG_DEV uint32_t kv_scale_at(int hd, int tok, int v, int gi) { return KV_TILE * hd + tok * (hd / 8) + v * (hd / 16) + 2 * gi; }
+ENVG_DEV float2 kv_scale(const uint8_t* tile, uint32_t at, int hd) {
+  const __half* p = reinterpret_cast<const __half*>(tile + at);
+  return make_float2(__half2float(p[0]), __half2float(p[hd / KV_GROUP]));
+}
 
 struct KvRowsArgs {
   Kv4View c;
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
     float x[8] = {};
     if (tile) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + word_at);
-      const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(tile + scale_at));
+      const float2 sm = kv_scale(tile, scale_at, a.hd);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = fmaf(sm.x, (float)((w >> (4 * j)) & 15u), sm.y);
     }
@@ -221,8 +231,8 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
     if (any) lo = hi = __int_as_float(0x7fc00000);  // a group with a NaN holds NaN
     const float low = lo < -KV_HALF_MAX ? -KV_HALF_MAX : lo > KV_HALF_MAX ? KV_HALF_MAX : lo;
     const float step = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    const __half2 sm = __halves2half2(__float2half_rn(step > KV_HALF_MAX ? KV_HALF_MAX : step), __float2half_rn(low));
-    const float s = __low2float(sm), m = __high2float(sm);
+    const __half hs = __float2half_rn(step > KV_HALF_MAX ? KV_HALF_MAX : step), hm = __float2half_rn(low);
+    const float s = __half2float(hs), m = __half2float(hm);
     uint32_t w = 0;
     if (s > 0.0f) {
 #pragma unroll
@@ -232,7 +242,10 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
       }
     }
     *reinterpret_cast<uint32_t*>(tile + word_at) = w;
-    if (r == 0) *reinterpret_cast<__half2*>(tile + scale_at) = sm;
+    if (r == 0) {
+      __half* p = reinterpret_cast<__half*>(tile + scale_at);
+      p[0] = hs, p[G] = hm;
+    }
   }
 }
 
@@ -247,55 +260,438 @@ struct KvAttnArgs {
   int64_t ldq, ldo;
   int batch, q_len, heads, hd, window, sinks;
   float sl2;  // softmax scale * log2 e
+  uint64_t wait_cap_ns;
 };
 
-// One warp per (row, head); lane l holds channels 8l..8l+7 (l < hd / 8).
-__global__ void __launch_bounds__(128) k_kv4_attn_simple(const KvAttnArgs a) {
+// k_kv4_attn: flash attention of up to eight query rows over one kv head's cached tokens.
+//
+// Mathematics.  The eight rows are (query token, head) pairs that read the same kv head.  A row's
+// score of token j is sum_g s_jg (q_g . c_jg) + m_jg sum(q_g) over its groups of 64 channels, and
+// its output sum_j p_j (s_jg (c_jg - 8) + (m_jg + 8 s_jg)).  Both products with codes run on the
+// tensor cores as m16n8k16 with fp16 operands and fp32 sums, exactly in the codes: a code is a
+// subnormal fp16 (c 2^-24, or 16 c 2^-24) for K, c - 8 for V (centred: the positive codes' sum
+// would be far larger than the outputs and cost its last bits).  q and p s are split into two
+// fp16 parts each, the high parts in rows 0..7 of the 16-row operand and the low parts in rows
+// 8..15, so that fp32 accuracy costs no further instruction; q is scaled by a power of two per
+// row, p s by the row maximum and by the largest s seen (both folded into the exponent).
+// The S accumulator's layout is the P operand's, so scores stay in their threads.
+//
+// Split.  Tokens are taken in units of two 16-token tiles, dealt out over the warps of a cluster
+// of CTAs (one cluster per sequence, kv head and eight rows).  Each warp runs a one-pass softmax
+// with its own ring of bulk copies; the warps' (max, sum, output) are joined in shared memory, the
+// CTAs' through distributed shared memory in rank order: no workspace, no atomics, one launch.
+ENVG_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+ENVG_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+ENVG_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+ENVG_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (x, y) as fp16 high parts and what they leave.
+ENVG_DEV void split_h2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 b = __half22float2(h);
+  hi = h2_bits(h);
+  lo = h2_bits(__floats2half2_rn(x - b.x, y - b.y));
+}
+ENVG_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+ENVG_DEV float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 4;
+constexpr int SITE_KVA_RING = 60;  // status[1] of a ring wait that ran out
+
+template <int HD>
+struct KvaSmem {
+  static constexpr int TILE = kv_tile_bytes(HD), STAGE = 2 * TILE;
+  static constexpr int RING = KVA_STAGES * STAGE;                  // per warp
+  static constexpr int BARS = KVA_WARPS * RING;                    // mbarriers
+  static constexpr int ABORT = BARS + KVA_WARPS * KVA_STAGES * 8;  // abort flag of the bounded waits
+  static constexpr int ML = ABORT + 16;                            // [warps + 1][max 8 | sum 8]
+  static constexpr int TOTAL = ML + (KVA_WARPS + 1) * 16 * 4;
+  // the rings are empty when the outputs of the warps are joined: [warp][8][HD], then the CTA's [8][HD]
+  static constexpr int OUT_LD = HD + 4;
+  static_assert((KVA_WARPS + 1) * 8 * OUT_LD * 4 <= BARS, "outputs fit the rings");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a) {
+  using S = KvaSmem<HD>;
+  constexpr int G = HD / KV_GROUP;  // groups per head
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t ring = sbase + warp * S::RING, bars = sbase + S::BARS + warp * KVA_STAGES * 8;
+  volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::ABORT);
+  float* ml = reinterpret_cast<float*>(smem + S::ML);
+  if (lane == 0)
+    for (int i = 0; i < KVA_STAGES; ++i) mbar_init(bars + 8 * i, 2);
+  if (threadIdx.x == 0) *abort_s = 0;
+  fence_mbar_init();
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31;
-  if (item >= (int64_t)a.batch * a.q_len * a.heads) return;
-  const int h = (int)(item % a.heads);
-  const int64_t row = item / a.heads;
-  const int b = (int)(row / a.q_len);
-  const int p = kv_len(a.c, b) - a.q_len + (int)(row % a.q_len);
-  const int kvh = h / (a.heads / a.c.kv_heads);
-  const bool on = lane < a.hd / 8;
-  const int gi = lane / 8, r = lane % 8;
-  float q[8] = {}, o[8] = {}, m = -INFINITY, l = 0.0f;
-  if (on)
-    for (int j = 0; j < 8; ++j) q[j] = a.q[row * a.ldq + (int64_t)h * a.hd + 8 * lane + j];
-  const int tile_bytes = kv_tile_bytes(a.hd);
-  for (int j = 0; j <= p; ++j) {
-    if (a.window > 0 && j <= p - a.window && j >= a.sinks) {
-      j = p - a.window;
-      continue;
+  __syncthreads();
+
+  const int splits = gridDim.x, rank = blockIdx.x, b = blockIdx.z;
+  const int per_kv = a.heads / a.c.kv_heads, rows = per_kv * a.q_len;
+  const int kvh = blockIdx.y % a.c.kv_heads, row0 = (blockIdx.y / a.c.kv_heads) * 8;
+  const int len = kv_len(a.c, b);
+  // the thread's query row
+  const int rr = row0 + g;
+  const bool have = rr < rows;
+  const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
+  const int64_t qrow = (int64_t)b * a.q_len + qi;
+  const int pos = have ? len - a.q_len + qi : -1;
+  // tiles that some row of the CTA sees: the first n_sink ones, then [first, last]
+  const int p_lo = len - a.q_len + row0 / per_kv, p_hi = len - a.q_len + min(rows - 1, row0 + 7) / per_kv;
+  const int lo = a.window > 0 ? max(0, p_lo - a.window + 1) : 0;
+  const int first = lo / KV_TILE;
+  const int n_sink = a.window > 0 ? min((a.sinks + KV_TILE - 1) / KV_TILE, first) : 0;
+  const int n_tiles = p_hi < 0 ? 0 : n_sink + p_hi / KV_TILE - first + 1;
+  const int units = (n_tiles + 1) / 2, stride = splits * KVA_WARPS, u0 = rank * KVA_WARPS + warp;
+
+  // q: two fp16 parts of the row scaled to [2^14, 2^15), in the order of the K words' nibbles
+  uint32_t qa[4 * G][4];
+  float qs[G], cq;
+  {
+    float x[16 * G], top = 0.0f;
+    const float* src = a.q + qrow * a.ldq + (int64_t)qh * HD;
+#pragma unroll
+    for (int w = 0; w < 2 * G; ++w)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = have ? __ldg(src + 64 * (w / 2) + 16 * t + 8 * (w & 1) + j) : 0.0f;
+        x[8 * w + j] = v;
+        top = fmaxf(top, fabsf(v));
+      }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int e = 0;
+    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
+    const float up = __int_as_float((127 + e) << 23);  // e is in [-113, 126]
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum += x[16 * gi + j];
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      qs[gi] = sum * a.sl2;
     }
-    const uint8_t* tile = kv_tile(a.c, b, kvh, j, tile_bytes);
-    if (!tile) continue;
-    const int tok = j % KV_TILE;
-    float s = 0.0f, v[8] = {};
-    if (on) {
-      const uint32_t wk = *reinterpret_cast<const uint32_t*>(tile + kv_k_word(a.hd, tok, gi, r));
-      const uint32_t wv = *reinterpret_cast<const uint32_t*>(tile + kv_v_word(a.hd, tok, gi, r));
-      const float2 ks = __half22float2(*reinterpret_cast<const __half2*>(tile + kv_scale_at(a.hd, tok, 0, gi)));
-      const float2 vs = __half22float2(*reinterpret_cast<const __half2*>(tile + kv_scale_at(a.hd, tok, 1, gi)));
-      for (int c = 0; c < 8; ++c) {
-        s = fmaf(q[c], fmaf(ks.x, (float)((wk >> (4 * c)) & 15u), ks.y), s);
-        v[c] = fmaf(vs.x, (float)((wv >> (4 * c)) & 15u), vs.y);
+#pragma unroll
+    for (int w = 0; w < 2 * G; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // nibbles (0, 4), (1, 5) and (2, 6), (3, 7)
+        const float* v = x + 8 * w + 2 * h;
+        split_h2(v[0] * up, v[4] * up, qa[2 * w + h][0], qa[2 * w + h][1]);
+        split_h2(v[1] * up * 0.0625f, v[5] * up * 0.0625f, qa[2 * w + h][2], qa[2 * w + h][3]);
+      }
+    cq = __int_as_float((127 - e) << 23) * (16777216.0f * a.sl2);
+  }
+
+  // ring of bulk copies: lanes 0 and 1 each bring one tile of a unit
+  const int per_page = a.c.page_size / KV_TILE;
+  const int32_t* table = a.c.table + (int64_t)b * a.c.table_stride;
+  auto tile_of = [&](int unit) { const int i = 2 * unit + (lane & 1); return i < n_sink ? i : first + i - n_sink; };
+  auto look_up = [&](int unit) -> int32_t {  // the page of the lane's tile, -1 past the end
+    if (lane >= 2 || 2 * unit + lane >= n_tiles) return -1;
+    return __ldg(table + tile_of(unit) / per_page);
+  };
+  uint32_t there = 0;  // two bits per stage: which tiles of the unit exist
+  auto issue = [&](int n, int unit, int32_t page) {
+    const int st = n % KVA_STAGES;
+    bool ok = lane < 2 && 2 * unit + lane < n_tiles;
+    if (ok && (page < 0 || page >= a.c.pages)) {
+      kv_flag(a.c.status, SITE_KV_PAGE);
+      ok = false;
+    }
+    const uint32_t vote = __ballot_sync(0xffffffffu, ok) & 3u;
+    there = (there & ~(3u << (2 * st))) | (vote << (2 * st));
+    if (lane < 2) {
+      const uint32_t bar = bars + 8 * st;
+      if (ok) {
+        mbar_arrive_expect_tx(bar, S::TILE);
+        const int tile = tile_of(unit);
+        const uint8_t* src = a.c.base + (((int64_t)page * a.c.kv_heads + kvh) * per_page + tile % per_page) * S::TILE;
+        bulk_load(ring + st * S::STAGE + lane * S::TILE, src, S::TILE, bar);
+      } else {
+        mbar_arrive(bar);
       }
     }
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= a.sl2;
-    const float top = fmaxf(m, s);
-    const float scale = exp2f(m - top), e = exp2f(s - top);
-    m = top;
-    l = fmaf(l, scale, e);
-    for (int c = 0; c < 8; ++c) o[c] = fmaf(o[c], scale, e * v[c]);
+  };
+  const int mine = u0 < units ? (units - u0 + stride - 1) / stride : 0;  // units of this warp
+  for (int n = 0; n < KVA_STAGES && n < mine; ++n) issue(n, u0 + n * stride, look_up(u0 + n * stride));
+  int32_t ahead = KVA_STAGES < mine ? look_up(u0 + KVA_STAGES * stride) : -1;
+
+  float o[8 * G][4];
+#pragma unroll
+  for (int i = 0; i < 8 * G; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m = -INFINITY, l = 0.0f, pm[G] = {};
+  float rexp = -32.0f;  // largest V scale seen is at most 2^rexp
+  const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
+  bool fine = true;
+  for (int n = 0; n < mine; ++n) {
+    const int st = n % KVA_STAGES, unit = u0 + n * stride;
+    fine = wait_bounded(bars + 8 * st, (n / KVA_STAGES) & 1, wc, SITE_KVA_RING);
+    if (!__all_sync(0xffffffffu, fine)) {
+      fine = false;
+      break;
+    }
+    const uint8_t* stage = smem + warp * S::RING + st * S::STAGE;
+    const uint32_t vote = (there >> (2 * st)) & 3u;
+    // scores of the thread's 2 x 4 tokens (t + 4 i of each tile), log2 units
+    float x[2][4], vs[2][4][G], vm[2][4][G];
+    float top = -INFINITY;
+    __half2 smax = bits_h2(0u);
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint8_t* tile = stage + tt * S::TILE;
+      float ks[4][G], km[4][G];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* p = tile + KV_TILE * HD + (t + 4 * i) * (HD / 8);
+        if (G == 2) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          const float2 f0 = __half22float2(bits_h2(u.x)), f1 = __half22float2(bits_h2(u.y));
+          const float2 f2 = __half22float2(bits_h2(u.z)), f3 = __half22float2(bits_h2(u.w));
+          ks[i][0] = f0.x, ks[i][G - 1] = f0.y, km[i][0] = f1.x, km[i][G - 1] = f1.y;
+          vs[tt][i][0] = f2.x, vs[tt][i][G - 1] = f2.y, vm[tt][i][0] = f3.x, vm[tt][i][G - 1] = f3.y;
+          smax = __hmax2(smax, bits_h2(u.z));
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          const float2 f0 = __half22float2(bits_h2(u.x)), f1 = __half22float2(bits_h2(u.y));
+          ks[i][0] = f0.x, km[i][0] = f0.y, vs[tt][i][0] = f1.x, vm[tt][i][0] = f1.y;
+          smax = __hmax2(smax, bits_h2((u.y & 0xffffu) * 0x10001u));
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        uint32_t kw[2 * G];
+        const uint8_t* p = tile + (8 * nt + g) * (HD / 2) + t * (HD / 8);
+        if (G == 2) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          kw[0] = u.x, kw[1] = u.y, kw[2 * G - 2] = u.z, kw[2 * G - 1] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          kw[0] = u.x, kw[1] = u.y;
+        }
+        float acc0 = 0.0f, acc1 = 0.0f, mn0 = 0.0f, mn1 = 0.0f;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 2 * gi; w < 2 * gi + 2; ++w) {
+            mma_f16(d, qa[2 * w], kw[w] & 0x000F000Fu, kw[w] & 0x00F000F0u);
+            const uint32_t y = kw[w] >> 8;
+            mma_f16(d, qa[2 * w + 1], y & 0x000F000Fu, y & 0x00F000F0u);
+          }
+          acc0 = fmaf(d[0] + d[2], ks[2 * nt][gi], acc0);
+          acc1 = fmaf(d[1] + d[3], ks[2 * nt + 1][gi], acc1);
+          mn0 = fmaf(qs[gi], km[2 * nt][gi], mn0);
+          mn1 = fmaf(qs[gi], km[2 * nt + 1][gi], mn1);
+        }
+        x[tt][2 * nt] = fmaf(acc0, cq, mn0);
+        x[tt][2 * nt + 1] = fmaf(acc1, cq, mn1);
+      }
+    }
+    // masks: only where a row of the CTA does not see the whole unit
+    bool whole = vote == 3u;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const int i = 2 * unit + tt, j0 = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
+      whole = whole && j0 + KV_TILE - 1 <= p_lo && (a.window <= 0 || j0 > p_hi - a.window || j0 + KV_TILE <= a.sinks);
+    }
+    if (!whole) {
+      smax = bits_h2(0u);
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const int i = 2 * unit + tt, j0 = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = j0 + t + 4 * k;
+          const bool see = ((vote >> tt) & 1u) && j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+          if (!see) {
+            x[tt][k] = -INFINITY;
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) vs[tt][k][gi] = vm[tt][k][gi] = 0.0f;
+          }
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) smax = __hmax2(smax, __float2half2_rn(vs[tt][k][gi]));
+        }
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, x[tt][k]);
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      smax = __hmax2(smax, bits_h2(__shfl_xor_sync(0xffffffffu, h2_bits(smax), off)));
+    }
+    // a larger score or a larger V scale moves the exponent's reference; the scale's power of two
+    // is shared by the warp so that all rows move together
+    const float sm = fmaxf(__low2float(smax), __high2float(smax));
+    float need = rexp;
+    if (sm > 0.0f) need = fmaxf(need, (float)(ilogbf(sm) + 1));
+    if (__any_sync(0xffffffffu, top > m || need > rexp)) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, off));
+      const float m2 = fmaxf(m, top);
+      const float alpha = m == -INFINITY ? 0.0f : ex2((m + rexp) - (m2 + need));
+      m = m2, rexp = need;
+      l *= alpha;
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) pm[gi] *= alpha;
+#pragma unroll
+      for (int i = 0; i < 8 * G; ++i) o[i][0] *= alpha, o[i][1] *= alpha, o[i][2] *= alpha, o[i][3] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m + rexp - 14.0f;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint8_t* tile = stage + tt * S::TILE;
+      uint32_t pa[G][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[tt][k] = ex2(x[tt][k] - ref);
+        l += x[tt][k];
+      }
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pm[gi] = fmaf(x[tt][k], fmaf(8.0f, vs[tt][k][gi], vm[tt][k][gi]), pm[gi]);
+        split_h2(x[tt][0] * vs[tt][0][gi], x[tt][1] * vs[tt][1][gi], pa[gi][0], pa[gi][1]);
+        split_h2(x[tt][2] * vs[tt][2][gi], x[tt][3] * vs[tt][3][gi], pa[gi][2], pa[gi][3]);
+      }
+      uint32_t vw[4][G];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* p = tile + KV_TILE * (HD / 2) + (t + 4 * i) * (HD / 2) + g * (HD / 16);
+        if (G == 2) {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          vw[i][0] = u.x, vw[i][G - 1] = u.y;
+        } else {
+          vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+      const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half + (0..3) of the group
+          uint32_t ab = __byte_perm(vw[0][gi], vw[1][gi], half ? 0x7632 : 0x5410);
+          uint32_t cd = __byte_perm(vw[2][gi], vw[3][gi], half ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int pr = 0; pr < 2; ++pr) {
+            const int j = 8 * gi + 4 * half + 2 * pr;
+            const uint32_t b0 = h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032));
+            const uint32_t b1 = h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032));
+            mma_f16(o[j], pa[gi], b0, b1);
+            const uint32_t e0 = h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72));
+            const uint32_t e1 = h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72));
+            mma_f16(o[j + 1], pa[gi], e0, e1);
+            ab >>= 8, cd >>= 8;
+          }
+        }
+    }
+    __syncwarp();  // every lane has read the stage
+    if (n + KVA_STAGES < mine) {
+      issue(n + KVA_STAGES, unit + KVA_STAGES * stride, ahead);
+      ahead = n + 1 + KVA_STAGES < mine ? look_up(unit + (KVA_STAGES + 1) * stride) : -1;
+    }
   }
-  if (on)
-    for (int c = 0; c < 8; ++c) a.out[row * a.ldo + (int64_t)h * a.hd + 8 * lane + c] = l > 0.0f ? o[c] / l : (l == l ? 0.0f : l);
+  if (!fine) {  // given up: no copy may be in flight when the rings are used again
+    if (lane == 0)
+      for (int i = 0; i < KVA_STAGES; ++i) wait_drain(bars + 8 * i, 0, a.wait_cap_ns), wait_drain(bars + 8 * i, 1, a.wait_cap_ns);
+    __syncwarp();
+  }
+  // join the warps
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, off);
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) pm[gi] += __shfl_xor_sync(0xffffffffu, pm[gi], off);
+  }
+  __syncthreads();
+  float* wout = reinterpret_cast<float*>(smem) + (size_t)warp * 8 * S::OUT_LD;
+#pragma unroll
+  for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int q4 = 0; q4 < 2; ++q4) {
+        float4 v;
+        float* pv = &v.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float(&d)[4] = o[8 * gi + 4 * q4 + j];
+          pv[j] = (d[c] + d[c + 2]) + pm[gi];
+        }
+        *reinterpret_cast<float4*>(wout + g * S::OUT_LD + 64 * gi + 16 * t + 8 * c + 4 * q4) = v;
+      }
+  if (t == 0) {
+    // a row of NaN scores has no maximum, but its sum is NaN and has to come through
+    ml[warp * 16 + g] = m > -INFINITY ? m + rexp : l == l ? -INFINITY : 0.0f;
+    ml[warp * 16 + 8 + g] = l;
+  }
+  __syncthreads();
+  float* cout = reinterpret_cast<float*>(smem) + KVA_WARPS * 8 * S::OUT_LD;
+  for (int i = threadIdx.x; i < 8 * HD; i += KVA_THREADS) {
+    const int r = i / HD, c = i % HD;
+    float top = -INFINITY, sum = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < KVA_WARPS; ++w) top = fmaxf(top, ml[w * 16 + r]);
+#pragma unroll
+    for (int w = 0; w < KVA_WARPS; ++w) {
+      const float f = ml[w * 16 + r] == -INFINITY ? 0.0f : ex2(ml[w * 16 + r] - top);
+      if (f > 0.0f) {
+        sum = fmaf(f, ml[w * 16 + 8 + r], sum);
+        y = fmaf(f, reinterpret_cast<float*>(smem)[(w * 8 + r) * S::OUT_LD + c], y);
+      }
+    }
+    if (splits == 1) {
+      const int q = row0 + r;
+      if (q < rows)
+        a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
+            top == -INFINITY ? 0.0f : y / sum;
+    } else {
+      cout[r * S::OUT_LD + c] = y;
+      if (c == 0) ml[KVA_WARPS * 16 + r] = top, ml[KVA_WARPS * 16 + 8 + r] = sum;
+    }
+  }
+  if (splits == 1) return;
+  // join the CTAs of the cluster, each writing its share of the outputs
+  cluster_sync();
+  const uint32_t cout_s = sbase + KVA_WARPS * 8 * S::OUT_LD * 4, ml_s = sbase + S::ML + KVA_WARPS * 64;
+  for (int i = rank * KVA_THREADS + threadIdx.x; i < 8 * HD; i += splits * KVA_THREADS) {
+    const int r = i / HD, c = i % HD, q = row0 + r;
+    if (q >= rows) continue;
+    float top = -INFINITY, sum = 0.0f, y = 0.0f;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, ld_cluster_f32(mapa_shared(ml_s + r * 4, s)));
+    for (int s = 0; s < splits; ++s) {
+      const float ms = ld_cluster_f32(mapa_shared(ml_s + r * 4, s));
+      const float f = ms == -INFINITY ? 0.0f : ex2(ms - top);
+      if (f > 0.0f) {
+        sum = fmaf(f, ld_cluster_f32(mapa_shared(ml_s + 32 + r * 4, s)), sum);
+        y = fmaf(f, ld_cluster_f32(mapa_shared(cout_s + (r * S::OUT_LD + c) * 4, s)), y);
+      }
+    }
+    a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
+        top == -INFINITY ? 0.0f : y / sum;
+  }
+  cluster_sync();  // no CTA leaves while others read its shared memory
 }
 
 }  // namespace envg

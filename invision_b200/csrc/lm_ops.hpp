@@ -212,14 +212,56 @@ int kv4_rows(envg_kv4 c, float* k, int64_t ldk, float* v, int64_t ldv, const int
   return finish_call(d, flags);
 }
 
-int launch_kv4_attn(Dev* d, const KvAttnArgs& a, int max_ctx) {
-  const int64_t items = (int64_t)a.batch * a.q_len * a.heads;
-  const double tok = (double)a.batch * max_ctx;
-  ProfScope ps(stream_of(d), KID_KV4_ATTN, 4.0 * a.hd * a.heads * (double)a.q_len * tok,
-               tok * a.c.kv_heads * (a.hd + 8 * (a.hd / KV_GROUP)) + 8.0 * (double)a.batch * a.q_len * a.heads * a.hd);
-  ENVG_TRY(launch_pdl(d, k_kv4_attn_simple, dim3((unsigned)cdiv(items, 4)), dim3(128), 0, a));
+// CTAs that share one (sequence, kv head, eight rows): enough for two waves of three CTAs per SM,
+// as long as each warp keeps a unit of two tiles.  A power of two up to 8 (the portable cluster).
+int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
+  int s = 1;
+  while (s < 8 && groups * s * 2 <= (int64_t)d->sms * 6 && cdiv(tokens, 2 * KV_TILE) >= (int64_t)s * 2 * KVA_WARPS) s *= 2;
+  return s;
+}
+
+template <int HD>
+int launch_kv4_attn_t(Dev* d, const KvAttnArgs& a, int splits) {
+  using S = KvaSmem<HD>;
+  static bool attr_set[64] = {};
+  if (!attr_set[d->id]) {
+    ENVG_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+    attr_set[d->id] = true;
+  }
+  const int64_t tiles = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, 8) * a.c.kv_heads;
+  if (tiles > 65535 || a.batch > 65535) return fail(ENVG_ERR_UNSUPPORTED, "attention_kv4: batch %d x %lld row tiles is too large", a.batch, (long long)tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)tiles, (unsigned)a.batch);
+  cfg.blockDim = dim3(KVA_THREADS);
+  cfg.dynamicSmemBytes = S::TOTAL;
+  cfg.stream = stream_of(d);
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (splits > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)splits, at[n].val.clusterDim.y = 1, at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (d->pdl && !g_prof_on) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)n;
+  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_kv4_attn<HD>, a));
   d->st.kernel_launches++;
   return ENVG_OK;
+}
+
+int launch_kv4_attn(Dev* d, const KvAttnArgs& a, int max_ctx) {
+  const int64_t rows = (int64_t)a.batch * a.q_len;
+  const double seen = a.window > 0 ? std::min<double>(max_ctx, (double)a.window + a.sinks + a.q_len) : max_ctx;
+  ProfScope ps(stream_of(d), KID_KV4_ATTN, 4.0 * a.hd * a.heads * (double)rows * seen,
+               seen * a.batch * a.c.kv_heads * (a.hd + 8 * (a.hd / KV_GROUP)) + 8.0 * (double)rows * a.heads * a.hd);
+  const int64_t groups = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, 8) * a.c.kv_heads * a.batch;
+  const int splits = kv4_splits(d, groups, (int64_t)seen);
+  return a.hd == 128 ? launch_kv4_attn_t<128>(d, a, splits) : launch_kv4_attn_t<64>(d, a, splits);
 }
 
 }  // namespace
@@ -550,6 +592,7 @@ int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, env
   a.batch = batch, a.q_len = q_len, a.heads = heads, a.hd = cache->head_dim;
   a.window = window, a.sinks = sinks;
   a.sl2 = scale * 1.4426950408889634f;
+  a.wait_cap_ns = d->wait_cap_ns;
   const int64_t most = table_stride * cache->page_size;
   ENVG_TRY(launch_kv4_attn(d, a, (int)(max_ctx > 0 ? std::min<int64_t>(max_ctx, most) : most)));
   if (!devp) ENVG_TRY(st.out(io, dst, ldo, rows, width));
