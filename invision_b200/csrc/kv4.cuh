@@ -435,9 +435,9 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
   for (int n = 0; n < KVA_STAGES && n < mine; ++n) issue(n, u0 + n * stride, look_up(u0 + n * stride));
   int32_t ahead = KVA_STAGES < mine ? look_up(u0 + KVA_STAGES * stride) : -1;
 
-  float o[8 * G][4];
+  float o[8 * G][2];
 #pragma unroll
-  for (int i = 0; i < 8 * G; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  for (int i = 0; i < 8 * G; ++i) o[i][0] = o[i][1] = 0.0f;
   float m = -INFINITY, l = 0.0f, pm[G] = {};
   float rexp = -32.0f;  // largest V scale seen is at most 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
@@ -556,13 +556,13 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) pm[gi] *= alpha;
 #pragma unroll
-      for (int i = 0; i < 8 * G; ++i) o[i][0] *= alpha, o[i][1] *= alpha, o[i][2] *= alpha, o[i][3] *= alpha;
+      for (int i = 0; i < 8 * G; ++i) o[i][0] *= alpha, o[i][1] *= alpha;
     }
     const float ref = m == -INFINITY ? 0.0f : m + rexp - 14.0f;
+    uint32_t pa[2][G][4], vw[2][4][G];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       const uint8_t* tile = stage + tt * S::TILE;
-      uint32_t pa[G][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[tt][k] = ex2(x[tt][k] - ref);
@@ -572,40 +572,45 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
       for (int gi = 0; gi < G; ++gi) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) pm[gi] = fmaf(x[tt][k], fmaf(8.0f, vs[tt][k][gi], vm[tt][k][gi]), pm[gi]);
-        split_h2(x[tt][0] * vs[tt][0][gi], x[tt][1] * vs[tt][1][gi], pa[gi][0], pa[gi][1]);
-        split_h2(x[tt][2] * vs[tt][2][gi], x[tt][3] * vs[tt][3][gi], pa[gi][2], pa[gi][3]);
+        split_h2(x[tt][0] * vs[tt][0][gi], x[tt][1] * vs[tt][1][gi], pa[tt][gi][0], pa[tt][gi][1]);
+        split_h2(x[tt][2] * vs[tt][2][gi], x[tt][3] * vs[tt][3][gi], pa[tt][gi][2], pa[tt][gi][3]);
       }
-      uint32_t vw[4][G];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint8_t* p = tile + KV_TILE * (HD / 2) + (t + 4 * i) * (HD / 2) + g * (HD / 16);
         if (G == 2) {
           const uint2 u = *reinterpret_cast<const uint2*>(p);
-          vw[i][0] = u.x, vw[i][G - 1] = u.y;
+          vw[tt][i][0] = u.x, vw[tt][i][G - 1] = u.y;
         } else {
-          vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+          vw[tt][i][0] = *reinterpret_cast<const uint32_t*>(p);
         }
       }
-      const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half + (0..3) of the group
-          uint32_t ab = __byte_perm(vw[0][gi], vw[1][gi], half ? 0x7632 : 0x5410);
-          uint32_t cd = __byte_perm(vw[2][gi], vw[3][gi], half ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int pr = 0; pr < 2; ++pr) {
-            const int j = 8 * gi + 4 * half + 2 * pr;
-            const uint32_t b0 = h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032));
-            const uint32_t b1 = h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032));
-            mma_f16(o[j], pa[gi], b0, b1);
-            const uint32_t e0 = h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72));
-            const uint32_t e1 = h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72));
-            mma_f16(o[j + 1], pa[gi], e0, e1);
-            ab >>= 8, cd >>= 8;
-          }
-        }
     }
+    // The tensor cores cut off what a product adds below the accumulator's last bit, always
+    // towards zero; over a long context that bias would reach 1e-5.  So each unit's two products
+    // start from zero and are added, high and low part together, in rounded fp32.
+    const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)  // channels 8 g + 4 half + (0..3) of the group
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) {
+          float d[2][4] = {};
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            uint32_t ab = __byte_perm(vw[tt][0][gi], vw[tt][1][gi], half ? 0x7632 : 0x5410);
+            uint32_t cd = __byte_perm(vw[tt][2][gi], vw[tt][3][gi], half ? 0x7632 : 0x5410);
+            if (pr) ab >>= 8, cd >>= 8;
+            mma_f16(d[0], pa[tt][gi], h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032)),
+                    h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032)));
+            mma_f16(d[1], pa[tt][gi], h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72)),
+                    h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72)));
+          }
+          const int j = 8 * gi + 4 * half + 2 * pr;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) o[j + i][0] += d[i][0] + d[i][2], o[j + i][1] += d[i][1] + d[i][3];
+        }
     __syncwarp();  // every lane has read the stage
     if (n + KVA_STAGES < mine) {
       issue(n + KVA_STAGES, unit + KVA_STAGES * stride, ahead);
@@ -635,10 +640,7 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
         float4 v;
         float* pv = &v.x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float(&d)[4] = o[8 * gi + 4 * q4 + j];
-          pv[j] = (d[c] + d[c + 2]) + pm[gi];
-        }
+        for (int j = 0; j < 4; ++j) pv[j] = o[8 * gi + 4 * q4 + j][c] + pm[gi];
         *reinterpret_cast<float4*>(wout + g * S::OUT_LD + 64 * gi + 16 * t + 8 * c + 4 * q4) = v;
       }
   if (t == 0) {
