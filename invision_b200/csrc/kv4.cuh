@@ -10,8 +10,8 @@
 // A 32-bit word holds 8 consecutive channels 64 gi + 8 r + j (nibble j, r = 0..7).  In a K row,
 // word (gi, r) stands at byte (r / 2) * hd / 8 + (2 gi + r % 2) * 4, so that lane t of a quad
 // finds the words of its 16-channel pieces side by side; in a V row at byte r * hd / 16 + 4 gi.
-// Token 8 a + 4 b + c of a tile takes K row 8 a + 2 c + b: the scores that lane t of a quad then
-// gets are those of tokens t, t + 4, t + 8, t + 12, whose V rows four lanes read side by side.
+// Token 8 a + 2 c + b of a tile takes V row 8 a + 4 b + c: lane t of a quad multiplies tokens 2 t,
+// 2 t + 1, 2 t + 8 and 2 t + 9, and the quad's four lanes read the rows of each side by side.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -159,10 +159,12 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(const NormRopeArgs a) {
 // each; the group's minimum and maximum are one shuffle tree.  Every rounding is IEEE (no
 // contraction), so equal inputs give equal codes on any path that uses the formula.
 ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) {
-  const int row = (tok & 8) + 2 * (tok & 3) + ((tok >> 2) & 1);
-  return row * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4;
+  return tok * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4;
 }
-ENVG_DEV uint32_t kv_v_word(int hd, int tok, int gi, int r) { return KV_TILE * (hd / 2) + tok * (hd / 2) + r * (hd / 16) + 4 * gi; }
+ENVG_DEV uint32_t kv_v_word(int hd, int tok, int gi, int r) {
+  const int row = (tok & 8) + 4 * (tok & 1) + ((tok >> 1) & 3);
+  return KV_TILE * (hd / 2) + row * (hd / 2) + r * (hd / 16) + 4 * gi;
+}
 // Byte offset of the scale of (token, K or V, group); its minimum stands hd / 64 halves further.
 ENVG_DEV uint32_t kv_scale_at(int hd, int tok, int v, int gi) { return KV_TILE * hd + tok * (hd / 8) + v * (hd / 16) + 2 * gi; }
 ENVG_DEV float2 kv_scale(const uint8_t* tile, uint32_t at, int hd) {
@@ -260,30 +262,44 @@ struct KvAttnArgs {
   int64_t ldq, ldo;
   int batch, q_len, heads, hd, window, sinks;
   float sl2;  // softmax scale * log2 e
+  int vec;    // rows of q are 16-byte aligned
   uint64_t wait_cap_ns;
 };
 
-// k_kv4_attn: flash attention of up to eight query rows over one kv head's cached tokens.
+// k_kv4_attn: flash attention of up to 4 NB query rows over one kv head's cached tokens.
 //
-// Mathematics.  The eight rows are (query token, head) pairs that read the same kv head.  A row's
-// score of token j is sum_g s_jg (q_g . c_jg) + m_jg sum(q_g) over its groups of 64 channels, and
-// its output sum_j p_j (s_jg (c_jg - 8) + (m_jg + 8 s_jg)).  Both products with codes run on the
+// Mathematics.  The rows are (query token, head) pairs that read the same kv head.  A row's score
+// of token j is sum_g s_jg (q_g . c_jg) + m_jg sum(q_g) over its groups of 64 channels, and its
+// output sum_j p_j (s_jg (c_jg - 8) + (m_jg + 8 s_jg)).  Both products with codes run on the
 // tensor cores as m16n8k16 with fp16 operands and fp32 sums, exactly in the codes: a code is a
 // subnormal fp16 (c 2^-24, or 16 c 2^-24) for K, c - 8 for V (centred: the positive codes' sum
-// would be far larger than the outputs and cost its last bits).  q and p s are split into two
-// fp16 parts each, the high parts in rows 0..7 of the 16-row operand and the low parts in rows
-// 8..15, so that fp32 accuracy costs no further instruction; q is scaled by a power of two per
-// row, p s by the row maximum and by the largest s seen (both folded into the exponent).
-// The S accumulator's layout is the P operand's, so scores stay in their threads.
+// would be far larger than the outputs and cost its last bits).  The codes are the 16-row operand
+// (16 tokens of K, 16 channels of V^T), so a code is unpacked once for all rows; q and p s are the
+// 8-column one, each split into two fp16 parts in adjacent columns, so that fp32 accuracy costs no
+// further instruction.  q is scaled by a power of two per row, p s by the row maximum and by the
+// largest s seen (both folded into the exponent).  Scores come out as [token][row]; an 8 x 8
+// transpose in registers (movmatrix) makes the P operand of them.
 //
 // Split.  Tokens are taken in units of two 16-token tiles, dealt out over the warps of a cluster
-// of CTAs (one cluster per sequence, kv head and eight rows).  Each warp runs a one-pass softmax
+// of CTAs (one cluster per sequence, kv head and 4 NB rows).  Each warp runs a one-pass softmax
 // with its own ring of bulk copies; the warps' (max, sum, output) are joined in shared memory, the
 // CTAs' through distributed shared memory in rank order: no workspace, no atomics, one launch.
-ENVG_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+ENVG_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+}
+// The same from a zero accumulator.
+ENVG_DEV void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.0f));
+}
+// Transpose of an 8 x 8 matrix of halves; thread 4 r + c holds row r, columns 2 c and 2 c + 1.
+ENVG_DEV uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 ENVG_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 ENVG_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
@@ -291,13 +307,6 @@ ENVG_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// (x, y) as fp16 high parts and what they leave.
-ENVG_DEV void split_h2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 b = __half22float2(h);
-  hi = h2_bits(h);
-  lo = h2_bits(__floats2half2_rn(x - b.x, y - b.y));
 }
 ENVG_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -310,26 +319,27 @@ ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 4;
+constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 3;
 constexpr int SITE_KVA_RING = 60;  // status[1] of a ring wait that ran out
 
-template <int HD>
+template <int HD, int NB>
 struct KvaSmem {
+  static constexpr int ROWS = 4 * NB;
   static constexpr int TILE = kv_tile_bytes(HD), STAGE = 2 * TILE;
-  static constexpr int RING = KVA_STAGES * STAGE;                  // per warp
-  static constexpr int BARS = KVA_WARPS * RING;                    // mbarriers
-  static constexpr int ABORT = BARS + KVA_WARPS * KVA_STAGES * 8;  // abort flag of the bounded waits
-  static constexpr int ML = ABORT + 16;                            // [warps + 1][max 8 | sum 8]
-  static constexpr int TOTAL = ML + (KVA_WARPS + 1) * 16 * 4;
-  // the rings are empty when the outputs of the warps are joined: [warp][8][HD], then the CTA's [8][HD]
-  static constexpr int OUT_LD = HD + 4;
-  static_assert((KVA_WARPS + 1) * 8 * OUT_LD * 4 <= BARS, "outputs fit the rings");
+  static constexpr int RING = KVA_STAGES * STAGE;  // per warp
+  // the rings are empty when the outputs of the warps are joined: [warp][ROWS][HD], then the CTA's
+  static constexpr int OUT_LD = HD + 4, OUT = (KVA_WARPS + 1) * ROWS * OUT_LD * 4;
+  static constexpr int BARS = KVA_WARPS * RING > OUT ? KVA_WARPS * RING : OUT;  // mbarriers
+  static constexpr int ABORT = BARS + KVA_WARPS * KVA_STAGES * 8;               // abort flag of the bounded waits
+  static constexpr int ML = ABORT + 16;                                         // [warps + 1][max ROWS | sum ROWS]
+  static constexpr int TOTAL = ML + (KVA_WARPS + 1) * 2 * ROWS * 4;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a) {
-  using S = KvaSmem<HD>;
+template <int HD, int NB>
+__global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 128 ? 2 : 3) k_kv4_attn(const KvAttnArgs a) {
+  using S = KvaSmem<HD, NB>;
   constexpr int G = HD / KV_GROUP;  // groups per head
+  constexpr int ROWS = S::ROWS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem);
@@ -346,60 +356,15 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
 
   const int splits = gridDim.x, rank = blockIdx.x, b = blockIdx.z;
   const int per_kv = a.heads / a.c.kv_heads, rows = per_kv * a.q_len;
-  const int kvh = blockIdx.y % a.c.kv_heads, row0 = (blockIdx.y / a.c.kv_heads) * 8;
+  const int kvh = blockIdx.y % a.c.kv_heads, row0 = (blockIdx.y / a.c.kv_heads) * ROWS;
   const int len = kv_len(a.c, b);
-  // the thread's query row
-  const int rr = row0 + g;
-  const bool have = rr < rows;
-  const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
-  const int64_t qrow = (int64_t)b * a.q_len + qi;
-  const int pos = have ? len - a.q_len + qi : -1;
   // tiles that some row of the CTA sees: the first n_sink ones, then [first, last]
-  const int p_lo = len - a.q_len + row0 / per_kv, p_hi = len - a.q_len + min(rows - 1, row0 + 7) / per_kv;
+  const int p_lo = len - a.q_len + row0 / per_kv, p_hi = len - a.q_len + min(rows - 1, row0 + ROWS - 1) / per_kv;
   const int lo = a.window > 0 ? max(0, p_lo - a.window + 1) : 0;
   const int first = lo / KV_TILE;
   const int n_sink = a.window > 0 ? min((a.sinks + KV_TILE - 1) / KV_TILE, first) : 0;
   const int n_tiles = p_hi < 0 ? 0 : n_sink + p_hi / KV_TILE - first + 1;
   const int units = (n_tiles + 1) / 2, stride = splits * KVA_WARPS, u0 = rank * KVA_WARPS + warp;
-
-  // q: two fp16 parts of the row scaled to [2^14, 2^15), in the order of the K words' nibbles
-  uint32_t qa[4 * G][4];
-  float qs[G], cq;
-  {
-    float x[16 * G], top = 0.0f;
-    const float* src = a.q + qrow * a.ldq + (int64_t)qh * HD;
-#pragma unroll
-    for (int w = 0; w < 2 * G; ++w)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = have ? __ldg(src + 64 * (w / 2) + 16 * t + 8 * (w & 1) + j) : 0.0f;
-        x[8 * w + j] = v;
-        top = fmaxf(top, fabsf(v));
-      }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
-    const float up = __int_as_float((127 + e) << 23);  // e is in [-113, 126]
-#pragma unroll
-    for (int gi = 0; gi < G; ++gi) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sum += x[16 * gi + j];
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      qs[gi] = sum * a.sl2;
-    }
-#pragma unroll
-    for (int w = 0; w < 2 * G; ++w)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // nibbles (0, 4), (1, 5) and (2, 6), (3, 7)
-        const float* v = x + 8 * w + 2 * h;
-        split_h2(v[0] * up, v[4] * up, qa[2 * w + h][0], qa[2 * w + h][1]);
-        split_h2(v[1] * up * 0.0625f, v[5] * up * 0.0625f, qa[2 * w + h][2], qa[2 * w + h][3]);
-      }
-    cq = __int_as_float((127 - e) << 23) * (16777216.0f * a.sl2);
-  }
 
   // ring of bulk copies: lanes 0 and 1 each bring one tile of a unit
   const int per_page = a.c.page_size / KV_TILE;
@@ -410,8 +375,7 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
     return __ldg(table + tile_of(unit) / per_page);
   };
   uint32_t there = 0;  // two bits per stage: which tiles of the unit exist
-  auto issue = [&](int n, int unit, int32_t page) {
-    const int st = n % KVA_STAGES;
+  auto issue = [&](int st, int unit, int32_t page) {
     bool ok = lane < 2 && 2 * unit + lane < n_tiles;
     if (ok && (page < 0 || page >= a.c.pages)) {
       kv_flag(a.c.status, SITE_KV_PAGE);
@@ -435,33 +399,94 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
   for (int n = 0; n < KVA_STAGES && n < mine; ++n) issue(n, u0 + n * stride, look_up(u0 + n * stride));
   int32_t ahead = KVA_STAGES < mine ? look_up(u0 + KVA_STAGES * stride) : -1;
 
-  float o[8 * G][2];
+  // q: column g of an operand is part g % 2 of row g / 2, scaled to [2^14, 2^15) before the split,
+  // in the order of the K words' nibbles; a thread's scores are those of row t
+  uint32_t qb[NB][4 * G][2];
+  float qs[NB][G], cq[NB];
+  int pos[NB];
 #pragma unroll
-  for (int i = 0; i < 8 * G; ++i) o[i][0] = o[i][1] = 0.0f;
-  float m = -INFINITY, l = 0.0f, pm[G] = {};
-  float rexp = -32.0f;  // largest V scale seen is at most 2^rexp
+  for (int nb = 0; nb < NB; ++nb) {
+    const int rr = row0 + 4 * nb + (g >> 1);
+    const bool have = rr < rows;
+    const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
+    const float* src = a.q + ((int64_t)b * a.q_len + qi) * a.ldq + (int64_t)qh * HD + 16 * t;
+    float x[16 * G], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (have) v = ld_f4(src + 64 * (i / 4) + 4 * (i % 4), a.vec != 0);
+      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int e = 0;
+    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
+    const float up = __int_as_float((127 + e) << 23);  // e is in [-113, 126]
+    const int from = 8 * t;                            // a lane whose g / 2 is this thread's t
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum += x[16 * gi + j];
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
+    }
+    cq[nb] = __int_as_float((127 - __shfl_sync(0xffffffffu, e, from)) << 23) * (16777216.0f * a.sl2);
+    const int mr = row0 + 4 * nb + t;
+    pos[nb] = mr < rows ? len - a.q_len + mr / per_kv : -1;
+#pragma unroll
+    for (int j = 0; j < 16 * G; ++j) {
+      const float v = x[j] * (((j & 7) & 1) ? up * 0.0625f : up);
+      const __half hi = __float2half_rn(v);
+      x[j] = (g & 1) ? v - __half2float(hi) : v;
+    }
+#pragma unroll
+    for (int w = 0; w < 2 * G; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // nibbles (0, 4), (1, 5) and (2, 6), (3, 7)
+        const float* v = x + 8 * w + 2 * h;
+        qb[nb][2 * w + h][0] = h2_bits(__floats2half2_rn(v[0], v[4]));
+        qb[nb][2 * w + h][1] = h2_bits(__floats2half2_rn(v[1], v[5]));
+      }
+  }
+
+  float o[NB][4 * G][2], m[NB], l[NB], pm[NB][G];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = -INFINITY, l[nb] = 0.0f;
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) pm[nb][gi] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = 0.0f;
+  }
+  float rexp = -32.0f, rscale = 0.0f;  // no V scale seen is above rscale = 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
   bool fine = true;
+  int st = 0;
+  uint32_t phase = 0;
   for (int n = 0; n < mine; ++n) {
-    const int st = n % KVA_STAGES, unit = u0 + n * stride;
-    fine = wait_bounded(bars + 8 * st, (n / KVA_STAGES) & 1, wc, SITE_KVA_RING);
+    const int unit = u0 + n * stride;
+    fine = wait_bounded(bars + 8 * st, phase, wc, SITE_KVA_RING);
     if (!__all_sync(0xffffffffu, fine)) {
       fine = false;
       break;
     }
     const uint8_t* stage = smem + warp * S::RING + st * S::STAGE;
     const uint32_t vote = (there >> (2 * st)) & 3u;
-    // scores of the thread's 2 x 4 tokens (t + 4 i of each tile), log2 units
-    float x[2][4], vs[2][4][G], vm[2][4][G];
-    float top = -INFINITY;
+    // scores of tokens g and g + 8 of each tile, log2 units
+    float x[NB][2][2], vs[2][2][G], vm[2][2][G];
     __half2 smax = bits_h2(0u);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       const uint8_t* tile = stage + tt * S::TILE;
-      float ks[4][G], km[4][G];
+      float ks[2][G], km[2][G];
+      uint32_t kw[2][2 * G];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = tile + KV_TILE * HD + (t + 4 * i) * (HD / 8);
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* p = tile + KV_TILE * HD + (g + 8 * i) * (HD / 8);
+        const uint8_t* pk = tile + (g + 8 * i) * (HD / 2) + t * (HD / 8);
         if (G == 2) {
           const uint4 u = *reinterpret_cast<const uint4*>(p);
           const float2 f0 = __half22float2(bits_h2(u.x)), f1 = __half22float2(bits_h2(u.y));
@@ -469,115 +494,138 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
           ks[i][0] = f0.x, ks[i][G - 1] = f0.y, km[i][0] = f1.x, km[i][G - 1] = f1.y;
           vs[tt][i][0] = f2.x, vs[tt][i][G - 1] = f2.y, vm[tt][i][0] = f3.x, vm[tt][i][G - 1] = f3.y;
           smax = __hmax2(smax, bits_h2(u.z));
+          const uint4 k4 = *reinterpret_cast<const uint4*>(pk);
+          kw[i][0] = k4.x, kw[i][1] = k4.y, kw[i][2 * G - 2] = k4.z, kw[i][2 * G - 1] = k4.w;
         } else {
           const uint2 u = *reinterpret_cast<const uint2*>(p);
           const float2 f0 = __half22float2(bits_h2(u.x)), f1 = __half22float2(bits_h2(u.y));
           ks[i][0] = f0.x, km[i][0] = f0.y, vs[tt][i][0] = f1.x, vm[tt][i][0] = f1.y;
           smax = __hmax2(smax, bits_h2((u.y & 0xffffu) * 0x10001u));
+          const uint2 k2 = *reinterpret_cast<const uint2*>(pk);
+          kw[i][0] = k2.x, kw[i][1] = k2.y;
         }
       }
+      float mn[NB][2];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        uint32_t kw[2 * G];
-        const uint8_t* p = tile + (8 * nt + g) * (HD / 2) + t * (HD / 8);
-        if (G == 2) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          kw[0] = u.x, kw[1] = u.y, kw[2 * G - 2] = u.z, kw[2 * G - 1] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          kw[0] = u.x, kw[1] = u.y;
-        }
-        float acc0 = 0.0f, acc1 = 0.0f, mn0 = 0.0f, mn1 = 0.0f;
+      for (int nb = 0; nb < NB; ++nb) x[nb][tt][0] = x[nb][tt][1] = mn[nb][0] = mn[nb][1] = 0.0f;
 #pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int gi = 0; gi < G; ++gi) {
+        float d[NB][4];
 #pragma unroll
-          for (int w = 2 * gi; w < 2 * gi + 2; ++w) {
-            mma_f16(d, qa[2 * w], kw[w] & 0x000F000Fu, kw[w] & 0x00F000F0u);
-            const uint32_t y = kw[w] >> 8;
-            mma_f16(d, qa[2 * w + 1], y & 0x000F000Fu, y & 0x00F000F0u);
+        for (int w = 2 * gi; w < 2 * gi + 2; ++w) {
+          const uint32_t u0w = kw[0][w], u1w = kw[1][w], y0 = u0w >> 8, y1 = u1w >> 8;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if (w == 2 * gi)
+              mma_f16_zero(d[nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
+            else
+              mma_f16(d[nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
+            mma_f16(d[nb], y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[nb][2 * w + 1]);
           }
-          acc0 = fmaf(d[0] + d[2], ks[2 * nt][gi], acc0);
-          acc1 = fmaf(d[1] + d[3], ks[2 * nt + 1][gi], acc1);
-          mn0 = fmaf(qs[gi], km[2 * nt][gi], mn0);
-          mn1 = fmaf(qs[gi], km[2 * nt + 1][gi], mn1);
         }
-        x[tt][2 * nt] = fmaf(acc0, cq, mn0);
-        x[tt][2 * nt + 1] = fmaf(acc1, cq, mn1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            x[nb][tt][i] = fmaf(d[nb][2 * i] + d[nb][2 * i + 1], ks[i][gi], x[nb][tt][i]);
+            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);
+          }
       }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[nb][tt][i] = fmaf(x[nb][tt][i], cq[nb], mn[nb][i]);
     }
-    // masks: only where a row of the CTA does not see the whole unit
+    // masks: only where a row of the CTA does not see the whole unit.  A row hides a token by its
+    // score; its scale and minimum are dropped where no row sees it (they may hold anything there).
     bool whole = vote == 3u;
+    int j0[2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const int i = 2 * unit + tt, j0 = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
-      whole = whole && j0 + KV_TILE - 1 <= p_lo && (a.window <= 0 || j0 > p_hi - a.window || j0 + KV_TILE <= a.sinks);
+      const int i = 2 * unit + tt;
+      j0[tt] = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
+      whole = whole && j0[tt] + KV_TILE - 1 <= p_lo && (a.window <= 0 || j0[tt] > p_hi - a.window || j0[tt] + KV_TILE <= a.sinks);
     }
     if (!whole) {
       smax = bits_h2(0u);
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const int i = 2 * unit + tt, j0 = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
+      for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int j = j0 + t + 4 * k;
-          const bool see = ((vote >> tt) & 1u) && j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
-          if (!see) {
-            x[tt][k] = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          const int j = j0[tt] + g + 8 * i;
+          bool any = false;
 #pragma unroll
-            for (int gi = 0; gi < G; ++gi) vs[tt][k][gi] = vm[tt][k][gi] = 0.0f;
+          for (int nb = 0; nb < NB; ++nb) {
+            const bool see = ((vote >> tt) & 1u) && j <= pos[nb] && (a.window <= 0 || j > pos[nb] - a.window || j < a.sinks);
+            if (!see) x[nb][tt][i] = -INFINITY;
+            any |= see;
           }
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) smax = __hmax2(smax, __float2half2_rn(vs[tt][k][gi]));
+          for (int gi = 0; gi < G; ++gi) {
+            if (!any) vs[tt][i][gi] = vm[tt][i][gi] = 0.0f;
+            smax = __hmax2(smax, __float2half2_rn(vs[tt][i][gi]));
+          }
         }
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top = fmaxf(top, x[tt][k]);
-#pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      smax = __hmax2(smax, bits_h2(__shfl_xor_sync(0xffffffffu, h2_bits(smax), off)));
     }
     // a larger score or a larger V scale moves the exponent's reference; the scale's power of two
     // is shared by the warp so that all rows move together
-    const float sm = fmaxf(__low2float(smax), __high2float(smax));
-    float need = rexp;
-    if (sm > 0.0f) need = fmaxf(need, (float)(ilogbf(sm) + 1));
-    if (__any_sync(0xffffffffu, top > m || need > rexp)) {
+    float top[NB];
+    bool moves = false;
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, off));
-      const float m2 = fmaxf(m, top);
-      const float alpha = m == -INFINITY ? 0.0f : ex2((m + rexp) - (m2 + need));
-      m = m2, rexp = need;
-      l *= alpha;
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi) pm[gi] *= alpha;
-#pragma unroll
-      for (int i = 0; i < 8 * G; ++i) o[i][0] *= alpha, o[i][1] *= alpha;
+    for (int nb = 0; nb < NB; ++nb) {
+      top[nb] = fmaxf(fmaxf(x[nb][0][0], x[nb][0][1]), fmaxf(x[nb][1][0], x[nb][1][1]));
+      moves |= top[nb] > m[nb];
     }
-    const float ref = m == -INFINITY ? 0.0f : m + rexp - 14.0f;
-    uint32_t pa[2][G][4], vw[2][4][G];
+    const float sm = fmaxf(__low2float(smax), __high2float(smax));
+    moves |= sm > rscale;
+    if (__any_sync(0xffffffffu, moves)) {
+      float need = rexp;
+      if (sm > 0.0f) need = fmaxf(need, (float)(ilogbf(sm) + 1));
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const uint8_t* tile = stage + tt * S::TILE;
+      for (int off = 1; off < 32; off <<= 1) need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, off));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[tt][k] = ex2(x[tt][k] - ref);
-        l += x[tt][k];
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top[nb] = fmaxf(top[nb], __shfl_xor_sync(0xffffffffu, top[nb], off));
+        const float m2 = fmaxf(m[nb], top[nb]);
+        const float alpha = m[nb] == -INFINITY ? 0.0f : ex2((m[nb] + rexp) - (m2 + need));
+        m[nb] = m2;
+        l[nb] *= alpha;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) pm[nb][gi] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 4 * G; ++i) o[nb][i][0] *= alpha, o[nb][i][1] *= alpha;
       }
+      rexp = need;
+      rscale = __int_as_float((127 + (int)need) << 23);
+    }
+    uint32_t pb[NB][2][G][2];
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
+    for (int nb = 0; nb < NB; ++nb) {
+      const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] + rexp - 14.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pm[gi] = fmaf(x[tt][k], fmaf(8.0f, vs[tt][k][gi], vm[tt][k][gi]), pm[gi]);
-        split_h2(x[tt][0] * vs[tt][0][gi], x[tt][1] * vs[tt][1][gi], pa[tt][gi][0], pa[tt][gi][1]);
-        split_h2(x[tt][2] * vs[tt][2][gi], x[tt][3] * vs[tt][3][gi], pa[tt][gi][2], pa[tt][gi][3]);
-      }
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p = ex2(x[nb][tt][i] - ref);
+          l[nb] += p;
+          // a hidden token's scale may be anything: 0 x NaN must not come through
+          const bool off = !whole && p == 0.0f;
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) {
+            const float w = off ? 0.0f : p * vs[tt][i][gi];
+            pm[nb][gi] = fmaf(p, off ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
+            const __half hi = __float2half_rn(w);
+            pb[nb][tt][gi][i] = transpose_8x8(h2_bits(__halves2half2(hi, __float2half_rn(w - __half2float(hi)))));
+          }
+        }
+    }
+    uint32_t vw[2][4][G];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = tile + KV_TILE * (HD / 2) + (t + 4 * i) * (HD / 2) + g * (HD / 16);
+        const uint8_t* p = stage + tt * S::TILE + KV_TILE * (HD / 2) + (t + 4 * i) * (HD / 2) + g * (HD / 16);
         if (G == 2) {
           const uint2 u = *reinterpret_cast<const uint2*>(p);
           vw[tt][i][0] = u.x, vw[tt][i][G - 1] = u.y;
@@ -585,7 +633,6 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
           vw[tt][i][0] = *reinterpret_cast<const uint32_t*>(p);
         }
       }
-    }
     // The tensor cores cut off what a product adds below the accumulator's last bit, always
     // towards zero; over a long context that bias would reach 1e-5.  So each unit's two products
     // start from zero and are added, high and low part together, in rounded fp32.
@@ -593,29 +640,35 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
 #pragma unroll
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-      for (int half = 0; half < 2; ++half)  // channels 8 g + 4 half + (0..3) of the group
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
-          float d[2][4] = {};
+        for (int pr = 0; pr < 2; ++pr) {  // channels 8 g + j and j + 1 of the group, j = 4 half + 2 pr
+          float d[NB][4];
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
             uint32_t ab = __byte_perm(vw[tt][0][gi], vw[tt][1][gi], half ? 0x7632 : 0x5410);
             uint32_t cd = __byte_perm(vw[tt][2][gi], vw[tt][3][gi], half ? 0x7632 : 0x5410);
             if (pr) ab >>= 8, cd >>= 8;
-            mma_f16(d[0], pa[tt][gi], h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032)),
-                    h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032)));
-            mma_f16(d[1], pa[tt][gi], h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72)),
-                    h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72)));
-          }
-          const int j = 8 * gi + 4 * half + 2 * pr;
+            const uint32_t a0 = h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032));
+            const uint32_t a1 = h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72));
+            const uint32_t a2 = h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032));
+            const uint32_t a3 = h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) o[j + i][0] += d[i][0] + d[i][2], o[j + i][1] += d[i][1] + d[i][3];
+            for (int nb = 0; nb < NB; ++nb) {
+              if (tt == 0) mma_f16_zero(d[nb], a0, a1, a2, a3, pb[nb][tt][gi]);
+              else mma_f16(d[nb], a0, a1, a2, a3, pb[nb][tt][gi]);
+            }
+          }
+          const int i = 4 * gi + 2 * half + pr;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) o[nb][i][0] += d[nb][0] + d[nb][1], o[nb][i][1] += d[nb][2] + d[nb][3];
         }
     __syncwarp();  // every lane has read the stage
     if (n + KVA_STAGES < mine) {
-      issue(n + KVA_STAGES, unit + KVA_STAGES * stride, ahead);
+      issue(st, unit + KVA_STAGES * stride, ahead);
       ahead = n + 1 + KVA_STAGES < mine ? look_up(unit + (KVA_STAGES + 1) * stride) : -1;
     }
+    if (++st == KVA_STAGES) st = 0, phase ^= 1;
   }
   if (!fine) {  // given up: no copy may be in flight when the rings are used again
     if (lane == 0)
@@ -623,70 +676,69 @@ __global__ void __launch_bounds__(KVA_THREADS, 3) k_kv4_attn(const KvAttnArgs a)
     __syncwarp();
   }
   // join the warps
-#pragma unroll
-  for (int off = 1; off < 4; off <<= 1) {
-    l += __shfl_xor_sync(0xffffffffu, l, off);
-#pragma unroll
-    for (int gi = 0; gi < G; ++gi) pm[gi] += __shfl_xor_sync(0xffffffffu, pm[gi], off);
-  }
   __syncthreads();
-  float* wout = reinterpret_cast<float*>(smem) + (size_t)warp * 8 * S::OUT_LD;
+  float* wout = reinterpret_cast<float*>(smem) + (size_t)warp * ROWS * S::OUT_LD;
 #pragma unroll
-  for (int gi = 0; gi < G; ++gi)
+  for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int off = 4; off < 32; off <<= 1) {
+      l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], off);
 #pragma unroll
-      for (int q4 = 0; q4 < 2; ++q4) {
-        float4 v;
-        float* pv = &v.x;
+      for (int gi = 0; gi < G; ++gi) pm[nb][gi] += __shfl_xor_sync(0xffffffffu, pm[nb][gi], off);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pv[j] = o[8 * gi + 4 * q4 + j][c] + pm[gi];
-        *reinterpret_cast<float4*>(wout + g * S::OUT_LD + 64 * gi + 16 * t + 8 * c + 4 * q4) = v;
+    for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float(&d0)[2] = o[nb][4 * gi + 2 * half];
+        const float(&d1)[2] = o[nb][4 * gi + 2 * half + 1];
+        *reinterpret_cast<float4*>(wout + (4 * nb + t) * S::OUT_LD + 64 * gi + 8 * g + 4 * half) =
+            make_float4(d0[0] + pm[nb][gi], d0[1] + pm[nb][gi], d1[0] + pm[nb][gi], d1[1] + pm[nb][gi]);
       }
-  if (t == 0) {
-    // a row of NaN scores has no maximum, but its sum is NaN and has to come through
-    ml[warp * 16 + g] = m > -INFINITY ? m + rexp : l == l ? -INFINITY : 0.0f;
-    ml[warp * 16 + 8 + g] = l;
+    if (g == 0) {
+      // a row of NaN scores has no maximum, but its sum is NaN and has to come through
+      ml[warp * 2 * ROWS + 4 * nb + t] = m[nb] > -INFINITY ? m[nb] + rexp : l[nb] == l[nb] ? -INFINITY : 0.0f;
+      ml[warp * 2 * ROWS + ROWS + 4 * nb + t] = l[nb];
+    }
   }
   __syncthreads();
-  float* cout = reinterpret_cast<float*>(smem) + KVA_WARPS * 8 * S::OUT_LD;
-  for (int i = threadIdx.x; i < 8 * HD; i += KVA_THREADS) {
-    const int r = i / HD, c = i % HD;
+  float* cout = reinterpret_cast<float*>(smem) + KVA_WARPS * ROWS * S::OUT_LD;
+  for (int i = threadIdx.x; i < ROWS * HD; i += KVA_THREADS) {
+    const int r = i / HD, c = i % HD, q = row0 + r;
+    if (q >= rows) break;
     float top = -INFINITY, sum = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < KVA_WARPS; ++w) top = fmaxf(top, ml[w * 16 + r]);
+    for (int w = 0; w < KVA_WARPS; ++w) top = fmaxf(top, ml[w * 2 * ROWS + r]);
 #pragma unroll
     for (int w = 0; w < KVA_WARPS; ++w) {
-      const float f = ml[w * 16 + r] == -INFINITY ? 0.0f : ex2(ml[w * 16 + r] - top);
+      const float mw = ml[w * 2 * ROWS + r], f = mw == -INFINITY ? 0.0f : ex2(mw - top);
       if (f > 0.0f) {
-        sum = fmaf(f, ml[w * 16 + 8 + r], sum);
-        y = fmaf(f, reinterpret_cast<float*>(smem)[(w * 8 + r) * S::OUT_LD + c], y);
+        sum = fmaf(f, ml[w * 2 * ROWS + ROWS + r], sum);
+        y = fmaf(f, reinterpret_cast<float*>(smem)[(w * ROWS + r) * S::OUT_LD + c], y);
       }
     }
     if (splits == 1) {
-      const int q = row0 + r;
-      if (q < rows)
-        a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
-            top == -INFINITY ? 0.0f : y / sum;
+      a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
+          top == -INFINITY ? 0.0f : y / sum;
     } else {
       cout[r * S::OUT_LD + c] = y;
-      if (c == 0) ml[KVA_WARPS * 16 + r] = top, ml[KVA_WARPS * 16 + 8 + r] = sum;
+      if (c == 0) ml[KVA_WARPS * 2 * ROWS + r] = top, ml[KVA_WARPS * 2 * ROWS + ROWS + r] = sum;
     }
   }
   if (splits == 1) return;
   // join the CTAs of the cluster, each writing its share of the outputs
   cluster_sync();
-  const uint32_t cout_s = sbase + KVA_WARPS * 8 * S::OUT_LD * 4, ml_s = sbase + S::ML + KVA_WARPS * 64;
-  for (int i = rank * KVA_THREADS + threadIdx.x; i < 8 * HD; i += splits * KVA_THREADS) {
+  const uint32_t cout_s = sbase + KVA_WARPS * ROWS * S::OUT_LD * 4, ml_s = sbase + S::ML + KVA_WARPS * 2 * ROWS * 4;
+  for (int i = rank * KVA_THREADS + threadIdx.x; i < ROWS * HD; i += splits * KVA_THREADS) {
     const int r = i / HD, c = i % HD, q = row0 + r;
-    if (q >= rows) continue;
+    if (q >= rows) break;
     float top = -INFINITY, sum = 0.0f, y = 0.0f;
     for (int s = 0; s < splits; ++s) top = fmaxf(top, ld_cluster_f32(mapa_shared(ml_s + r * 4, s)));
     for (int s = 0; s < splits; ++s) {
       const float ms = ld_cluster_f32(mapa_shared(ml_s + r * 4, s));
       const float f = ms == -INFINITY ? 0.0f : ex2(ms - top);
       if (f > 0.0f) {
-        sum = fmaf(f, ld_cluster_f32(mapa_shared(ml_s + 32 + r * 4, s)), sum);
+        sum = fmaf(f, ld_cluster_f32(mapa_shared(ml_s + ROWS * 4 + r * 4, s)), sum);
         y = fmaf(f, ld_cluster_f32(mapa_shared(cout_s + (r * S::OUT_LD + c) * 4, s)), y);
       }
     }

@@ -212,7 +212,7 @@ int kv4_rows(envg_kv4 c, float* k, int64_t ldk, float* v, int64_t ldv, const int
   return finish_call(d, flags);
 }
 
-// CTAs that share one (sequence, kv head, eight rows): enough for two waves of three CTAs per SM,
+// CTAs that share one (sequence, kv head, row tile): enough for two waves of three CTAs per SM,
 // as long as each warp keeps a unit of two tiles.  A power of two up to 8 (the portable cluster).
 int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
   int s = 1;
@@ -220,15 +220,15 @@ int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
   return s;
 }
 
-template <int HD>
+template <int HD, int NB>
 int launch_kv4_attn_t(Dev* d, const KvAttnArgs& a, int splits) {
-  using S = KvaSmem<HD>;
+  using S = KvaSmem<HD, NB>;
   static bool attr_set[64] = {};
   if (!attr_set[d->id]) {
-    ENVG_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+    ENVG_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
     attr_set[d->id] = true;
   }
-  const int64_t tiles = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, 8) * a.c.kv_heads;
+  const int64_t tiles = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, S::ROWS) * a.c.kv_heads;
   if (tiles > 65535 || a.batch > 65535) return fail(ENVG_ERR_UNSUPPORTED, "attention_kv4: batch %d x %lld row tiles is too large", a.batch, (long long)tiles);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)tiles, (unsigned)a.batch);
@@ -249,7 +249,7 @@ int launch_kv4_attn_t(Dev* d, const KvAttnArgs& a, int splits) {
   }
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)n;
-  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_kv4_attn<HD>, a));
+  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_kv4_attn<HD, NB>, a));
   d->st.kernel_launches++;
   return ENVG_OK;
 }
@@ -259,9 +259,13 @@ int launch_kv4_attn(Dev* d, const KvAttnArgs& a, int max_ctx) {
   const double seen = a.window > 0 ? std::min<double>(max_ctx, (double)a.window + a.sinks + a.q_len) : max_ctx;
   ProfScope ps(stream_of(d), KID_KV4_ATTN, 4.0 * a.hd * a.heads * (double)rows * seen,
                seen * a.batch * a.c.kv_heads * (a.hd + 8 * (a.hd / KV_GROUP)) + 8.0 * (double)rows * a.heads * a.hd);
-  const int64_t groups = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, 8) * a.c.kv_heads * a.batch;
-  const int splits = kv4_splits(d, groups, (int64_t)seen);
-  return a.hd == 128 ? launch_kv4_attn_t<128>(d, a, splits) : launch_kv4_attn_t<64>(d, a, splits);
+  // rows that read one kv head: 4, 8 or 16 at a time
+  const int64_t shared = (int64_t)(a.heads / a.c.kv_heads) * a.q_len;
+  const int nb = shared <= 4 ? 1 : shared <= 8 ? 2 : 4;
+  const int splits = kv4_splits(d, cdiv(shared, 4 * nb) * a.c.kv_heads * a.batch, (int64_t)seen);
+  if (a.hd == 128)
+    return nb == 1 ? launch_kv4_attn_t<128, 1>(d, a, splits) : nb == 2 ? launch_kv4_attn_t<128, 2>(d, a, splits) : launch_kv4_attn_t<128, 4>(d, a, splits);
+  return nb == 1 ? launch_kv4_attn_t<64, 1>(d, a, splits) : nb == 2 ? launch_kv4_attn_t<64, 2>(d, a, splits) : launch_kv4_attn_t<64, 4>(d, a, splits);
 }
 
 }  // namespace
@@ -593,6 +597,7 @@ int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, env
   a.window = window, a.sinks = sinks;
   a.sl2 = scale * 1.4426950408889634f;
   a.wait_cap_ns = d->wait_cap_ns;
+  a.vec = f4_ok(a.q, a.ldq);
   const int64_t most = table_stride * cache->page_size;
   ENVG_TRY(launch_kv4_attn(d, a, (int)(max_ctx > 0 ? std::min<int64_t>(max_ctx, most) : most)));
   if (!devp) ENVG_TRY(st.out(io, dst, ldo, rows, width));
