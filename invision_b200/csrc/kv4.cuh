@@ -308,6 +308,26 @@ ENVG_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// An output's sum: the high and the low parts' apart where registers allow (one packed addition
+// instead of two), else together in x.
+template <bool APART>
+ENVG_DEV void acc_add(float2& o, float x, float y) {
+  if (APART)
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(o.x), "+f"(o.y)
+        : "f"(x), "f"(y));
+  else
+    o.x += x + y;
+}
+template <bool APART>
+ENVG_DEV void acc_scale(float2& o, float f) {
+  if (APART)
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(o.x), "+f"(o.y)
+        : "f"(f));
+  else
+    o.x *= f;
+}
 ENVG_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
@@ -366,38 +386,45 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   const int n_tiles = p_hi < 0 ? 0 : n_sink + p_hi / KV_TILE - first + 1;
   const int units = (n_tiles + 1) / 2, stride = splits * KVA_WARPS, u0 = rank * KVA_WARPS + warp;
 
-  // ring of bulk copies: lanes 0 and 1 each bring one tile of a unit
+  // Ring of bulk copies.  Sixteen units at a time, each lane looks up one tile and later brings it:
+  // lanes 2 (n % 16) and 2 (n % 16) + 1 those of the warp's n-th unit.
   const int per_page = a.c.page_size / KV_TILE;
   const int32_t* table = a.c.table + (int64_t)b * a.c.table_stride;
-  auto tile_of = [&](int unit) { const int i = 2 * unit + (lane & 1); return i < n_sink ? i : first + i - n_sink; };
-  auto look_up = [&](int unit) -> int32_t {  // the page of the lane's tile, -1 past the end
-    if (lane >= 2 || 2 * unit + lane >= n_tiles) return -1;
-    return __ldg(table + tile_of(unit) / per_page);
+  const int mine = u0 < units ? (units - u0 + stride - 1) / stride : 0;  // units of this warp
+  auto tile_at = [&](int batch) { const int i = 2 * (u0 + (16 * batch + (lane >> 1)) * stride) + (lane & 1); return i >= n_tiles ? -1 : i < n_sink ? i : first + i - n_sink; };
+  auto look_up = [&](int batch) -> int32_t {
+    const int tile = 16 * batch < mine ? tile_at(batch) : -1;
+    return tile >= 0 ? __ldg(table + tile / per_page) : -1;
   };
-  uint32_t there = 0;  // two bits per stage: which tiles of the unit exist
-  auto issue = [&](int st, int unit, int32_t page) {
-    bool ok = lane < 2 && 2 * unit + lane < n_tiles;
-    if (ok && (page < 0 || page >= a.c.pages)) {
-      kv_flag(a.c.status, SITE_KV_PAGE);
-      ok = false;
+  int32_t ahead = look_up(0);
+  const uint8_t* src = nullptr;
+  uint32_t there = 0, there_next = 0;  // tiles that exist: of the batch being worked on, being brought
+  auto issue = [&](int n, int st) {
+    if ((n & 15) == 0) {
+      const int tile = tile_at(n >> 4);
+      bool ok = tile >= 0;
+      if (ok && (ahead < 0 || ahead >= a.c.pages)) {
+        kv_flag(a.c.status, SITE_KV_PAGE);
+        ok = false;
+      }
+      src = ok ? a.c.base + (((int64_t)ahead * a.c.kv_heads + kvh) * per_page + tile % per_page) * S::TILE : nullptr;
+      there_next = __ballot_sync(0xffffffffu, ok);
+      ahead = look_up((n >> 4) + 1);
     }
-    const uint32_t vote = __ballot_sync(0xffffffffu, ok) & 3u;
-    there = (there & ~(3u << (2 * st))) | (vote << (2 * st));
-    if (lane < 2) {
+    if ((lane >> 1) == (n & 15)) {
       const uint32_t bar = bars + 8 * st;
-      if (ok) {
+      if (src) {
         mbar_arrive_expect_tx(bar, S::TILE);
-        const int tile = tile_of(unit);
-        const uint8_t* src = a.c.base + (((int64_t)page * a.c.kv_heads + kvh) * per_page + tile % per_page) * S::TILE;
-        bulk_load(ring + st * S::STAGE + lane * S::TILE, src, S::TILE, bar);
+        bulk_load(ring + st * S::STAGE + (lane & 1) * S::TILE, src, S::TILE, bar);
       } else {
         mbar_arrive(bar);
       }
     }
   };
-  const int mine = u0 < units ? (units - u0 + stride - 1) / stride : 0;  // units of this warp
-  for (int n = 0; n < KVA_STAGES && n < mine; ++n) issue(n, u0 + n * stride, look_up(u0 + n * stride));
-  int32_t ahead = KVA_STAGES < mine ? look_up(u0 + KVA_STAGES * stride) : -1;
+  for (int n = 0; n < KVA_STAGES && n < mine; ++n) issue(n, n);
+  // tiles [w_lo, w_hi) and [0, w_sink) of the list are seen whole by every row of the CTA
+  const int w_hi = n_sink + (p_lo + 1) / KV_TILE - first, w_sink = min(n_sink, a.sinks / KV_TILE);
+  const int w_lo = n_sink + (a.window > 0 ? max(0, p_hi - a.window) / KV_TILE + 1 - first : 0);
 
   // q: column g of an operand is part g % 2 of row g / 2, scaled to [2^14, 2^15) before the split,
   // in the order of the K words' nibbles; a thread's scores are those of row t
@@ -452,14 +479,15 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       }
   }
 
-  float o[NB][4 * G][2], m[NB], l[NB], pm[NB][G];
+  float2 o[NB][4 * G][2];  // [.][.][row half]: sums of the high and of the low parts
+  float m[NB], l[NB], pm[NB][G];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     m[nb] = -INFINITY, l[nb] = 0.0f;
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) pm[nb][gi] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = 0.0f;
+    for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = make_float2(0.0f, 0.0f);
   }
   float rexp = -32.0f, rscale = 0.0f;  // no V scale seen is above rscale = 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
@@ -474,7 +502,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       break;
     }
     const uint8_t* stage = smem + warp * S::RING + st * S::STAGE;
-    const uint32_t vote = (there >> (2 * st)) & 3u;
+    if ((n & 15) == 0) there = there_next;
+    const uint32_t vote = (there >> (2 * (n & 15))) & 3u;
     // scores of tokens g and g + 8 of each tile, log2 units
     float x[NB][2][2], vs[2][2][G], vm[2][2][G];
     __half2 smax = bits_h2(0u);
@@ -510,24 +539,24 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       for (int nb = 0; nb < NB; ++nb) x[nb][tt][0] = x[nb][tt][1] = mn[nb][0] = mn[nb][1] = 0.0f;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        float d[NB][4];
+        // two chains of two products, added in rounded fp32 (see the outputs below)
+        float d[2][NB][4];
 #pragma unroll
-        for (int w = 2 * gi; w < 2 * gi + 2; ++w) {
+        for (int h = 0; h < 2; ++h) {
+          const int w = 2 * gi + h;
           const uint32_t u0w = kw[0][w], u1w = kw[1][w], y0 = u0w >> 8, y1 = u1w >> 8;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            if (w == 2 * gi)
-              mma_f16_zero(d[nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
-            else
-              mma_f16(d[nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
-            mma_f16(d[nb], y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[nb][2 * w + 1]);
+            mma_f16_zero(d[h][nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
+            mma_f16(d[h][nb], y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[nb][2 * w + 1]);
           }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            x[nb][tt][i] = fmaf(d[nb][2 * i] + d[nb][2 * i + 1], ks[i][gi], x[nb][tt][i]);
+            const float sum = (d[0][nb][2 * i] + d[1][nb][2 * i]) + (d[0][nb][2 * i + 1] + d[1][nb][2 * i + 1]);
+            x[nb][tt][i] = fmaf(sum, ks[i][gi], x[nb][tt][i]);
             mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);
           }
       }
@@ -538,21 +567,14 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     }
     // masks: only where a row of the CTA does not see the whole unit.  A row hides a token by its
     // score; its scale and minimum are dropped where no row sees it (they may hold anything there).
-    bool whole = vote == 3u;
-    int j0[2];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const int i = 2 * unit + tt;
-      j0[tt] = (i < n_sink ? i : first + i - n_sink) * KV_TILE;
-      whole = whole && j0[tt] + KV_TILE - 1 <= p_lo && (a.window <= 0 || j0[tt] > p_hi - a.window || j0[tt] + KV_TILE <= a.sinks);
-    }
+    const bool whole = vote == 3u && ((2 * unit >= w_lo && 2 * unit + 1 < w_hi) || 2 * unit + 1 < w_sink);
     if (!whole) {
       smax = bits_h2(0u);
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int j = j0[tt] + g + 8 * i;
+          const int at = 2 * unit + tt, j = (at < n_sink ? at : first + at - n_sink) * KV_TILE + g + 8 * i;
           bool any = false;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
@@ -594,12 +616,15 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) pm[nb][gi] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 4 * G; ++i) o[nb][i][0] *= alpha, o[nb][i][1] *= alpha;
+        for (int i = 0; i < 4 * G; ++i) acc_scale<NB == 1>(o[nb][i][0], alpha), acc_scale<NB == 1>(o[nb][i][1], alpha);
       }
       rexp = need;
       rscale = __int_as_float((127 + (int)need) << 23);
     }
     uint32_t pb[NB][2][G][2];
+    // a token that one thread's row sees may be hidden from its other rows: 0 x NaN must not come
+    // through there (with one row to a thread, what it does not see is zero already)
+    auto hidden = [&](float p) { return NB > 1 && !whole && p == 0.0f; };
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] + rexp - 14.0f;
@@ -609,12 +634,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
         for (int i = 0; i < 2; ++i) {
           const float p = ex2(x[nb][tt][i] - ref);
           l[nb] += p;
-          // a hidden token's scale may be anything: 0 x NaN must not come through
-          const bool off = !whole && p == 0.0f;
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
-            const float w = off ? 0.0f : p * vs[tt][i][gi];
-            pm[nb][gi] = fmaf(p, off ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
+            const float w = hidden(p) ? 0.0f : p * vs[tt][i][gi];
+            pm[nb][gi] = fmaf(p, hidden(p) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
             const __half hi = __float2half_rn(w);
             pb[nb][tt][gi][i] = transpose_8x8(h2_bits(__halves2half2(hi, __float2half_rn(w - __half2float(hi)))));
           }
@@ -661,13 +684,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           }
           const int i = 4 * gi + 2 * half + pr;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[nb][i][0] += d[nb][0] + d[nb][1], o[nb][i][1] += d[nb][2] + d[nb][3];
+          for (int nb = 0; nb < NB; ++nb) acc_add<NB == 1>(o[nb][i][0], d[nb][0], d[nb][1]), acc_add<NB == 1>(o[nb][i][1], d[nb][2], d[nb][3]);
         }
     __syncwarp();  // every lane has read the stage
-    if (n + KVA_STAGES < mine) {
-      issue(st, unit + KVA_STAGES * stride, ahead);
-      ahead = n + 1 + KVA_STAGES < mine ? look_up(unit + (KVA_STAGES + 1) * stride) : -1;
-    }
+    if (n + KVA_STAGES < mine) issue(n + KVA_STAGES, st);
     if (++st == KVA_STAGES) st = 0, phase ^= 1;
   }
   if (!fine) {  // given up: no copy may be in flight when the rings are used again
@@ -690,10 +710,11 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float(&d0)[2] = o[nb][4 * gi + 2 * half];
-        const float(&d1)[2] = o[nb][4 * gi + 2 * half + 1];
+        const float2(&d0)[2] = o[nb][4 * gi + 2 * half];
+        const float2(&d1)[2] = o[nb][4 * gi + 2 * half + 1];
         *reinterpret_cast<float4*>(wout + (4 * nb + t) * S::OUT_LD + 64 * gi + 8 * g + 4 * half) =
-            make_float4(d0[0] + pm[nb][gi], d0[1] + pm[nb][gi], d1[0] + pm[nb][gi], d1[1] + pm[nb][gi]);
+            make_float4(d0[0].x + d0[0].y + pm[nb][gi], d0[1].x + d0[1].y + pm[nb][gi], d1[0].x + d1[0].y + pm[nb][gi],
+                        d1[1].x + d1[1].y + pm[nb][gi]);
       }
     if (g == 0) {
       // a row of NaN scores has no maximum, but its sum is NaN and has to come through
