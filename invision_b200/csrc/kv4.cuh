@@ -308,6 +308,17 @@ ENVG_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (v & mask) | magic in one instruction: both constants stay in registers.
+ENVG_DEV uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
+  return r;
+}
+ENVG_DEV uint32_t in_register(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // An output's sum: the high and the low parts' apart where registers allow (one packed addition
 // instead of two), else together in x.
 template <bool APART>
@@ -491,6 +502,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   }
   float rexp = -32.0f, rscale = 0.0f;  // no V scale seen is above rscale = 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
+  const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
   bool fine = true;
   int st = 0;
   uint32_t phase = 0;
@@ -638,8 +650,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           for (int gi = 0; gi < G; ++gi) {
             const float w = hidden(p) ? 0.0f : p * vs[tt][i][gi];
             pm[nb][gi] = fmaf(p, hidden(p) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
-            const __half hi = __float2half_rn(w);
-            pb[nb][tt][gi][i] = transpose_8x8(h2_bits(__halves2half2(hi, __float2half_rn(w - __half2float(hi)))));
+            // one conversion rounds w to its high part again beside the low part
+            pb[nb][tt][gi][i] = transpose_8x8(h2_bits(__floats2half2_rn(w, w - __half2float(__float2half_rn(w)))));
           }
         }
     }
@@ -672,10 +684,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
             uint32_t ab = __byte_perm(vw[tt][0][gi], vw[tt][1][gi], half ? 0x7632 : 0x5410);
             uint32_t cd = __byte_perm(vw[tt][2][gi], vw[tt][3][gi], half ? 0x7632 : 0x5410);
             if (pr) ab >>= 8, cd >>= 8;
-            const uint32_t a0 = h2_bits(__hadd2(bits_h2((ab & 0x000F000Fu) | 0x64006400u), c1032));
-            const uint32_t a1 = h2_bits(__hfma2(bits_h2((ab & 0x00F000F0u) | 0x64006400u), c16, c72));
-            const uint32_t a2 = h2_bits(__hadd2(bits_h2((cd & 0x000F000Fu) | 0x64006400u), c1032));
-            const uint32_t a3 = h2_bits(__hfma2(bits_h2((cd & 0x00F000F0u) | 0x64006400u), c16, c72));
+            const uint32_t a0 = h2_bits(__hadd2(bits_h2(and_or(ab, mask0, magic)), c1032));
+            const uint32_t a1 = h2_bits(__hfma2(bits_h2(and_or(ab, mask1, magic)), c16, c72));
+            const uint32_t a2 = h2_bits(__hadd2(bits_h2(and_or(cd, mask0, magic)), c1032));
+            const uint32_t a3 = h2_bits(__hfma2(bits_h2(and_or(cd, mask1, magic)), c16, c72));
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
               if (tt == 0) mma_f16_zero(d[nb], a0, a1, a2, a3, pb[nb][tt][gi]);
