@@ -354,7 +354,7 @@ int envg_quantize_q4(const uint16_t* w_bf16, const float* w_f32, int64_t N, int6
 /* Uploads a 4-bit weight W[n][k] = (c - z) s in the form envg_quantize_q4 writes; zeros may be
  * NULL (z = 8 throughout), its entries are 0..15.  codes, scales and zeros are host or device
  * pointers by `flags`; they may be freed after the call.  layout_flags: ENVG_LAYOUT_PLAIN or
- * ENVG_LAYOUT_GATE_UP.  The codes are re-laid out once, here, for the kernels. */
+ * ENVG_LAYOUT_GATE_UP.  K is at most 57344.  The codes are re-laid out once, here, for the kernels. */
 int envg_weight_upload_q4(const uint8_t* codes, const float* scales, const uint8_t* zeros, int64_t N,
                           int64_t K, int group, int layout_flags, int flags, envg_q4weight* out);
 int envg_q4weight_free(envg_q4weight w);

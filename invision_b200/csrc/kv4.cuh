@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "mma16.cuh"
 #include "ptx.cuh"
 
 namespace envg {
@@ -67,18 +68,6 @@ ENVG_DEV uint8_t* kv_tile(const Kv4View& c, int b, int h, int pos, int tile_byte
   }
   const int64_t per_page = c.page_size / KV_TILE;
   return c.base + (((int64_t)page * c.kv_heads + h) * per_page + (pos % c.page_size) / KV_TILE) * tile_bytes;
-}
-
-ENVG_DEV float4 ld_f4(const float* p, bool vec) {
-  if (vec) return *reinterpret_cast<const float4*>(p);
-  return make_float4(p[0], p[1], p[2], p[3]);
-}
-ENVG_DEV void st_f4(float* p, float4 v, bool vec) {
-  if (vec) {
-    *reinterpret_cast<float4*>(p) = v;
-  } else {
-    p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
-  }
 }
 
 // ---- norm of queries and keys per head + position rotation ------------------------------------
@@ -271,9 +260,9 @@ struct KvAttnArgs {
 // Mathematics.  The rows are (query token, head) pairs that read the same kv head.  A row's score
 // of token j is sum_g s_jg (q_g . c_jg) + m_jg sum(q_g) over its groups of 64 channels, and its
 // output sum_j p_j (s_jg (c_jg - 8) + (m_jg + 8 s_jg)).  Both products with codes run on the
-// tensor cores as m16n8k16 with fp16 operands and fp32 sums, exactly in the codes: a code is a
-// subnormal fp16 (c 2^-24, or 16 c 2^-24) for K, c - 8 for V (centred: the positive codes' sum
-// would be far larger than the outputs and cost its last bits).  The codes are the 16-row operand
+// tensor cores as m16n8k16 with fp16 operands and fp32 sums, exactly in the codes, which go in as
+// c - 8 (centred: the positive codes' sums would be far larger than the result and cost its last
+// bits), so that the minimum becomes the middle m + 8 s.  The codes are the 16-row operand
 // (16 tokens of K, 16 channels of V^T), so a code is unpacked once for all rows; q and p s are the
 // 8-column one, each split into two fp16 parts in adjacent columns, so that fp32 accuracy costs no
 // further instruction.  q is scaled by a power of two per row, p s by the row maximum and by the
@@ -284,72 +273,6 @@ struct KvAttnArgs {
 // of CTAs (one cluster per sequence, kv head and 4 NB rows).  Each warp runs a one-pass softmax
 // with its own ring of bulk copies; the warps' (max, sum, output) are joined in shared memory, the
 // CTAs' through distributed shared memory in rank order: no workspace, no atomics, one launch.
-ENVG_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
-}
-// The same from a zero accumulator.
-ENVG_DEV void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.0f));
-}
-// Transpose of an 8 x 8 matrix of halves; thread 4 r + c holds row r, columns 2 c and 2 c + 1.
-ENVG_DEV uint32_t transpose_8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-ENVG_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-ENVG_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-ENVG_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// (v & mask) | magic in one instruction: both constants stay in registers.
-ENVG_DEV uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
-  return r;
-}
-ENVG_DEV uint32_t in_register(uint32_t v) {
-  uint32_t r;
-  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-// An output's sum: the high and the low parts' apart where registers allow (one packed addition
-// instead of two), else together in x.
-template <bool APART>
-ENVG_DEV void acc_add(float2& o, float x, float y) {
-  if (APART)
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(o.x), "+f"(o.y)
-        : "f"(x), "f"(y));
-  else
-    o.x += x + y;
-}
-template <bool APART>
-ENVG_DEV void acc_scale(float2& o, float f) {
-  if (APART)
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(o.x), "+f"(o.y)
-        : "f"(f));
-  else
-    o.x *= f;
-}
-ENVG_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
-               : "memory");
-}
-ENVG_DEV float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 3;
 constexpr int SITE_KVA_RING = 60;  // status[1] of a ring wait that ran out
 
@@ -471,12 +394,12 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
     }
-    cq[nb] = __int_as_float((127 - __shfl_sync(0xffffffffu, e, from)) << 23) * (16777216.0f * a.sl2);
+    cq[nb] = __int_as_float((127 - __shfl_sync(0xffffffffu, e, from)) << 23) * a.sl2;
     const int mr = row0 + 4 * nb + t;
     pos[nb] = mr < rows ? len - a.q_len + mr / per_kv : -1;
 #pragma unroll
     for (int j = 0; j < 16 * G; ++j) {
-      const float v = x[j] * (((j & 7) & 1) ? up * 0.0625f : up);
+      const float v = x[j] * up;
       const __half hi = __float2half_rn(v);
       x[j] = (g & 1) ? v - __half2float(hi) : v;
     }
@@ -490,19 +413,21 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       }
   }
 
-  float2 o[NB][4 * G][2];  // [.][.][row half]: sums of the high and of the low parts
-  float m[NB], l[NB], pm[NB][G];
+  float o[NB][4 * G][2], m[NB], l[NB], pm[NB][G];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     m[nb] = -INFINITY, l[nb] = 0.0f;
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) pm[nb][gi] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = 0.0f;
   }
   float rexp = -32.0f, rscale = 0.0f;  // no V scale seen is above rscale = 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
+  // c into the mantissa of 1024, then - 1032; 16 c, then x 1/16 - 72 (a bare c would be a subnormal,
+  // which the cores align by its nominal exponent and so lose up to ten low bits of the other factor)
   const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
+  const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
   bool fine = true;
   int st = 0;
   uint32_t phase = 0;
@@ -546,6 +471,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           kw[i][0] = k2.x, kw[i][1] = k2.y;
         }
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) km[i][gi] = fmaf(8.0f, ks[i][gi], km[i][gi]);
       float mn[NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) x[nb][tt][0] = x[nb][tt][1] = mn[nb][0] = mn[nb][1] = 0.0f;
@@ -556,11 +485,18 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int w = 2 * gi + h;
-          const uint32_t u0w = kw[0][w], u1w = kw[1][w], y0 = u0w >> 8, y1 = u1w >> 8;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            mma_f16_zero(d[h][nb], u0w & 0x000F000Fu, u1w & 0x000F000Fu, u0w & 0x00F000F0u, u1w & 0x00F000F0u, qb[nb][2 * w]);
-            mma_f16(d[h][nb], y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[nb][2 * w + 1]);
+          for (int b8 = 0; b8 < 2; ++b8) {
+            const uint32_t u0 = b8 ? kw[0][w] >> 8 : kw[0][w], u1 = b8 ? kw[1][w] >> 8 : kw[1][w];
+            const uint32_t a0 = h2_bits(__hadd2(bits_h2(and_or(u0, mask0, magic)), c1032));
+            const uint32_t a1 = h2_bits(__hadd2(bits_h2(and_or(u1, mask0, magic)), c1032));
+            const uint32_t a2 = h2_bits(__hfma2(bits_h2(and_or(u0, mask1, magic)), c16, c72));
+            const uint32_t a3 = h2_bits(__hfma2(bits_h2(and_or(u1, mask1, magic)), c16, c72));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              if (b8 == 0) mma_f16_zero(d[h][nb], a0, a1, a2, a3, qb[nb][2 * w]);
+              else mma_f16(d[h][nb], a0, a1, a2, a3, qb[nb][2 * w + 1]);
+            }
           }
         }
 #pragma unroll
@@ -569,7 +505,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           for (int i = 0; i < 2; ++i) {
             const float sum = (d[0][nb][2 * i] + d[1][nb][2 * i]) + (d[0][nb][2 * i + 1] + d[1][nb][2 * i + 1]);
             x[nb][tt][i] = fmaf(sum, ks[i][gi], x[nb][tt][i]);
-            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);
+            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);  // km: the middle
           }
       }
 #pragma unroll
@@ -628,7 +564,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) pm[nb][gi] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 4 * G; ++i) acc_scale<NB == 1>(o[nb][i][0], alpha), acc_scale<NB == 1>(o[nb][i][1], alpha);
+        for (int i = 0; i < 4 * G; ++i) o[nb][i][0] *= alpha, o[nb][i][1] *= alpha;
       }
       rexp = need;
       rscale = __int_as_float((127 + (int)need) << 23);
@@ -671,7 +607,6 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     // The tensor cores cut off what a product adds below the accumulator's last bit, always
     // towards zero; over a long context that bias would reach 1e-5.  So each unit's two products
     // start from zero and are added, high and low part together, in rounded fp32.
-    const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
 #pragma unroll
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
@@ -696,7 +631,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           }
           const int i = 4 * gi + 2 * half + pr;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) acc_add<NB == 1>(o[nb][i][0], d[nb][0], d[nb][1]), acc_add<NB == 1>(o[nb][i][1], d[nb][2], d[nb][3]);
+          for (int nb = 0; nb < NB; ++nb) o[nb][i][0] += d[nb][0] + d[nb][1], o[nb][i][1] += d[nb][2] + d[nb][3];
         }
     __syncwarp();  // every lane has read the stage
     if (n + KVA_STAGES < mine) issue(n + KVA_STAGES, st);
@@ -722,11 +657,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float2(&d0)[2] = o[nb][4 * gi + 2 * half];
-        const float2(&d1)[2] = o[nb][4 * gi + 2 * half + 1];
+        const float(&d0)[2] = o[nb][4 * gi + 2 * half];
+        const float(&d1)[2] = o[nb][4 * gi + 2 * half + 1];
         *reinterpret_cast<float4*>(wout + (4 * nb + t) * S::OUT_LD + 64 * gi + 8 * g + 4 * half) =
-            make_float4(d0[0].x + d0[0].y + pm[nb][gi], d0[1].x + d0[1].y + pm[nb][gi], d1[0].x + d1[0].y + pm[nb][gi],
-                        d1[1].x + d1[1].y + pm[nb][gi]);
+            make_float4(d0[0] + pm[nb][gi], d0[1] + pm[nb][gi], d1[0] + pm[nb][gi], d1[1] + pm[nb][gi]);
       }
     if (g == 0) {
       // a row of NaN scores has no maximum, but its sum is NaN and has to come through

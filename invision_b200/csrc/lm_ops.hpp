@@ -6,6 +6,7 @@
 namespace {
 constexpr uint32_t Q4_MAGIC = 0xE17A9E44u;
 constexpr uint32_t KV4_MAGIC = 0xE17A9E4Cu;
+constexpr int Q4_MAX_K = 57344;  // eight CTAs' shared memory holds four rows of x of this length
 }  // namespace
 
 struct envg_q4weight_s {
@@ -89,12 +90,80 @@ int finish_call(Dev* d, int flags) {
   return ENVG_OK;
 }
 
+// How a 4-bit linear is spread over the SMs (one CTA each): the cluster size, a power of two, that
+// leaves the least work on the busiest CTA, counted in blocks plus a fixed cost per cluster
+// exchange, among those whose part of x leaves room for a ring.
+template <int NT>
+bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
+  using S = Q4Smem<NT>;
+  double least = 0.0;
+  bool found = false;
+  for (int s = 1; s <= 8; s *= 2) {
+    const int kb = (int)cdiv(w.kblocks, s);
+    const int room = Q4_SMEM - S::FIXED - S::x_bytes(kb);
+    const int stages = std::min(Q4_MAX_STAGES, room / (Q4_WARPS * q4_block_bytes(w.group)));
+    if (stages < 3 || kb * (s - 1) >= w.kblocks) continue;  // (every CTA has work)
+    const int clusters = (int)std::min<int64_t>(w.tiles, std::max(1, d->sms / s));
+    const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
+    if (found && cost >= least) continue;
+    least = cost, found = true;
+    best->splits = s, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
+  }
+  return found;
+}
+
+template <int NT, int GROUP>
+int launch_q4_t(Dev* d, const Q4Args& a, const Q4Plan& p) {
+  static bool attr_set[64] = {};
+  if (!attr_set[d->id]) {
+    ENVG_CUDA(cudaFuncSetAttribute(k_q4<NT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM));
+    attr_set[d->id] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.clusters * p.splits), (unsigned)cdiv(a.M, 4 * NT));
+  cfg.blockDim = dim3(Q4_THREADS);
+  cfg.dynamicSmemBytes = Q4Smem<NT>::total(p.kb_per, p.stages, GROUP);
+  cfg.stream = stream_of(d);
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (p.splits > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)p.splits, at[n].val.clusterDim.y = 1, at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (d->pdl && !g_prof_on) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)n;
+  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_q4<NT, GROUP>, a, p));
+  d->st.kernel_launches++;
+  return ENVG_OK;
+}
+
+template <int NT>
+int launch_q4_n(Dev* d, const Q4Args& a, const Q4Plan& p) {
+  switch (a.w.group) {
+    case 32: return launch_q4_t<NT, 32>(d, a, p);
+    case 64: return launch_q4_t<NT, 64>(d, a, p);
+    default: return launch_q4_t<NT, 128>(d, a, p);
+  }
+}
+
 int launch_q4(Dev* d, const Q4Args& a) {
   const double bytes = (double)a.w.tiles * a.w.kblocks * q4_block_bytes(a.w.group) + 4.0 * a.M * a.w.K + 4.0 * a.M * a.w.N;
   ProfScope ps(stream_of(d), KID_Q4, 2.0 * a.M * (double)a.w.N * (double)a.w.K, bytes);
-  ENVG_TRY(launch_pdl(d, k_q4_simple, dim3((unsigned)cdiv(a.w.tiles, 4), (unsigned)a.M), dim3(128), 0, a));
-  d->st.kernel_launches++;
-  return ENVG_OK;
+  Q4Plan p{};
+  p.vec = f4_ok(a.x, a.ldx);
+  p.wait_cap_ns = d->wait_cap_ns;
+  p.status = d->d_status;
+  // 16, 8 or 4 rows at a time: as many as there are, fewer where K leaves no room for their parts
+  if (a.M > 8 && q4_plan<4>(d, a.w, &p)) return launch_q4_n<4>(d, a, p);
+  if (a.M > 4 && q4_plan<2>(d, a.w, &p)) return launch_q4_n<2>(d, a, p);
+  if (q4_plan<1>(d, a.w, &p)) return launch_q4_n<1>(d, a, p);
+  return fail(ENVG_ERR_UNSUPPORTED, "linear_q4: K=%lld is too long", (long long)a.w.K);
 }
 
 int launch_norm_rope(Dev* d, const NormRopeArgs& a) {
@@ -313,6 +382,7 @@ int envg_weight_upload_q4(const uint8_t* codes, const float* scales, const uint8
   if (!codes || !scales) return fail(ENVG_ERR_ARG, "weight_upload_q4: codes or scales is NULL");
   if (N <= 0 || K <= 0 || N > INT32_MAX / 2 || K > INT32_MAX / 2)
     return fail(ENVG_ERR_ARG, "weight_upload_q4: N=%lld K=%lld", (long long)N, (long long)K);
+  if (K > Q4_MAX_K) return fail(ENVG_ERR_UNSUPPORTED, "weight_upload_q4: K=%lld (at most %d)", (long long)K, Q4_MAX_K);
   if (group != 32 && group != 64 && group != 128)
     return fail(ENVG_ERR_ARG, "weight_upload_q4: group %d (32, 64 or 128)", group);
   if (layout_flags != ENVG_LAYOUT_PLAIN && layout_flags != ENVG_LAYOUT_GATE_UP)

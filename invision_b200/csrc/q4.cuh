@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "mma16.cuh"
 #include "ptx.cuh"
 
 namespace envg {
@@ -105,35 +106,246 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
   }
 }
 
-// One warp per (tile, row m), one lane per (r, t): plain fp32 products in the layout's order.
-__global__ void __launch_bounds__(128) k_q4_simple(const Q4Args a) {
+// k_q4: y = x . W^T over the 4-bit blocks, 4 NT rows of x per launch row.
+//
+// Mathematics.  Of a block, group gi adds s[n][gi] sum_k (c[n][k] - z[n][gi]) x[m][k].  The products
+// run on the tensor cores as m16n8k16: c - z, exact as an fp16, is the 16-row operand (c or 16 c is
+// put into the mantissa of 1024, then one subtraction or multiply-add.  A bare c would be a
+// subnormal, which the cores align by its nominal exponent and so lose up to ten low bits of x);
+// x is the 8-column one, each row of it in two fp16 parts in adjacent columns, scaled by a power of
+// two per (row, block) so that its largest value is in [2^14, 2^15).  Each group's fp32 sum starts
+// from zero, gets both parts added and is then multiplied by its scale: nothing is rounded to 16
+// bits, and the cores' cutting off of low bits stays within one group.
+//
+// Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
+// of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
+// (tile, block) pairs are cut evenly among its warps, each of which streams its run of blocks
+// through a ring of bulk copies and leaves one sum per tile it touched in shared memory; the sums
+// are added in warp order and, in a cluster, handed to the tile's owner and added in rank order.
+// Weights do not depend on the previous kernel: the ring starts before waiting for it.
+constexpr int Q4_WARPS = 16, Q4_THREADS = 32 * Q4_WARPS, Q4_MAX_STAGES = 8;
+constexpr int Q4_SMEM = 227 * 1024;
+constexpr int SITE_Q4_RING = 61;  // status[1] of a ring wait that ran out
+
+struct Q4Plan {
+  int splits;         // CTAs of a cluster: K ranges
+  int clusters;       // runs of tiles
+  int kb_per;         // blocks of K per CTA
+  int stages;         // ring depth
+  int vec;            // rows of x are 16-byte aligned
+  uint64_t wait_cap_ns;
+  int* status;
+};
+template <int NT>
+struct Q4Smem {
+  static constexpr int R = 32 / NT;            // tiles at a time
+  static constexpr int SUMS = NT * 2 * 32 * 4;  // bytes of one tile's sums
+  static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
+  static constexpr int RECV = 2 * R * SUMS;  // [2][ranks][tiles of the owner], used by clusters
+  static constexpr int X_ROW = 4 * Q4_COLS;   // bytes of x's parts per (row, block)
+  static constexpr int FIXED = SLOTS + RECV + Q4_WARPS * Q4_MAX_STAGES * 8 + 16;
+  __host__ __device__ static int x_bytes(int kb) { return kb * 4 * NT * (X_ROW + 4); }
+  __host__ __device__ static int total(int kb, int stages, int group) {
+    return FIXED + x_bytes(kb) + Q4_WARPS * stages * q4_block_bytes(group);
+  }
+};
+
+ENVG_DEV void st_cluster_f2(uint32_t addr, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
+}
+
+template <int NT, int GROUP>
+__global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Plan p) {
+  using S = Q4Smem<NT>;
+  constexpr int R = S::R, BLOCK = q4_block_bytes(GROUP), PER = Q4_COLS / GROUP, MC = 4 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float* slots = reinterpret_cast<float*>(smem);
+  float* recv = reinterpret_cast<float*>(smem + S::SLOTS);
+  const uint32_t bars = smem_u32(smem + S::SLOTS + S::RECV) + warp * Q4_MAX_STAGES * 8;
+  volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::SLOTS + S::RECV + Q4_WARPS * Q4_MAX_STAGES * 8);
+  uint8_t* xf = smem + S::FIXED;                                         // [kb][word][row][part][t] 16 bytes
+  float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // [kb][row] 2^-e
+  uint8_t* ring = xf + S::x_bytes(p.kb_per) + warp * p.stages * BLOCK;
+
+  const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x / p.splits;
+  const int kb0 = rank * p.kb_per, kbn = max(0, min(p.kb_per, a.w.kblocks - kb0));
+  const int tile0 = (int)((int64_t)a.w.tiles * cl / p.clusters), tile1 = (int)((int64_t)a.w.tiles * (cl + 1) / p.clusters);
+  const int m0 = blockIdx.y * MC, mn = min(MC, a.M - m0);
+
+  if (lane == 0)
+    for (int i = 0; i < p.stages; ++i) mbar_init(bars + 8 * i, 1);
+  if (threadIdx.x == 0) *abort_s = 0;
+  fence_mbar_init();
+  __syncwarp();
+  // the warp's blocks: of each round (R tiles), an even share of its (tile, block) pairs
+  auto share = [&](int r0, int w) { return (int)((int64_t)min(R, tile1 - r0) * kbn * w / Q4_WARPS); };
+  int fr = tile0, fi = share(tile0, warp), fe = share(tile0, warp + 1);  // next block to fetch: round, index, end
+  auto fetch = [&](int st) {
+    while (fi >= fe && fr + R < tile1) fr += R, fi = share(fr, warp), fe = share(fr, warp + 1);
+    if (fi >= fe) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bars + 8 * st, BLOCK);
+      const int j = fi / kbn;
+      bulk_load(smem_u32(ring + st * BLOCK), a.w.base + ((int64_t)(fr + j) * a.w.kblocks + kb0 + fi - j * kbn) * BLOCK, BLOCK,
+                bars + 8 * st);
+    }
+    ++fi;
+  };
+  for (int i = 0; i < p.stages; ++i) fetch(i);
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const int64_t tile = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  const int m = blockIdx.y;
-  if (tile >= a.w.tiles) return;
-  const int bytes = q4_block_bytes(a.w.group), per = Q4_COLS / a.w.group;
-  float acc[2] = {};
-  for (int kb = 0; kb < a.w.kblocks; ++kb) {
-    const uint8_t* blk = a.w.base + (tile * a.w.kblocks + kb) * bytes;
-    for (int i = 0; i < 2; ++i)
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t v = reinterpret_cast<const uint32_t*>(blk)[i * 128 + lane * 4 + w];
-        const int gi = 32 * w / a.w.group;
-        const float s = reinterpret_cast<const float*>(blk + 1024)[gi * 16 + r + 8 * i];
-        const int z = blk[1024 + 64 * per + gi * 16 + r + 8 * i];
-        float part = 0.0f;
-        for (int j = 0; j < 8; ++j) {
-          const int64_t k = (int64_t)kb * Q4_COLS + 32 * w + 8 * t + j;
-          if (k < a.w.K) part = fmaf(a.x[(int64_t)m * a.ldx + k], (float)((int)((v >> (4 * j)) & 15u) - z), part);
-        }
-        acc[i] = fmaf(part, s, acc[i]);
+
+  // x of this K range as operand parts: a warp takes 128 columns of a row at a time
+  for (int i = warp; i < kbn * MC; i += Q4_WARPS) {
+    const int kb = i / MC, m = i % MC, k = (kb0 + kb) * Q4_COLS + 4 * lane;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m < mn) {
+      const float* src = a.x + (int64_t)(m0 + m) * a.ldx + k;
+      if (k + 3 < a.w.K) {
+        v = ld_f4(src, p.vec != 0);
+      } else {
+        if (k < a.w.K) v.x = src[0];
+        if (k + 1 < a.w.K) v.y = src[1];
+        if (k + 2 < a.w.K) v.z = src[2];
       }
+    }
+    float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int e = 0;
+    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
+    const float up = __int_as_float((127 + e) << 23);
+    v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+    const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+    const uint32_t l0 = h2_bits(__floats2half2_rn(v.x - b0.x, v.y - b0.y)), l1 = h2_bits(__floats2half2_rn(v.z - b1.x, v.w - b1.y));
+    // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
+    // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+    const bool odd = lane & 1;
+    const uint32_t s0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
+    const uint32_t a0 = odd ? s0 : h2_bits(h0), a1 = odd ? s1 : h2_bits(h1), c0 = odd ? l0 : s0, c1 = odd ? l1 : s1;
+    uint4 u;
+    u.x = __byte_perm(a0, c0, 0x5410), u.y = __byte_perm(a0, c0, 0x7632);
+    u.z = __byte_perm(a1, c1, 0x5410), u.w = __byte_perm(a1, c1, 0x7632);
+    const int word = lane >> 3, tt = (lane >> 1) & 3;
+    *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) = u;
+    if (lane == 0) xs[kb * MC + m] = __int_as_float((127 - e) << 23);
   }
-  for (int o = 1; o < 4; o <<= 1)
-    for (int i = 0; i < 2; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-  if (t == 0) q4_store(a, tile, r, m, acc[0], acc[1]);
+  if (p.splits > 1) cluster_sync();  // every CTA of the cluster is there to be written to
+  else __syncthreads();
+
+  const WaitCtl wc{p.wait_cap_ns, p.status, abort_s, 0};
+  const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
+  const __half2 c16 = __float2half2_rn(0.0625f);
+  bool fine = true;
+  int st = 0, buf = 0;
+  uint32_t phase = 0;
+  for (int r0 = tile0; r0 < tile1; r0 += R) {
+    const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
+    const int i1 = share(r0, warp + 1);
+    float acc[NT][2] = {};
+    for (int i = share(r0, warp); i < i1 && fine; ++i) {
+      const int j = i / kbn, kb = i - j * kbn;
+      fine = wait_bounded(bars + 8 * st, phase, wc, SITE_Q4_RING);
+      if (!__all_sync(0xffffffffu, fine)) {
+        fine = false;
+        break;
+      }
+      const uint8_t* blk = ring + st * BLOCK;
+      const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
+      const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
+      float xsc[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) xsc[nt] = xs[kb * MC + 4 * nt + t];
+      const uint8_t* xk = xf + (size_t)kb * MC * S::X_ROW + g * 64 + t * 16;
+#pragma unroll
+      for (int gi = 0; gi < PER; ++gi) {
+        const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
+        const uint32_t z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
+        // 1024 + z, and -(64 + z) for 16 times the code
+        const __half2 zl0 = bits_h2(z0 * 0x00010001u + magic), zh0 = bits_h2(z0 * 0x00100010u + 0xD400D400u);
+        const __half2 zl1 = bits_h2(z1 * 0x00010001u + magic), zh1 = bits_h2(z1 * 0x00100010u + 0xD400D400u);
+        float d[NT][4];
+#pragma unroll
+        for (int wi = 0; wi < 4 / PER; ++wi) {
+          const int w = gi * (4 / PER) + wi;
+          uint4 xw[NT];  // the word's eight columns of x, for both of its products
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + (w * MC + 4 * nt) * 128);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t u0 = h ? w0[w] >> 8 : w0[w], u1 = h ? w1[w] >> 8 : w1[w];
+            const uint32_t A0 = h2_bits(__hsub2(bits_h2(and_or(u0, mask0, magic)), zl0));
+            const uint32_t A1 = h2_bits(__hsub2(bits_h2(and_or(u1, mask0, magic)), zl1));
+            const uint32_t A2 = h2_bits(__hfma2(bits_h2(and_or(u0, mask1, magic)), c16, zh0));
+            const uint32_t A3 = h2_bits(__hfma2(bits_h2(and_or(u1, mask1, magic)), c16, zh1));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t bb[2] = {h ? xw[nt].z : xw[nt].x, h ? xw[nt].w : xw[nt].y};
+              if (wi == 0 && h == 0) mma_f16_zero(d[nt], A0, A1, A2, A3, bb);
+              else mma_f16(d[nt], A0, A1, A2, A3, bb);
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          acc[nt][0] = fmaf(d[nt][0] + d[nt][1], s0 * xsc[nt], acc[nt][0]);
+          acc[nt][1] = fmaf(d[nt][2] + d[nt][3], s1 * xsc[nt], acc[nt][1]);
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      fetch(st);
+      if (++st == p.stages) st = 0, phase ^= 1;
+      if (kb == kbn - 1 || i == i1 - 1) {  // the warp leaves the tile
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 64 + 2 * lane) = make_float2(acc[nt][0], acc[nt][1]);
+          acc[nt][0] = acc[nt][1] = 0.0f;
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tiles * NT * 32; i += Q4_THREADS) {
+      const int j = i / (NT * 32), nt = (i / 32) % NT, ln = i & 31;
+      float2 v = make_float2(0.0f, 0.0f);
+      if (kbn > 0) {
+        // warp of block b: the last w whose share starts at or before b
+        const int wa = (int)(((int64_t)j * kbn + 1) * Q4_WARPS - 1) / nb, wb = (int)(((int64_t)(j + 1) * kbn) * Q4_WARPS - 1) / nb;
+        for (int w = wa; w <= wb; ++w) {
+          if (nb * w / Q4_WARPS == nb * (w + 1) / Q4_WARPS) continue;  // a warp without a block
+          const float2 s = *reinterpret_cast<const float2*>(slots + ((j + w) * NT + nt) * 64 + 2 * ln);
+          v.x += s.x, v.y += s.y;
+        }
+      }
+      if (p.splits == 1) {
+        const int m = 4 * nt + (ln & 3);
+        if (m < mn) q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
+      } else {
+        const int owner = j % p.splits, at = buf * R + rank * ((R + p.splits - 1) / p.splits) + j / p.splits;
+        st_cluster_f2(mapa_shared(smem_u32(recv + (at * NT + nt) * 64 + 2 * ln), owner), v.x, v.y);
+      }
+    }
+    if (p.splits == 1) {
+      __syncthreads();
+      continue;
+    }
+    cluster_sync();
+    const int each = (R + p.splits - 1) / p.splits;
+    for (int i = threadIdx.x; i < each * NT * 32; i += Q4_THREADS) {
+      const int jj = i / (NT * 32), j = jj * p.splits + rank, nt = (i / 32) % NT, ln = i & 31, m = 4 * nt + (ln & 3);
+      if (j >= tiles || m >= mn) continue;
+      float2 v = make_float2(0.0f, 0.0f);
+      for (int q = 0; q < p.splits; ++q) {
+        const float2 s = *reinterpret_cast<const float2*>(recv + ((buf * R + q * each + jj) * NT + nt) * 64 + 2 * ln);
+        v.x += s.x, v.y += s.y;
+      }
+      q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
+    }
+    buf ^= 1;  // a buffer is written again after the next barrier, when its owner has read it
+  }
+  if (!fine && lane == 0)  // given up: no copy may be in flight when the CTA leaves
+    for (int i = 0; i < p.stages; ++i) wait_drain(bars + 8 * i, 0, p.wait_cap_ns), wait_drain(bars + 8 * i, 1, p.wait_cap_ns);
 }
 
 }  // namespace envg

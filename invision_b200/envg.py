@@ -578,54 +578,62 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
 # projection's output is passed as it is.
 # ---------------------------------------------------------------------------------------------
 
+_torch = None  # the torch module, once a tensor has been passed
+_TORCH_DTYPES = {}
+
+
 def _device_of(arrays):
     """DEVICE_PTRS (and the library put on torch's current stream) for CUDA tensors, HOST_PTRS for
     numpy arrays; never mixed."""
+    global _torch
     torch_side = None
+    device = 0
     for a in arrays:
         if a is None:
             continue
-        t = not isinstance(a, np.ndarray)
-        if torch_side is None:
-            torch_side = t
-        elif torch_side != t:
+        if isinstance(a, np.ndarray):
+            if torch_side:
+                raise TypeError("operands must be all numpy (host) or all torch CUDA tensors (device)")
+            torch_side = False
+            continue
+        if torch_side is False:
             raise TypeError("operands must be all numpy (host) or all torch CUDA tensors (device)")
+        torch_side = True
+        if _torch is None:
+            import torch
+
+            _torch = torch
+            _TORCH_DTYPES.update(float32=torch.float32, int32=torch.int32, uint8=torch.uint8)
+        if not (isinstance(a, _torch.Tensor) and a.is_cuda):
+            raise TypeError("device operands must be CUDA tensors")
     if not torch_side:
         return HOST_PTRS
-    import torch
-
-    for a in arrays:
-        if a is not None and not (isinstance(a, torch.Tensor) and a.is_cuda):
-            raise TypeError("device operands must be CUDA tensors")
     if _follow_torch_stream:
-        h = torch.cuda.current_stream().cuda_stream
+        h = _torch.cuda.current_stream().cuda_stream
         lib().envg_set_stream(h if h else CUDA_STREAM_LEGACY)
     return DEVICE_PTRS
 
 
-_DTYPE_NAMES = {"float32": ("float32", "torch.float32"), "int32": ("int32", "torch.int32"),
-                "uint8": ("uint8", "torch.uint8")}
-
-
-def _typed(a, dtype, name):
-    if str(a.dtype) not in _DTYPE_NAMES[dtype]:
-        raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
+_NP_DTYPES = {"float32": np.dtype(np.float32), "int32": np.dtype(np.int32), "uint8": np.dtype(np.uint8)}
 
 
 def _matrix(a, rows, cols, name, dtype="float32"):
     """(pointer, row stride in elements) of a 2-D array [rows, >= cols] whose columns are adjacent."""
     if a is None:
         return None, 0
-    _typed(a, dtype, name)
-    if a.ndim != 2 or a.shape[0] != rows or a.shape[1] < cols:
-        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(a.shape)}")
-    if isinstance(a, np.ndarray):
+    host = isinstance(a, np.ndarray)
+    if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
+        raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
+    shape = a.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] < cols:
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(shape)}")
+    if host:
         st, ptr = [s // a.itemsize for s in a.strides], a.ctypes.data
     else:
         st, ptr = a.stride(), a.data_ptr()
-    if a.shape[1] > 1 and st[1] != 1:
+    if shape[1] > 1 and st[1] != 1:
         raise TypeError(f"{name}: columns must be adjacent")
-    ld = st[0] if rows > 1 else max(a.shape[1], 1)
+    ld = st[0] if rows > 1 else max(shape[1], 1)
     if ld < cols:
         raise TypeError(f"{name}: rows overlap")
     return ptr, ld
@@ -634,16 +642,14 @@ def _matrix(a, rows, cols, name, dtype="float32"):
 def _vector(a, n, name, dtype="float32"):
     if a is None:
         return None
-    _typed(a, dtype, name)
-    if a.ndim != 1 or a.shape[0] != n:
+    host = isinstance(a, np.ndarray)
+    if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
+        raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
+    if len(a.shape) != 1 or a.shape[0] != n:
         raise ValueError(f"{name}: expected [{n}], got {list(a.shape)}")
-    if isinstance(a, np.ndarray):
-        if n > 1 and a.strides[0] != a.itemsize:
-            raise TypeError(f"{name}: must be contiguous")
-        return a.ctypes.data
-    if n > 1 and a.stride(0) != 1:
+    if n > 1 and (a.strides[0] != a.itemsize if host else a.stride(0) != 1):
         raise TypeError(f"{name}: must be contiguous")
-    return a.data_ptr()
+    return a.ctypes.data if host else a.data_ptr()
 
 
 def _flags(mode, sync):
