@@ -364,9 +364,20 @@ int envg_q4weight_free(envg_q4weight w);
  * codes are exact in the tensor cores' 16-bit operands, x is carried as two of them, scales are
  * applied to the fp32 sums of their groups (about 1e-7 relative).  Made for few rows (M up to
  * about 64); 0 <= M <= 65535.  A row of x that holds an infinity or a NaN gives non-finite
- * outputs in that row.  dst must not overlap x. */
-int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4weight W, const float* bias,
-                   int64_t M, int64_t K, int64_t N, int epilogue, const float* gate, int flags);
+ * outputs in that row.  dst must not overlap x.  The matrices of this and the following calls are
+ * many, so each call takes them in a structure. */
+typedef struct envg_linear_q4_args {
+  float* dst;
+  int64_t ldd;
+  const float* x;
+  int64_t ldx;
+  envg_q4weight W;
+  const float* bias;  /* fp32 [N] or NULL                               */
+  const float* gate;  /* fp32 [N] for ENVG_EPI_GATED_RESIDUAL, else NULL */
+  int64_t M, K, N;
+  int epilogue;
+} envg_linear_q4_args;
+int envg_linear_q4(const envg_linear_q4_args* args, int flags);
 
 /* For every token t and head h of q (heads) and k (kv_heads):
  *   y = rot(x * weight / sqrt(mean(x^2) + eps), position of t)
@@ -377,11 +388,24 @@ int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4
  * q_weight / k_weight: [head_dim] or NULL.  Head h starts at column h * head_dim of its row.  One of
  * heads and kv_heads may be 0 (its operands are then not read).  q_dst may be q and k_dst may be k
  * (with the same stride).  head_dim: a multiple of 8 up to 256. */
-int envg_qk_norm_rope(float* q_dst, int64_t ldqd, float* k_dst, int64_t ldkd, const float* q, int64_t ldq,
-                      const float* k, int64_t ldk, const float* q_weight, const float* k_weight,
-                      const float* cos_table, const float* sin_table, int64_t table_rows,
-                      const int32_t* positions, int64_t pos0, int64_t tokens, int heads, int kv_heads,
-                      int head_dim, float eps, int interleaved, int flags);
+typedef struct envg_qk_norm_rope_args {
+  float* q_dst;
+  int64_t ldqd;
+  float* k_dst;
+  int64_t ldkd;
+  const float* q;
+  int64_t ldq;
+  const float* k;
+  int64_t ldk;
+  const float *q_weight, *k_weight, *cos_table, *sin_table;
+  int64_t table_rows;
+  const int32_t* positions;
+  int64_t pos0, tokens;
+  int heads, kv_heads, head_dim;
+  float eps;
+  int interleaved;
+} envg_qk_norm_rope_args;
+int envg_qk_norm_rope(const envg_qk_norm_rope_args* args, int flags);
 
 /* A key/value cache in 4 bits: `pages` pages of `page_size` (a multiple of 16 up to 1024) tokens,
  * kv_heads heads of head_dim (64 or 128) channels.  For each token, head and group of 64 channels
@@ -397,13 +421,21 @@ int envg_kv4_free(envg_kv4 c);
  * sequence b (rows that would come before its first token are left out): ctx_lens counts the new
  * tokens.  Token p stands in page table[b * table_stride + p / page_size] at p % page_size.  Pages
  * may be shared between sequences as long as one call does not write a token twice. */
-int envg_kv4_append(envg_kv4 cache, const float* k, int64_t ldk, const float* v, int64_t ldv,
-                    const int32_t* table, int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len,
-                    int flags);
+typedef struct envg_kv4_rows {
+  envg_kv4 cache;
+  float* k;  /* read by envg_kv4_append, written by envg_kv4_read; v alike */
+  int64_t ldk;
+  float* v;
+  int64_t ldv;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* ctx_lens;
+  int batch, q_len;
+} envg_kv4_rows;
+int envg_kv4_append(const envg_kv4_rows* rows, int flags);
 
 /* The values the cache holds for the same tokens (zeros for rows before a sequence's first token). */
-int envg_kv4_read(envg_kv4 cache, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table,
-                  int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int flags);
+int envg_kv4_read(const envg_kv4_rows* rows, int flags);
 
 /* Attention of the newest q_len tokens of each sequence over the cache (which holds them too):
  * row b * q_len + i of q and dst ([batch * q_len, heads * head_dim]) stands at position
@@ -412,9 +444,19 @@ int envg_kv4_read(envg_kv4 cache, float* k, int64_t ldk, float* v, int64_t ldv, 
  * h / (heads / kv_heads).  dst = softmax(scale * q . k) . v in fp32 (about 1e-6 relative); a row
  * that sees nothing is zeros.  max_ctx is the largest of ctx_lens where the caller knows it, or 0:
  * it only plans how the work is split.  dst must not overlap q. */
-int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, envg_kv4 cache,
-                       const int32_t* table, int64_t table_stride, const int32_t* ctx_lens, int batch,
-                       int q_len, int max_ctx, int heads, int window, int sinks, float scale, int flags);
+typedef struct envg_attention_kv4_args {
+  float* dst;
+  int64_t ldo;
+  const float* q;
+  int64_t ldq;
+  envg_kv4 cache;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* ctx_lens;
+  int batch, q_len, max_ctx, heads, window, sinks;
+  float scale;
+} envg_attention_kv4_args;
+int envg_attention_kv4(const envg_attention_kv4_args* args, int flags);
 
 /* cblas_sgemm-compatible fp32 GEMM on host pointers: the signature of the function-pointer
  * slot TQNNSingleOPS.cblas_sgemm (quicknncpu.pas:102-109; enums quicknn_common.pas:54-58:

@@ -93,6 +93,29 @@ int finish_call(Dev* d, int flags) {
 // How a 4-bit linear is spread over the SMs (one CTA each): the cluster size, a power of two, that
 // leaves the least work on the busiest CTA, counted in blocks plus a fixed cost per cluster
 // exchange, among those whose part of x leaves room for a ring.
+// Clusters of s CTAs that the GPU holds at once (they do not span its processor groups).
+int q4_clusters(const Dev* d, int s) {
+  static int held[64][4];
+  int& n = held[d->id][s == 2 ? 1 : s == 4 ? 2 : s == 8 ? 3 : 0];
+  if (s == 1) return d->sms;
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(d->sms / s * s));
+  cfg.blockDim = dim3(Q4_THREADS);
+  cfg.dynamicSmemBytes = Q4_SMEM;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)s, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(k_q4<1, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, k_q4<1, 128>, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, d->sms / (2 * s));
+  }
+  if (getenv("X_V")) fprintf(stderr, "clusters of %d: %d\n", s, n);
+  return n;
+}
+
 template <int NT>
 bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
   using S = Q4Smem<NT>;
@@ -103,9 +126,10 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
     const int room = Q4_SMEM - S::FIXED - S::x_bytes(kb);
     const int stages = std::min(Q4_MAX_STAGES, room / (Q4_WARPS * q4_block_bytes(w.group)));
     if (stages < 3 || kb * (s - 1) >= w.kblocks) continue;  // (every CTA has work)
-    const int clusters = (int)std::min<int64_t>(w.tiles, std::max(1, d->sms / s));
+    const int clusters = (int)std::min<int64_t>(w.tiles, q4_clusters(d, s));
     const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
     if (found && cost >= least) continue;
+    if (getenv("X_S") && atoi(getenv("X_S")) != s) continue;
     least = cost, found = true;
     best->splits = s, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
   }
@@ -230,11 +254,16 @@ Kv4View kv_view(Dev* d, envg_kv4 c, const int32_t* table, int64_t stride, const 
 }
 
 // Append (k, v are read) or read back (k, v are written) the last q_len tokens of each sequence.
-int kv4_rows(envg_kv4 c, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table, int64_t stride,
-             const int32_t* lens, int batch, int q_len, int flags, bool read) {
+int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   const char* what = read ? "kv4_read" : "kv4_append";
   Dev* d;
   ENVG_TRY(lm_dev(&d));
+  if (!r) return fail(ENVG_ERR_ARG, "%s: NULL arguments", what);
+  const envg_kv4 c = r->cache;
+  float *k = r->k, *v = r->v;
+  const int64_t ldk = r->ldk, ldv = r->ldv, stride = r->table_stride;
+  const int32_t *table = r->table, *lens = r->ctx_lens;
+  const int batch = r->batch, q_len = r->q_len;
   ENVG_TRY(check_kv_call(d, c, table, stride, lens, batch, q_len, 0, 0, flags, what));
   const int64_t rows = (int64_t)batch * q_len, width = (int64_t)c->kv_heads * c->head_dim;
   if (rows == 0) return ENVG_OK;
@@ -451,11 +480,16 @@ int envg_q4weight_free(envg_q4weight w) {
   return ENVG_OK;
 }
 
-int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4weight W, const float* bias, int64_t M,
-                   int64_t K, int64_t N, int epilogue, const float* gate, int flags) {
+int envg_linear_q4(const envg_linear_q4_args* q, int flags) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   Dev* d;
   ENVG_TRY(lm_dev(&d));
+  if (!q) return fail(ENVG_ERR_ARG, "linear_q4: NULL arguments");
+  float* dst = q->dst;
+  const float *x = q->x, *bias = q->bias, *gate = q->gate;
+  const envg_q4weight W = q->W;
+  const int64_t ldd = q->ldd, ldx = q->ldx, M = q->M, K = q->K, N = q->N;
+  const int epilogue = q->epilogue;
   ENVG_TRY(check_q4(d, W));
   if (K != W->v.K || N != W->v.N)
     return fail(ENVG_ERR_ARG, "linear_q4: [K=%lld, N=%lld] does not match the weight [N=%lld, K=%lld]", (long long)K,
@@ -502,13 +536,19 @@ int envg_linear_q4(float* dst, int64_t ldd, const float* x, int64_t ldx, envg_q4
   return finish_call(d, flags);
 }
 
-int envg_qk_norm_rope(float* q_dst, int64_t ldqd, float* k_dst, int64_t ldkd, const float* q, int64_t ldq,
-                      const float* k, int64_t ldk, const float* q_weight, const float* k_weight, const float* cos_table,
-                      const float* sin_table, int64_t table_rows, const int32_t* positions, int64_t pos0, int64_t tokens,
-                      int heads, int kv_heads, int head_dim, float eps, int interleaved, int flags) {
+int envg_qk_norm_rope(const envg_qk_norm_rope_args* r, int flags) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   Dev* d;
   ENVG_TRY(lm_dev(&d));
+  if (!r) return fail(ENVG_ERR_ARG, "qk_norm_rope: NULL arguments");
+  float *q_dst = r->q_dst, *k_dst = r->k_dst;
+  const float *q = r->q, *k = r->k, *q_weight = r->q_weight, *k_weight = r->k_weight;
+  const float *cos_table = r->cos_table, *sin_table = r->sin_table;
+  const int64_t ldqd = r->ldqd, ldkd = r->ldkd, ldq = r->ldq, ldk = r->ldk;
+  const int64_t table_rows = r->table_rows, pos0 = r->pos0, tokens = r->tokens;
+  const int32_t* positions = r->positions;
+  const int heads = r->heads, kv_heads = r->kv_heads, head_dim = r->head_dim, interleaved = r->interleaved;
+  const float eps = r->eps;
   if (head_dim < 8 || head_dim > 256 || head_dim % 8)
     return fail(ENVG_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d (a multiple of 8 up to 256)", head_dim);
   if (tokens < 0 || heads < 0 || kv_heads < 0 || heads > 65535 || kv_heads > 65535)
@@ -616,25 +656,28 @@ int envg_kv4_free(envg_kv4 c) {
   return ENVG_OK;
 }
 
-int envg_kv4_append(envg_kv4 cache, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* table,
-                    int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int flags) {
+int envg_kv4_append(const envg_kv4_rows* rows, int flags) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  return kv4_rows(cache, const_cast<float*>(k), ldk, const_cast<float*>(v), ldv, table, table_stride, ctx_lens, batch, q_len,
-                  flags, false);
+  return kv4_rows(rows, flags, false);
 }
 
-int envg_kv4_read(envg_kv4 cache, float* k, int64_t ldk, float* v, int64_t ldv, const int32_t* table, int64_t table_stride,
-                  const int32_t* ctx_lens, int batch, int q_len, int flags) {
+int envg_kv4_read(const envg_kv4_rows* rows, int flags) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  return kv4_rows(cache, k, ldk, v, ldv, table, table_stride, ctx_lens, batch, q_len, flags, true);
+  return kv4_rows(rows, flags, true);
 }
 
-int envg_attention_kv4(float* dst, int64_t ldo, const float* q, int64_t ldq, envg_kv4 cache, const int32_t* table,
-                       int64_t table_stride, const int32_t* ctx_lens, int batch, int q_len, int max_ctx, int heads,
-                       int window, int sinks, float scale, int flags) {
+int envg_attention_kv4(const envg_attention_kv4_args* r, int flags) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   Dev* d;
   ENVG_TRY(lm_dev(&d));
+  if (!r) return fail(ENVG_ERR_ARG, "attention_kv4: NULL arguments");
+  float* dst = r->dst;
+  const float* q = r->q;
+  const envg_kv4 cache = r->cache;
+  const int32_t *table = r->table, *ctx_lens = r->ctx_lens;
+  const int64_t ldo = r->ldo, ldq = r->ldq, table_stride = r->table_stride;
+  const int batch = r->batch, q_len = r->q_len, max_ctx = r->max_ctx, heads = r->heads, window = r->window, sinks = r->sinks;
+  const float scale = r->scale;
   if (window < 0 || sinks < 0) return fail(ENVG_ERR_ARG, "attention_kv4: window %d, sinks %d", window, sinks);
   ENVG_TRY(check_kv_call(d, cache, table, table_stride, ctx_lens, batch, q_len, window > 0 ? window - 1 : INT32_MAX,
                          window > 0 ? sinks : 0, flags, "attention_kv4"));

@@ -138,10 +138,10 @@ struct Q4Plan {
 };
 template <int NT>
 struct Q4Smem {
-  static constexpr int R = 32 / NT;            // tiles at a time
+  static constexpr int R = NT == 4 ? 16 : 32;   // tiles at a time
   static constexpr int SUMS = NT * 2 * 32 * 4;  // bytes of one tile's sums
   static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
-  static constexpr int RECV = 2 * R * SUMS;  // [2][ranks][tiles of the owner], used by clusters
+  static constexpr int RECV = R * SUMS;       // [ranks][tiles of the owner], used by clusters
   static constexpr int X_ROW = 4 * Q4_COLS;   // bytes of x's parts per (row, block)
   static constexpr int FIXED = SLOTS + RECV + Q4_WARPS * Q4_MAX_STAGES * 8 + 16;
   __host__ __device__ static int x_bytes(int kb) { return kb * 4 * NT * (X_ROW + 4); }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
   const __half2 c16 = __float2half2_rn(0.0625f);
   bool fine = true;
-  int st = 0, buf = 0;
+  int st = 0;
   uint32_t phase = 0;
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         const int m = 4 * nt + (ln & 3);
         if (m < mn) q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
       } else {
-        const int owner = j % p.splits, at = buf * R + rank * ((R + p.splits - 1) / p.splits) + j / p.splits;
+        const int owner = j % p.splits, at = rank * (R / p.splits) + j / p.splits;
         st_cluster_f2(mapa_shared(smem_u32(recv + (at * NT + nt) * 64 + 2 * ln), owner), v.x, v.y);
       }
     }
@@ -331,18 +331,18 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       continue;
     }
     cluster_sync();
-    const int each = (R + p.splits - 1) / p.splits;
+    const int each = R / p.splits;
     for (int i = threadIdx.x; i < each * NT * 32; i += Q4_THREADS) {
       const int jj = i / (NT * 32), j = jj * p.splits + rank, nt = (i / 32) % NT, ln = i & 31, m = 4 * nt + (ln & 3);
       if (j >= tiles || m >= mn) continue;
       float2 v = make_float2(0.0f, 0.0f);
       for (int q = 0; q < p.splits; ++q) {
-        const float2 s = *reinterpret_cast<const float2*>(recv + ((buf * R + q * each + jj) * NT + nt) * 64 + 2 * ln);
+        const float2 s = *reinterpret_cast<const float2*>(recv + ((q * each + jj) * NT + nt) * 64 + 2 * ln);
         v.x += s.x, v.y += s.y;
       }
       q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
     }
-    buf ^= 1;  // a buffer is written again after the next barrier, when its owner has read it
+    if (r0 + R < tile1) cluster_sync();  // the next round's sums may come when all have read these
   }
   if (!fine && lane == 0)  // given up: no copy may be in flight when the CTA leaves
     for (int i = 0; i < p.stages; ++i) wait_drain(bars + 8 * i, 0, p.wait_cap_ns), wait_drain(bars + 8 * i, 1, p.wait_cap_ns);

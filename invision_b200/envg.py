@@ -15,6 +15,7 @@ argument order and meaning (``src/quicknn_kernels.pas``) and raise ``AssertionEr
 import ctypes
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -115,15 +116,10 @@ def lib():
         L.envg_quantize_q4.argtypes = [_vp, _vp, _i64, _i64, _ci, _vp, _vp, _vp]
         L.envg_weight_upload_q4.argtypes = [_vp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, ctypes.POINTER(_vp)]
         L.envg_q4weight_free.argtypes = [_vp]
-        L.envg_linear_q4.argtypes = [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _vp, _ci]
-        L.envg_qk_norm_rope.argtypes = [_vp, _i64] * 4 + [_vp] * 4 + [_i64, _vp, _i64, _i64, _ci, _ci, _ci,
-                                                                      ctypes.c_float, _ci, _ci]
+        for f in (L.envg_linear_q4, L.envg_qk_norm_rope, L.envg_kv4_append, L.envg_kv4_read, L.envg_attention_kv4):
+            f.argtypes = [ctypes.c_char_p, _ci]  # a structure, packed
         L.envg_kv4_create.argtypes = [_i64, _ci, _ci, _ci, ctypes.POINTER(_vp)]
         L.envg_kv4_free.argtypes = [_vp]
-        L.envg_kv4_append.argtypes = [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _ci, _ci, _ci]
-        L.envg_kv4_read.argtypes = [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _ci, _ci, _ci]
-        L.envg_attention_kv4.argtypes = [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _ci, _ci, _ci, _ci, _ci, _ci,
-                                         ctypes.c_float, _ci]
         L.envg_set_stream.argtypes = [_vp]
         L.envg_get_stats.argtypes = [ctypes.POINTER(Stats)]
         L.envg_set_wait_cap_ns.argtypes = [ctypes.c_uint64]
@@ -580,48 +576,54 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
 
 _torch = None  # the torch module, once a tensor has been passed
 _TORCH_DTYPES = {}
+_NP_DTYPES = {"float32": np.dtype(np.float32), "int32": np.dtype(np.int32), "uint8": np.dtype(np.uint8)}
+# the argument structures of the C ABI (native alignment)
+_LINEAR_Q4 = struct.Struct("PqPqPPPqqqi")
+_QK_NORM_ROPE = struct.Struct("PqPqPqPqPPPPqPqqiiifi")
+_KV4_ROWS = struct.Struct("PPqPqPqPii")
+_ATTENTION_KV4 = struct.Struct("PqPqPPqPiiiiiif")
 
 
-def _device_of(arrays):
-    """DEVICE_PTRS (and the library put on torch's current stream) for CUDA tensors, HOST_PTRS for
-    numpy arrays; never mixed."""
+def _side(a):
+    """HOST_PTRS for a call whose operand ``a`` is a numpy array; DEVICE_PTRS, with the library put on
+    torch's current stream, for a CUDA tensor."""
     global _torch
-    torch_side = None
-    device = 0
-    for a in arrays:
-        if a is None:
-            continue
-        if isinstance(a, np.ndarray):
-            if torch_side:
-                raise TypeError("operands must be all numpy (host) or all torch CUDA tensors (device)")
-            torch_side = False
-            continue
-        if torch_side is False:
-            raise TypeError("operands must be all numpy (host) or all torch CUDA tensors (device)")
-        torch_side = True
-        if _torch is None:
-            import torch
-
-            _torch = torch
-            _TORCH_DTYPES.update(float32=torch.float32, int32=torch.int32, uint8=torch.uint8)
-        if not (isinstance(a, _torch.Tensor) and a.is_cuda):
-            raise TypeError("device operands must be CUDA tensors")
-    if not torch_side:
+    if isinstance(a, np.ndarray):
         return HOST_PTRS
+    if _torch is None:
+        import torch
+
+        _TORCH_DTYPES.update(float32=torch.float32, int32=torch.int32, uint8=torch.uint8)
+        _torch = torch
+    if not (isinstance(a, _torch.Tensor) and a.is_cuda):
+        raise TypeError("operands must be numpy arrays (host) or CUDA tensors (device)")
     if _follow_torch_stream:
-        h = _torch.cuda.current_stream().cuda_stream
-        lib().envg_set_stream(h if h else CUDA_STREAM_LEGACY)
+        lib().envg_set_stream(_raw_stream(a.get_device()) or CUDA_STREAM_LEGACY)
     return DEVICE_PTRS
 
 
-_NP_DTYPES = {"float32": np.dtype(np.float32), "int32": np.dtype(np.int32), "uint8": np.dtype(np.uint8)}
+def _raw_stream(device):
+    """Handle of torch's current stream (the short way where this torch has it: a call per operator)."""
+    get = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device) if get else _torch.cuda.current_stream(device).cuda_stream
 
 
-def _matrix(a, rows, cols, name, dtype="float32"):
+def _on_side(a, mode, name):
+    host = isinstance(a, np.ndarray)
+    if host != (mode == HOST_PTRS) or not (host or a.is_cuda):
+        raise TypeError(f"{name}: operands must be all numpy (host) or all torch CUDA tensors (device)")
+    return host
+
+
+def _matrix(a, rows, cols, name, mode, dtype="float32"):
     """(pointer, row stride in elements) of a 2-D array [rows, >= cols] whose columns are adjacent."""
     if a is None:
-        return None, 0
-    host = isinstance(a, np.ndarray)
+        return 0, 0
+    if mode == DEVICE_PTRS and type(a) is _torch.Tensor and a.dim() == 2:  # the usual case, checked at once
+        (r, c), (s0, s1) = a.shape, a.stride()
+        if a.is_cuda and a.dtype is _TORCH_DTYPES[dtype] and r == rows and c >= cols and s1 == 1 and s0 >= c:
+            return a.data_ptr(), s0
+    host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
         raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
     shape = a.shape
@@ -639,17 +641,25 @@ def _matrix(a, rows, cols, name, dtype="float32"):
     return ptr, ld
 
 
-def _vector(a, n, name, dtype="float32"):
+def _vector(a, n, name, mode, dtype="float32"):
     if a is None:
-        return None
-    host = isinstance(a, np.ndarray)
+        return 0
+    host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
         raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
-    if len(a.shape) != 1 or a.shape[0] != n:
+    if a.ndim != 1 or a.shape[0] != n:
         raise ValueError(f"{name}: expected [{n}], got {list(a.shape)}")
     if n > 1 and (a.strides[0] != a.itemsize if host else a.stride(0) != 1):
         raise TypeError(f"{name}: must be contiguous")
     return a.ctypes.data if host else a.data_ptr()
+
+
+def _packed(a, rows, cols, name, mode, dtype="float32"):
+    """Pointer of a contiguous array [rows, cols]."""
+    p, ld = _matrix(a, rows, cols, name, mode, dtype)
+    if a is not None and (a.shape[1] != cols or (rows > 1 and ld != cols)):
+        raise ValueError(f"{name}: expected a contiguous [{rows}, {cols}], got {list(a.shape)}")
+    return p
 
 
 def _flags(mode, sync):
@@ -680,7 +690,7 @@ class Q4Weight:
 
     def __init__(self, codes, scales, zeros=None, K=None, group=128, layout=LAYOUT_PLAIN):
         self.h = None
-        mode = _device_of((codes, scales, zeros))
+        mode = _side(codes)
         self.N = codes.shape[0]
         self.K = 2 * codes.shape[1] if K is None else int(K)
         if codes.ndim != 2 or codes.shape[1] != (self.K + 1) // 2:
@@ -688,15 +698,10 @@ class Q4Weight:
         if group not in (32, 64, 128):
             raise ValueError(f"group {group}: 32, 64 or 128")
         groups = -(-self.K // group)
-        ptrs = []
-        for a, n, dt, what in ((codes, codes.shape[1], "uint8", "codes"), (scales, groups, "float32", "scales"),
-                               (zeros, groups, "uint8", "zeros")):
-            p, ld = _matrix(a, self.N, n, what, dt)
-            if a is not None and (a.shape[1] != n or ld != n):
-                raise ValueError(f"{what}: expected a contiguous [{self.N}, {n}], got {list(a.shape)}")
-            ptrs.append(p)
+        ptrs = [_packed(codes, self.N, codes.shape[1], "codes", mode, "uint8"),
+                _packed(scales, self.N, groups, "scales", mode), _packed(zeros, self.N, groups, "zeros", mode, "uint8")]
         h = _vp()
-        _check(lib().envg_weight_upload_q4(*ptrs, self.N, self.K, group, layout, mode, ctypes.byref(h)))
+        _check(lib().envg_weight_upload_q4(*[p or None for p in ptrs], self.N, self.K, group, layout, mode, ctypes.byref(h)))
         self.group, self.layout, self.h = group, layout, h
 
     def free(self):
@@ -715,14 +720,15 @@ def linear_q4(dst, x, W, bias=None, epilogue=None, gate=None, sync=True):
     """dst = epilogue(x . W^T) for a Q4Weight: envg_linear_q4.  x [M, K]; dst [M, N] (N/2 for SILU_GATE)."""
     if epilogue is None:
         epilogue = EPI_SILU_GATE if W.layout == LAYOUT_GATE_UP else (EPI_BIAS if bias is not None else EPI_NONE)
-    mode = _device_of((dst, x, bias, gate))
+    mode = _side(x)
     M, N = x.shape[0], W.N
-    px, ldx = _matrix(x, M, W.K, "x")
+    px, ldx = _matrix(x, M, W.K, "x", mode)
     if x.shape[1] != W.K:
         raise ValueError(f"x: expected {W.K} columns, got {x.shape[1]}")
-    py, ldd = _matrix(dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, "dst")
-    return _check(lib().envg_linear_q4(py, ldd, px, ldx, W.h, _vector(bias, N, "bias"), M, W.K, N, epilogue,
-                                       _vector(gate, N, "gate"), _flags(mode, sync)))
+    py, ldd = _matrix(dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, "dst", mode)
+    return _check(lib().envg_linear_q4(
+        _LINEAR_Q4.pack(py, ldd, px, ldx, _handle(W), _vector(bias, N, "bias", mode), _vector(gate, N, "gate", mode), M,
+                        W.K, N, epilogue), _flags(mode, sync)))
 
 
 def qk_norm_rope(q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, heads, kv_heads, head_dim=128, positions=None,
@@ -731,28 +737,26 @@ def qk_norm_rope(q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, heads, kv_hea
 
     q [T, heads * hd], k [T, kv_heads * hd] (either may be None with 0 heads); cos / sin
     [P, hd / 2] or None (the norm alone); positions int32 [T], or None for pos0 + t."""
-    mode = _device_of((q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, positions))
-    T = q.shape[0] if q is not None else k.shape[0]
-    (pqd, lqd), (pq, lq) = _matrix(q_dst, T, heads * head_dim, "q_dst"), _matrix(q, T, heads * head_dim, "q")
-    (pkd, lkd), (pk, lk) = _matrix(k_dst, T, kv_heads * head_dim, "k_dst"), _matrix(k, T, kv_heads * head_dim, "k")
+    first = q if q is not None else k
+    mode = _side(first)
+    T, wq, wk, half = first.shape[0], heads * head_dim, kv_heads * head_dim, head_dim // 2
     rows = cos.shape[0] if cos is not None else 0
-    tables = []
-    for a, what in ((cos, "cos"), (sin, "sin")):
-        p, ld = _matrix(a, rows, head_dim // 2, what)
-        if a is not None and (a.shape[1] != head_dim // 2 or ld != head_dim // 2):
-            raise ValueError(f"{what}: expected a contiguous [{rows}, {head_dim // 2}], got {list(a.shape)}")
-        tables.append(p)
-    return _check(lib().envg_qk_norm_rope(pqd, lqd, pkd, lkd, pq, lq, pk, lk, _vector(q_weight, head_dim, "q_weight"),
-                                          _vector(k_weight, head_dim, "k_weight"), *tables, rows,
-                                          _vector(positions, T, "positions", "int32"), pos0, T, heads, kv_heads,
-                                          head_dim, eps, 1 if interleaved else 0, _flags(mode, sync)))
+    return _check(lib().envg_qk_norm_rope(
+        _QK_NORM_ROPE.pack(*_matrix(q_dst, T, wq, "q_dst", mode), *_matrix(k_dst, T, wk, "k_dst", mode),
+                           *_matrix(q, T, wq, "q", mode), *_matrix(k, T, wk, "k", mode),
+                           _vector(q_weight, head_dim, "q_weight", mode), _vector(k_weight, head_dim, "k_weight", mode),
+                           _packed(cos, rows, half, "cos", mode), _packed(sin, rows, half, "sin", mode), rows,
+                           _vector(positions, T, "positions", mode, "int32"), pos0, T, heads, kv_heads, head_dim, eps,
+                           1 if interleaved else 0), _flags(mode, sync)))
 
 
-def _table(table, ctx_lens, batch):
-    p, ld = _matrix(table, batch, 0, "table", "int32")
-    if batch > 1 and ld != table.shape[1]:
-        raise TypeError("table: must be contiguous")
-    return p, table.shape[1], _vector(ctx_lens, batch, "ctx_lens", "int32")
+def _table(table, ctx_lens, batch, mode):
+    return (_packed(table, batch, table.shape[1], "table", mode, "int32"), table.shape[1],
+            _vector(ctx_lens, batch, "ctx_lens", mode, "int32"))
+
+
+def _handle(obj):
+    return obj.h.value if obj.h is not None else 0
 
 
 class KV4Cache:
@@ -768,11 +772,11 @@ class KV4Cache:
         self.pages, self.page_size, self.kv_heads, self.head_dim, self.h = pages, page_size, kv_heads, head_dim, h
 
     def _rows(self, call, k, v, table, ctx_lens, q_len, sync):
-        mode = _device_of((k, v, table, ctx_lens))
+        mode = _side(k)
         B, width = ctx_lens.shape[0], self.kv_heads * self.head_dim
-        (pk, lk), (pv, lv) = _matrix(k, B * q_len, width, "k"), _matrix(v, B * q_len, width, "v")
-        pt, stride, pl = _table(table, ctx_lens, B)
-        return _check(call(self.h, pk, lk, pv, lv, pt, stride, pl, B, q_len, _flags(mode, sync)))
+        return _check(call(_KV4_ROWS.pack(_handle(self), *_matrix(k, B * q_len, width, "k", mode),
+                                          *_matrix(v, B * q_len, width, "v", mode), *_table(table, ctx_lens, B, mode),
+                                          B, q_len), _flags(mode, sync)))
 
     def append(self, k, v, table, ctx_lens, q_len=1, sync=True):
         """Write the newest ``q_len`` tokens of each sequence; k, v [B * q_len, kv_heads * hd]: envg_kv4_append."""
@@ -799,14 +803,14 @@ def attention_kv4(dst, q, cache, table, ctx_lens, heads, q_len=1, max_ctx=0, win
 
     q, dst [B * q_len, heads * hd]; causal, with ``window`` > 0 only the last ``window`` tokens and the
     first ``sinks``; ``max_ctx`` (0: unknown) is the largest of ctx_lens and only plans the launch."""
-    mode = _device_of((dst, q, table, ctx_lens))
+    mode = _side(q)
     B, width = ctx_lens.shape[0], heads * cache.head_dim
-    (po, lo), (pq, lq) = _matrix(dst, B * q_len, width, "dst"), _matrix(q, B * q_len, width, "q")
-    pt, stride, pl = _table(table, ctx_lens, B)
     if scale is None:
         scale = cache.head_dim ** -0.5
-    return _check(lib().envg_attention_kv4(po, lo, pq, lq, cache.h, pt, stride, pl, B, q_len, max_ctx, heads, window,
-                                           sinks, scale, _flags(mode, sync)))
+    return _check(lib().envg_attention_kv4(
+        _ATTENTION_KV4.pack(*_matrix(dst, B * q_len, width, "dst", mode), *_matrix(q, B * q_len, width, "q", mode),
+                            _handle(cache), *_table(table, ctx_lens, B, mode), B, q_len, max_ctx, heads, window, sinks,
+                            scale), _flags(mode, sync)))
 
 
 # ---------------------------------------------------------------------------------------------

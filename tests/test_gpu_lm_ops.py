@@ -163,16 +163,17 @@ def test_linear_q4_refusals(gpu):
     W = gpu.Q4Weight(codes, scales, z, K=128, group=64)
     x, y = np.zeros((2, 128), np.float32), np.zeros((2, 64), np.float32)
     L = gpu.lib()
-    call = lambda **k: L.envg_linear_q4(*{**dict(dst=y.ctypes.data, ldd=64, x=x.ctypes.data, ldx=128, W=W.h, bias=None, M=2, K=128, N=64, epi=0, gate=None, flags=0), **k}.values())  # noqa: E731
+    call = lambda **k: L.envg_linear_q4(gpu._LINEAR_Q4.pack(*{**dict(dst=y.ctypes.data, ldd=64, x=x.ctypes.data, ldx=128, W=W.h.value, bias=0, gate=0, M=2, K=128, N=64, epi=0), **k}.values()), 0)  # noqa: E731
     assert call() == gpu.OK
     for bad in (dict(K=127), dict(N=63), dict(M=-1), dict(ldx=127), dict(ldd=63), dict(epi=gpu.EPI_BIAS), dict(epi=gpu.EPI_SILU_GATE),
-                dict(epi=gpu.EPI_GATED_RESIDUAL), dict(epi=9), dict(dst=None), dict(x=None), dict(x=y.ctypes.data, ldx=128)):
+                dict(epi=gpu.EPI_GATED_RESIDUAL), dict(epi=9), dict(dst=0), dict(x=0), dict(x=y.ctypes.data, ldx=128)):
         assert call(**bad) == gpu.ERR_ARG, bad
         assert gpu.last_error()
-    assert call(W=None) == gpu.ERR_STATE
-    assert call(M=0, dst=None, x=None) == gpu.OK
+    assert L.envg_linear_q4(None, 0) == gpu.ERR_ARG
+    assert call(W=0) == gpu.ERR_STATE
+    assert call(M=0, dst=0, x=0) == gpu.OK
     plain = gpu.Weight(np.zeros((64, 128), np.uint16))
-    assert call(W=plain.h) == gpu.ERR_STATE  # a 16-bit weight is not a 4-bit one, and the other way
+    assert call(W=plain.h.value) == gpu.ERR_STATE  # a 16-bit weight is not a 4-bit one, and the other way
     assert L.envg_linear(y.ctypes.data, x.ctypes.data, W.h, None, 2, 128, 64, 0, None, 0) == gpu.ERR_STATE
     with pytest.raises(ValueError, match="group"):
         gpu.Q4Weight(codes, scales, z, K=128, group=48)

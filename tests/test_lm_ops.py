@@ -60,10 +60,10 @@ def test_binding_refuses_before_any_call():
     with pytest.raises(TypeError, match="scales"):
         envg.Q4Weight(np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.float64), group=64)
     with pytest.raises(TypeError, match="adjacent"):
-        envg._matrix(f[:, ::2], 2, 64, "x")
+        envg._matrix(f[:, ::2], 2, 64, "x", envg.HOST_PTRS)
     with pytest.raises(TypeError, match="overlap"):
-        envg._matrix(np.lib.stride_tricks.as_strided(f, (2, 64), (4, 4)), 2, 64, "x")
-    assert envg._matrix(f[:, 3:60], 2, 57, "x")[1] == 128
+        envg._matrix(np.lib.stride_tricks.as_strided(f, (2, 64), (4, 4)), 2, 64, "x", envg.HOST_PTRS)
+    assert envg._matrix(f[:, 3:60], 2, 57, "x", envg.HOST_PTRS)[1] == 128
 
 
 def test_calls_before_init_return_state_error():
@@ -75,8 +75,8 @@ def test_calls_before_init_return_state_error():
     except ImportError:
         pass
     L = envg.lib()
-    assert L.envg_linear_q4(None, 0, None, 0, None, None, 1, 1, 1, 0, None, 0) == envg.ERR_STATE
-    assert L.envg_qk_norm_rope(*([None, 0] * 4), None, None, None, None, 0, None, 0, 1, 1, 0, 128, 1e-6, 0, 0) == envg.ERR_STATE
+    for call in (L.envg_linear_q4, L.envg_qk_norm_rope, L.envg_kv4_append, L.envg_kv4_read, L.envg_attention_kv4):
+        assert call(None, 0) == envg.ERR_STATE
     for go in (lambda: envg.KV4Cache(4, 16, 1, 128),
                lambda: envg.Q4Weight(np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.float32), group=64)):
         with pytest.raises(envg.EnvgError) as e:
@@ -84,3 +84,20 @@ def test_calls_before_init_return_state_error():
         assert e.value.code == envg.ERR_STATE
     assert L.envg_kv4_free(None) == envg.ERR_STATE and L.envg_q4weight_free(None) == envg.ERR_STATE
     assert L.envg_weight_upload_q4(None, None, None, 1, 1, 32, 0, 0, None) == envg.ERR_ARG
+
+
+def test_packed_structures_match_the_header(tmp_path):
+    """The binding packs each argument structure as the C compiler lays it out."""
+    import os
+    import subprocess
+
+    names = {"envg_linear_q4_args": envg._LINEAR_Q4, "envg_qk_norm_rope_args": envg._QK_NORM_ROPE,
+             "envg_kv4_rows": envg._KV4_ROWS, "envg_attention_kv4_args": envg._ATTENTION_KV4}
+    last = {"envg_linear_q4_args": "epilogue", "envg_qk_norm_rope_args": "interleaved", "envg_kv4_rows": "q_len",
+            "envg_attention_kv4_args": "scale"}
+    src = tmp_path / "s.c"
+    src.write_text("#include <stdio.h>\n#include <stddef.h>\n#include \"envgemm.h\"\nint main(void) {\n" + "".join(
+        f'printf("%zu\\n", offsetof({n}, {last[n]}) + 4);\n' for n in names) + "return 0; }\n")
+    subprocess.check_call(["gcc", "-I", os.path.dirname(envg.HEADER_PATH), str(src), "-o", str(tmp_path / "s")])
+    sizes = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in sizes] == [st.size for st in names.values()]
