@@ -381,9 +381,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
-    const float up = __int_as_float((127 + e) << 23);  // e is in [-113, 126]
+    const int e = scale_exp(top);
+    const float up = pow2(e);
     const int from = 8 * t;                            // a lane whose g / 2 is this thread's t
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
@@ -394,7 +393,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
     }
-    cq[nb] = __int_as_float((127 - __shfl_sync(0xffffffffu, e, from)) << 23) * a.sl2;
+    cq[nb] = pow2(-__shfl_sync(0xffffffffu, e, from)) * a.sl2;
     const int mr = row0 + 4 * nb + t;
     pos[nb] = mr < rows ? len - a.q_len + mr / per_kv : -1;
 #pragma unroll

@@ -59,6 +59,14 @@ ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// The power of two e that takes a row's largest magnitude to [2^14, 2^15) (at most 2^126; 0 for an
+// infinity, whose row ends non-finite anyway), and 2^e.
+ENVG_DEV int scale_exp(float top) {
+  const int field = (int)(__float_as_uint(top) >> 23);
+  return field == 255 ? 0 : min(126, 141 - field);
+}
+ENVG_DEV float pow2(int e) { return __int_as_float((127 + e) << 23); }
+
 // Four consecutive floats, as one access where `vec` (the address is 16-byte aligned).
 ENVG_DEV float4 ld_f4(const float* p, bool vec) {
   if (vec) return *reinterpret_cast<const float4*>(p);

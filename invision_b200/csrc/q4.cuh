@@ -179,18 +179,28 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   fence_mbar_init();
   __syncwarp();
   // the warp's blocks: of each round (R tiles), an even share of its (tile, block) pairs
-  auto share = [&](int r0, int w) { return (int)((int64_t)min(R, tile1 - r0) * kbn * w / Q4_WARPS); };
-  int fr = tile0, fi = share(tile0, warp), fe = share(tile0, warp + 1);  // next block to fetch: round, index, end
+  auto share = [&](int r0, int w) { return min(R, tile1 - r0) * kbn * w / Q4_WARPS; };
+  int fr = tile0, left = 0, fkb = 0;  // next block to fetch: its round, how many of the round are left, its place in the row
+  const uint8_t* next = nullptr;
+  auto fetch_round = [&]() {
+    const int i = share(fr, warp);
+    left = share(fr, warp + 1) - i;
+    const int j = kbn > 0 ? i / kbn : 0;
+    fkb = i - j * kbn;
+    next = a.w.base + ((int64_t)(fr + j) * a.w.kblocks + kb0 + fkb) * BLOCK;
+  };
+  fetch_round();
+  const int64_t row_step = (int64_t)(a.w.kblocks - kbn) * BLOCK;
   auto fetch = [&](int st) {
-    while (fi >= fe && fr + R < tile1) fr += R, fi = share(fr, warp), fe = share(fr, warp + 1);
-    if (fi >= fe) return;
+    while (left == 0 && fr + R < tile1) fr += R, fetch_round();
+    if (left == 0) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(bars + 8 * st, BLOCK);
-      const int j = fi / kbn;
-      bulk_load(smem_u32(ring + st * BLOCK), a.w.base + ((int64_t)(fr + j) * a.w.kblocks + kb0 + fi - j * kbn) * BLOCK, BLOCK,
-                bars + 8 * st);
+      bulk_load(smem_u32(ring + st * BLOCK), next, BLOCK, bars + 8 * st);
     }
-    ++fi;
+    --left;
+    next += BLOCK;
+    if (++fkb == kbn) fkb = 0, next += row_step;
   };
   for (int i = 0; i < p.stages; ++i) fetch(i);
   griddep_wait();
@@ -213,9 +223,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) e = min(126, 14 - ilogbf(top));
-    const float up = __int_as_float((127 + e) << 23);
+    const int e = scale_exp(top);
+    const float up = pow2(e);
     v.x *= up, v.y *= up, v.z *= up, v.w *= up;
     const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
     const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     u.z = __byte_perm(a1, c1, 0x5410), u.w = __byte_perm(a1, c1, 0x7632);
     const int word = lane >> 3, tt = (lane >> 1) & 3;
     *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) = u;
-    if (lane == 0) xs[kb * MC + m] = __int_as_float((127 - e) << 23);
+    if (lane == 0) xs[kb * MC + m] = pow2(-e);
   }
   if (p.splits > 1) cluster_sync();  // every CTA of the cluster is there to be written to
   else __syncthreads();
@@ -243,11 +252,11 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   uint32_t phase = 0;
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
+    int i = share(r0, warp), j = kbn > 0 ? i / kbn : 0, kb = i - j * kbn;
     const int i1 = share(r0, warp + 1);
     float acc[NT][2] = {};
-    for (int i = share(r0, warp); i < i1 && fine; ++i) {
-      const int j = i / kbn, kb = i - j * kbn;
-      fine = wait_bounded(bars + 8 * st, phase, wc, SITE_Q4_RING);
+    for (; i < i1; ++i) {
+      fine = fine && wait_bounded(bars + 8 * st, phase, wc, SITE_Q4_RING);
       if (!__all_sync(0xffffffffu, fine)) {
         fine = false;
         break;
@@ -255,10 +264,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       const uint8_t* blk = ring + st * BLOCK;
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
-      float xsc[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) xsc[nt] = xs[kb * MC + 4 * nt + t];
-      const uint8_t* xk = xf + (size_t)kb * MC * S::X_ROW + g * 64 + t * 16;
+      float sum[NT][2] = {};
+      const uint8_t* xk = xf + kb * (MC * S::X_ROW) + g * 64 + t * 16;
 #pragma unroll
       for (int gi = 0; gi < PER; ++gi) {
         const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         // 1024 + z, and -(64 + z) for 16 times the code
         const __half2 zl0 = bits_h2(z0 * 0x00010001u + magic), zh0 = bits_h2(z0 * 0x00100010u + 0xD400D400u);
         const __half2 zl1 = bits_h2(z1 * 0x00010001u + magic), zh1 = bits_h2(z1 * 0x00100010u + 0xD400D400u);
-        float d[NT][4];
+        float d[2][NT][4];  // two chains of products where a group has more than one word
 #pragma unroll
         for (int wi = 0; wi < 4 / PER; ++wi) {
           const int w = gi * (4 / PER) + wi;
@@ -283,26 +290,37 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint32_t bb[2] = {h ? xw[nt].z : xw[nt].x, h ? xw[nt].w : xw[nt].y};
-              if (wi == 0 && h == 0) mma_f16_zero(d[nt], A0, A1, A2, A3, bb);
-              else mma_f16(d[nt], A0, A1, A2, A3, bb);
+              if (wi < 2 && h == 0) mma_f16_zero(d[wi & 1][nt], A0, A1, A2, A3, bb);
+              else mma_f16(d[wi & 1][nt], A0, A1, A2, A3, bb);
             }
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[nt][0] = fmaf(d[nt][0] + d[nt][1], s0 * xsc[nt], acc[nt][0]);
-          acc[nt][1] = fmaf(d[nt][2] + d[nt][3], s1 * xsc[nt], acc[nt][1]);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2) {
+            float v = d[0][nt][2 * i2] + d[0][nt][2 * i2 + 1];
+            if (PER < 4) v += d[1][nt][2 * i2] + d[1][nt][2 * i2 + 1];
+            sum[nt][i2] = fmaf(v, i2 ? s1 : s0, sum[nt][i2]);
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float xsc = xs[kb * MC + 4 * nt + t];
+        acc[nt][0] = fmaf(sum[nt][0], xsc, acc[nt][0]);
+        acc[nt][1] = fmaf(sum[nt][1], xsc, acc[nt][1]);
       }
       __syncwarp();  // every lane has read the stage
       fetch(st);
       if (++st == p.stages) st = 0, phase ^= 1;
-      if (kb == kbn - 1 || i == i1 - 1) {  // the warp leaves the tile
+      ++kb;
+      if (kb == kbn || i + 1 == i1) {  // the warp leaves the tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 64 + 2 * lane) = make_float2(acc[nt][0], acc[nt][1]);
           acc[nt][0] = acc[nt][1] = 0.0f;
         }
+        kb = 0, ++j;
       }
     }
     __syncthreads();
