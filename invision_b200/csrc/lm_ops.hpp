@@ -124,7 +124,8 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
   for (int s = 1; s <= 8; s *= 2) {
     const int kb = (int)cdiv(w.kblocks, s);
     const int room = Q4_SMEM - S::FIXED - S::x_bytes(kb);
-    const int stages = std::min(Q4_MAX_STAGES, room / (Q4_WARPS * q4_block_bytes(w.group)));
+    int stages = room / (Q4_WARPS * q4_block_bytes(w.group));
+    stages = stages >= 6 ? 6 : stages >= 4 ? 4 : stages;
     if (stages < 3 || kb * (s - 1) >= w.kblocks) continue;  // (every CTA has work)
     const int clusters = (int)std::min<int64_t>(w.tiles, q4_clusters(d, s));
     const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
@@ -181,8 +182,6 @@ int launch_q4(Dev* d, const Q4Args& a) {
   ProfScope ps(stream_of(d), KID_Q4, 2.0 * a.M * (double)a.w.N * (double)a.w.K, bytes);
   Q4Plan p{};
   p.vec = f4_ok(a.x, a.ldx);
-  p.wait_cap_ns = d->wait_cap_ns;
-  p.status = d->d_status;
   // 16, 8 or 4 rows at a time: as many as there are, fewer where K leaves no room for their parts
   if (a.M > 8 && q4_plan<4>(d, a.w, &p)) return launch_q4_n<4>(d, a, p);
   if (a.M > 4 && q4_plan<2>(d, a.w, &p)) return launch_q4_n<2>(d, a, p);

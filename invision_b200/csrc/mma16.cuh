@@ -53,6 +53,16 @@ ENVG_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t 
                "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
                : "memory");
 }
+// Sixteen bytes from global to shared memory by this thread, in its current group of such copies.
+ENVG_DEV void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(__cvta_generic_to_global(src)) : "memory");
+}
+ENVG_DEV void copy_group_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Wait until at most N of this thread's newest groups are still under way.
+template <int N>
+ENVG_DEV void copy_groups_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

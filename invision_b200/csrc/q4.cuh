@@ -120,21 +120,19 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
 // Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
 // of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
 // (tile, block) pairs are cut evenly among its warps, each of which streams its run of blocks
-// through a ring of bulk copies and leaves one sum per tile it touched in shared memory; the sums
-// are added in warp order and, in a cluster, handed to the tile's owner and added in rank order.
-// Weights do not depend on the previous kernel: the ring starts before waiting for it.
-constexpr int Q4_WARPS = 16, Q4_THREADS = 32 * Q4_WARPS, Q4_MAX_STAGES = 8;
+// through a ring of its own (a lane copies the codes that it will read itself) and leaves one sum
+// per tile it touched in shared memory; the sums are added in warp order and, in a cluster, handed
+// to the tile's owner and added in rank order.  Weights do not depend on the previous kernel: the
+// ring starts before waiting for it.
+constexpr int Q4_WARPS = 16, Q4_THREADS = 32 * Q4_WARPS;
 constexpr int Q4_SMEM = 227 * 1024;
-constexpr int SITE_Q4_RING = 61;  // status[1] of a ring wait that ran out
 
 struct Q4Plan {
   int splits;         // CTAs of a cluster: K ranges
   int clusters;       // runs of tiles
   int kb_per;         // blocks of K per CTA
-  int stages;         // ring depth
+  int stages;         // ring depth: 6, 4 or 3
   int vec;            // rows of x are 16-byte aligned
-  uint64_t wait_cap_ns;
-  int* status;
 };
 template <int NT>
 struct Q4Smem {
@@ -143,7 +141,7 @@ struct Q4Smem {
   static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
   static constexpr int RECV = R * SUMS;       // [ranks][tiles of the owner], used by clusters
   static constexpr int X_ROW = 4 * Q4_COLS;   // bytes of x's parts per (row, block)
-  static constexpr int FIXED = SLOTS + RECV + Q4_WARPS * Q4_MAX_STAGES * 8 + 16;
+  static constexpr int FIXED = SLOTS + RECV;
   __host__ __device__ static int x_bytes(int kb) { return kb * 4 * NT * (X_ROW + 4); }
   __host__ __device__ static int total(int kb, int stages, int group) {
     return FIXED + x_bytes(kb) + Q4_WARPS * stages * q4_block_bytes(group);
@@ -162,8 +160,6 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float* slots = reinterpret_cast<float*>(smem);
   float* recv = reinterpret_cast<float*>(smem + S::SLOTS);
-  const uint32_t bars = smem_u32(smem + S::SLOTS + S::RECV) + warp * Q4_MAX_STAGES * 8;
-  volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::SLOTS + S::RECV + Q4_WARPS * Q4_MAX_STAGES * 8);
   uint8_t* xf = smem + S::FIXED;                                         // [kb][word][row][part][t] 16 bytes
   float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // [kb][row] 2^-e
   uint8_t* ring = xf + S::x_bytes(p.kb_per) + warp * p.stages * BLOCK;
@@ -173,11 +169,6 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   const int tile0 = (int)((int64_t)a.w.tiles * cl / p.clusters), tile1 = (int)((int64_t)a.w.tiles * (cl + 1) / p.clusters);
   const int m0 = blockIdx.y * MC, mn = min(MC, a.M - m0);
 
-  if (lane == 0)
-    for (int i = 0; i < p.stages; ++i) mbar_init(bars + 8 * i, 1);
-  if (threadIdx.x == 0) *abort_s = 0;
-  fence_mbar_init();
-  __syncwarp();
   // the warp's blocks: of each round (R tiles), an even share of its (tile, block) pairs
   auto share = [&](int r0, int w) { return min(R, tile1 - r0) * kbn * w / Q4_WARPS; };
   int fr = tile0, left = 0, fkb = 0;  // next block to fetch: its round, how many of the round are left, its place in the row
@@ -191,76 +182,86 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   };
   fetch_round();
   const int64_t row_step = (int64_t)(a.w.kblocks - kbn) * BLOCK;
-  auto fetch = [&](int st) {
+  const uint32_t ring_s = smem_u32(ring);
+  auto fetch = [&](int st) {  // one group of copies, empty past the warp's last block
     while (left == 0 && fr + R < tile1) fr += R, fetch_round();
-    if (left == 0) return;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(bars + 8 * st, BLOCK);
-      bulk_load(smem_u32(ring + st * BLOCK), next, BLOCK, bars + 8 * st);
+    if (left > 0) {
+      const uint32_t dst = ring_s + st * BLOCK + lane * 16;
+      copy16_async(dst, next + lane * 16);
+      copy16_async(dst + 512, next + 512 + lane * 16);
+      if (lane < 5 * PER) copy16_async(dst + 1024, next + 1024 + lane * 16);
+      --left;
+      next += BLOCK;
+      if (++fkb == kbn) fkb = 0, next += row_step;
     }
-    --left;
-    next += BLOCK;
-    if (++fkb == kbn) fkb = 0, next += row_step;
+    copy_group_end();
   };
   for (int i = 0; i < p.stages; ++i) fetch(i);
   griddep_wait();
   griddep_launch_dependents();
 
   // x of this K range as operand parts: a warp takes 128 columns of a row at a time
-  for (int i = warp; i < kbn * MC; i += Q4_WARPS) {
-    const int kb = i / MC, m = i % MC, k = (kb0 + kb) * Q4_COLS + 4 * lane;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m < mn) {
-      const float* src = a.x + (int64_t)(m0 + m) * a.ldx + k;
-      if (k + 3 < a.w.K) {
-        v = ld_f4(src, p.vec != 0);
-      } else {
-        if (k < a.w.K) v.x = src[0];
-        if (k + 1 < a.w.K) v.y = src[1];
-        if (k + 2 < a.w.K) v.z = src[2];
+  constexpr int AHEAD = 8;  // loads of a warp under way at a time
+  for (int i0 = warp; i0 < kbn * MC; i0 += AHEAD * Q4_WARPS) {
+    float4 in[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC, k = (kb0 + kb) * Q4_COLS + 4 * lane;
+      in[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (kb < kbn && m < mn) {
+        const float* src = a.x + (int64_t)(m0 + m) * a.ldx + k;
+        if (k + 3 < a.w.K) {
+          in[u] = ld_f4(src, p.vec != 0);
+        } else {
+          if (k < a.w.K) in[u].x = src[0];
+          if (k + 1 < a.w.K) in[u].y = src[1];
+          if (k + 2 < a.w.K) in[u].z = src[2];
+        }
       }
     }
-    float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = scale_exp(top);
-    const float up = pow2(e);
-    v.x *= up, v.y *= up, v.z *= up, v.w *= up;
-    const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
-    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-    const uint32_t l0 = h2_bits(__floats2half2_rn(v.x - b0.x, v.y - b0.y)), l1 = h2_bits(__floats2half2_rn(v.z - b1.x, v.w - b1.y));
-    // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
-    // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
-    const bool odd = lane & 1;
-    const uint32_t s0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
-    const uint32_t a0 = odd ? s0 : h2_bits(h0), a1 = odd ? s1 : h2_bits(h1), c0 = odd ? l0 : s0, c1 = odd ? l1 : s1;
-    uint4 u;
-    u.x = __byte_perm(a0, c0, 0x5410), u.y = __byte_perm(a0, c0, 0x7632);
-    u.z = __byte_perm(a1, c1, 0x5410), u.w = __byte_perm(a1, c1, 0x7632);
-    const int word = lane >> 3, tt = (lane >> 1) & 3;
-    *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) = u;
-    if (lane == 0) xs[kb * MC + m] = pow2(-e);
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC;
+      if (kb >= kbn) break;
+      float4 v = in[u];
+      float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = scale_exp(top);
+      const float up = pow2(e);
+      v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+      const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+      const uint32_t l0 = h2_bits(__floats2half2_rn(v.x - b0.x, v.y - b0.y)), l1 = h2_bits(__floats2half2_rn(v.z - b1.x, v.w - b1.y));
+      // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
+      // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+      const bool odd = lane & 1;
+      const uint32_t s0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
+      const uint32_t a0 = odd ? s0 : h2_bits(h0), a1 = odd ? s1 : h2_bits(h1), c0 = odd ? l0 : s0, c1 = odd ? l1 : s1;
+      uint4 out;
+      out.x = __byte_perm(a0, c0, 0x5410), out.y = __byte_perm(a0, c0, 0x7632);
+      out.z = __byte_perm(a1, c1, 0x5410), out.w = __byte_perm(a1, c1, 0x7632);
+      const int word = lane >> 3, tt = (lane >> 1) & 3;
+      *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) = out;
+      if (lane == 0) xs[kb * MC + m] = pow2(-e);
+    }
   }
   if (p.splits > 1) cluster_sync();  // every CTA of the cluster is there to be written to
   else __syncthreads();
 
-  const WaitCtl wc{p.wait_cap_ns, p.status, abort_s, 0};
   const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
   const __half2 c16 = __float2half2_rn(0.0625f);
-  bool fine = true;
   int st = 0;
-  uint32_t phase = 0;
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
     int i = share(r0, warp), j = kbn > 0 ? i / kbn : 0, kb = i - j * kbn;
     const int i1 = share(r0, warp + 1);
     float acc[NT][2] = {};
     for (; i < i1; ++i) {
-      fine = fine && wait_bounded(bars + 8 * st, phase, wc, SITE_Q4_RING);
-      if (!__all_sync(0xffffffffu, fine)) {
-        fine = false;
-        break;
-      }
+      if (p.stages == 6) copy_groups_wait<5>();
+      else if (p.stages == 4) copy_groups_wait<3>();
+      else copy_groups_wait<2>();
+      __syncwarp();  // the scales were copied by other lanes
       const uint8_t* blk = ring + st * BLOCK;
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       }
       __syncwarp();  // every lane has read the stage
       fetch(st);
-      if (++st == p.stages) st = 0, phase ^= 1;
+      if (++st == p.stages) st = 0;
       ++kb;
       if (kb == kbn || i + 1 == i1) {  // the warp leaves the tile
 #pragma unroll
@@ -362,8 +363,6 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     }
     if (r0 + R < tile1) cluster_sync();  // the next round's sums may come when all have read these
   }
-  if (!fine && lane == 0)  // given up: no copy may be in flight when the CTA leaves
-    for (int i = 0; i < p.stages; ++i) wait_drain(bars + 8 * i, 0, p.wait_cap_ns), wait_drain(bars + 8 * i, 1, p.wait_cap_ns);
 }
 
 }  // namespace envg
