@@ -171,32 +171,36 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
 
   // the warp's blocks: of each round (R tiles), an even share of its (tile, block) pairs
   auto share = [&](int r0, int w) { return min(R, tile1 - r0) * kbn * w / Q4_WARPS; };
-  int fr = tile0, left = 0, fkb = 0;  // next block to fetch: its round, how many of the round are left, its place in the row
-  const uint8_t* next = nullptr;
+  const int stage_end = p.stages * BLOCK;
+  const uint32_t ring_s = smem_u32(ring) + lane * 16;
+  int fr = tile0, left = 0, run = 0;  // fetching: the round, its blocks left, those up to the end of their row
+  const uint8_t* next = nullptr;      // the lane's piece of the next one
   auto fetch_round = [&]() {
-    const int i = share(fr, warp);
+    const int i = share(fr, warp), j = kbn > 0 ? i / kbn : 0;
     left = share(fr, warp + 1) - i;
-    const int j = kbn > 0 ? i / kbn : 0;
-    fkb = i - j * kbn;
-    next = a.w.base + ((int64_t)(fr + j) * a.w.kblocks + kb0 + fkb) * BLOCK;
+    run = min(left, (j + 1) * kbn - i);
+    next = a.w.base + ((int64_t)(fr + j) * a.w.kblocks + kb0 + i - j * kbn) * BLOCK + lane * 16;
   };
   fetch_round();
-  const int64_t row_step = (int64_t)(a.w.kblocks - kbn) * BLOCK;
-  const uint32_t ring_s = smem_u32(ring);
-  auto fetch = [&](int st) {  // one group of copies, empty past the warp's last block
-    while (left == 0 && fr + R < tile1) fr += R, fetch_round();
-    if (left > 0) {
-      const uint32_t dst = ring_s + st * BLOCK + lane * 16;
-      copy16_async(dst, next + lane * 16);
-      copy16_async(dst + 512, next + 512 + lane * 16);
-      if (lane < 5 * PER) copy16_async(dst + 1024, next + 1024 + lane * 16);
-      --left;
+  auto fetch = [&](int at) {  // one group of copies to ring offset `at`, empty past the warp's last block
+    if (run == 0) {
+      if (left > 0) {
+        run = min(left, kbn);
+        next += (int64_t)(a.w.kblocks - kbn) * BLOCK;
+      } else {
+        while (left == 0 && fr + R < tile1) fr += R, fetch_round();
+      }
+    }
+    if (run > 0) {
+      copy16_async(ring_s + at, next);
+      copy16_async(ring_s + at + 512, next + 512);
+      if (lane < 5 * PER) copy16_async(ring_s + at + 1024, next + 1024);
+      --left, --run;
       next += BLOCK;
-      if (++fkb == kbn) fkb = 0, next += row_step;
     }
     copy_group_end();
   };
-  for (int i = 0; i < p.stages; ++i) fetch(i);
+  for (int i = 0; i < p.stages; ++i) fetch(i * BLOCK);
   griddep_wait();
   griddep_launch_dependents();
 
@@ -251,22 +255,24 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
 
   const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
   const __half2 c16 = __float2half2_rn(0.0625f);
-  int st = 0;
+  int at = 0;  // ring offset
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
-    int i = share(r0, warp), j = kbn > 0 ? i / kbn : 0, kb = i - j * kbn;
-    const int i1 = share(r0, warp + 1);
+    int i = share(r0, warp), j = kbn > 0 ? i / kbn : 0;
+    int more = share(r0, warp + 1) - i;              // blocks of the round left
+    int row = min(more, (j + 1) * kbn - i);          // of them in this tile
+    const uint8_t* xk = xf + (i - j * kbn) * (MC * S::X_ROW) + g * 64 + t * 16;
+    const float* xsk = xs + (i - j * kbn) * MC + t;
     float acc[NT][2] = {};
-    for (; i < i1; ++i) {
+    for (; more > 0; --more) {
       if (p.stages == 6) copy_groups_wait<5>();
       else if (p.stages == 4) copy_groups_wait<3>();
       else copy_groups_wait<2>();
       __syncwarp();  // the scales were copied by other lanes
-      const uint8_t* blk = ring + st * BLOCK;
+      const uint8_t* blk = ring + at;
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
       float sum[NT][2] = {};
-      const uint8_t* xk = xf + kb * (MC * S::X_ROW) + g * 64 + t * 16;
 #pragma unroll
       for (int gi = 0; gi < PER; ++gi) {
         const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
@@ -307,21 +313,24 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float xsc = xs[kb * MC + 4 * nt + t];
+        const float xsc = xsk[4 * nt];
         acc[nt][0] = fmaf(sum[nt][0], xsc, acc[nt][0]);
         acc[nt][1] = fmaf(sum[nt][1], xsc, acc[nt][1]);
       }
       __syncwarp();  // every lane has read the stage
-      fetch(st);
-      if (++st == p.stages) st = 0;
-      ++kb;
-      if (kb == kbn || i + 1 == i1) {  // the warp leaves the tile
+      fetch(at);
+      at += BLOCK;
+      if (at == stage_end) at = 0;
+      xk += MC * S::X_ROW, xsk += MC;
+      if (--row == 0) {  // the warp leaves the tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 64 + 2 * lane) = make_float2(acc[nt][0], acc[nt][1]);
           acc[nt][0] = acc[nt][1] = 0.0f;
         }
-        kb = 0, ++j;
+        ++j;
+        row = min(more - 1, kbn);
+        xk = xf + g * 64 + t * 16, xsk = xs + t;
       }
     }
     __syncthreads();
