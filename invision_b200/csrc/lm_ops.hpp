@@ -112,7 +112,6 @@ int q4_clusters(const Dev* d, int s) {
     cudaGetLastError();
     n = std::max(1, d->sms / (2 * s));
   }
-  if (getenv("X_V")) fprintf(stderr, "clusters of %d: %d\n", s, n);
   return n;
 }
 
@@ -123,14 +122,13 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
   bool found = false;
   for (int s = 1; s <= 8; s *= 2) {
     const int kb = (int)cdiv(w.kblocks, s);
-    const int room = Q4_SMEM - S::FIXED - S::x_bytes(kb);
+    const int room = Q4_SMEM - S::FIXED - S::x_bytes(kb, w.group);
     int stages = room / (Q4_WARPS * q4_block_bytes(w.group));
     stages = stages >= 6 ? 6 : stages >= 4 ? 4 : stages;
     if (stages < 3 || kb * (s - 1) >= w.kblocks) continue;  // (every CTA has work)
     const int clusters = (int)std::min<int64_t>(w.tiles, q4_clusters(d, s));
     const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
     if (found && cost >= least) continue;
-    if (getenv("X_S") && atoi(getenv("X_S")) != s) continue;
     least = cost, found = true;
     best->splits = s, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
   }
@@ -145,7 +143,7 @@ int launch_q4_t(Dev* d, const Q4Args& a, const Q4Plan& p) {
     attr_set[d->id] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.clusters * p.splits), (unsigned)cdiv(a.M, 4 * NT));
+  cfg.gridDim = dim3((unsigned)(p.clusters * p.splits), (unsigned)cdiv(a.M, Q4Smem<NT>::MC));
   cfg.blockDim = dim3(Q4_THREADS);
   cfg.dynamicSmemBytes = Q4Smem<NT>::total(p.kb_per, p.stages, GROUP);
   cfg.stream = stream_of(d);
@@ -182,9 +180,10 @@ int launch_q4(Dev* d, const Q4Args& a) {
   ProfScope ps(stream_of(d), KID_Q4, 2.0 * a.M * (double)a.w.N * (double)a.w.K, bytes);
   Q4Plan p{};
   p.vec = f4_ok(a.x, a.ldx);
-  // 16, 8 or 4 rows at a time: as many as there are, fewer where K leaves no room for their parts
-  if (a.M > 8 && q4_plan<4>(d, a.w, &p)) return launch_q4_n<4>(d, a, p);
-  if (a.M > 4 && q4_plan<2>(d, a.w, &p)) return launch_q4_n<2>(d, a, p);
+  // 16, 8, 4 or 2 rows at a time: as many as there are, fewer where K leaves no room for their digits
+  if (a.M > 8 && q4_plan<8>(d, a.w, &p)) return launch_q4_n<8>(d, a, p);
+  if (a.M > 4 && q4_plan<4>(d, a.w, &p)) return launch_q4_n<4>(d, a, p);
+  if (a.M > 2 && q4_plan<2>(d, a.w, &p)) return launch_q4_n<2>(d, a, p);
   if (q4_plan<1>(d, a.w, &p)) return launch_q4_n<1>(d, a, p);
   return fail(ENVG_ERR_UNSUPPORTED, "linear_q4: K=%lld is too long", (long long)a.w.K);
 }

@@ -63,6 +63,27 @@ template <int N>
 ENVG_DEV void copy_groups_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// m16n8k32 on 8-bit integers with 32-bit sums, 16-row operand unsigned, 8-column operand signed;
+// from a zero accumulator where ZERO.
+template <bool ZERO>
+ENVG_DEV void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (ZERO)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A fixed-point value as four signed digits to the base 256, one to a byte.
+ENVG_DEV uint32_t digits256(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
+// The power of two e that takes a row's largest magnitude to [2^29, 2^30), where it and all smaller
+// fp32 values down to 2^-6 of it are held exactly (at most 2^126: beyond that only denormals round).
+ENVG_DEV int fixed_exp(float top) {
+  const int field = (int)(__float_as_uint(top) >> 23);
+  return field == 255 ? 0 : min(126, 156 - field);
+}
 ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

@@ -106,16 +106,17 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
   }
 }
 
-// k_q4: y = x . W^T over the 4-bit blocks, 4 NT rows of x per launch row.
+// k_q4: y = x . W^T over the 4-bit blocks, 2 NT rows of x per launch row.
 //
-// Mathematics.  Of a block, group gi adds s[n][gi] sum_k (c[n][k] - z[n][gi]) x[m][k].  The products
-// run on the tensor cores as m16n8k16: c - z, exact as an fp16, is the 16-row operand (c or 16 c is
-// put into the mantissa of 1024, then one subtraction or multiply-add.  A bare c would be a
-// subnormal, which the cores align by its nominal exponent and so lose up to ten low bits of x);
-// x is the 8-column one, each row of it in two fp16 parts in adjacent columns, scaled by a power of
-// two per (row, block) so that its largest value is in [2^14, 2^15).  Each group's fp32 sum starts
-// from zero, gets both parts added and is then multiplied by its scale: nothing is rounded to 16
-// bits, and the cores' cutting off of low bits stays within one group.
+// Mathematics.  Of a block, group gi adds s[n][gi] sum_k (c[n][k] - z[n][gi]) x[m][k].  The sums run
+// on the tensor cores as 8-bit integer m16n8k32 products, exactly: codes are the unsigned 16-row
+// operand (two logic operations unpack four of them); x, held per (row, block) as a fixed-point
+// number of 31 bits relative to its largest value, is the 8-column one, in four signed digits to
+// the base 256, a row's in adjacent columns.  A thread joins its two digits' sums and takes off
+// z sum(x) in integers, converts once and multiplies by the group's scale and the digits' weight;
+// the two threads of a row are added when the tile is left.  (fp16 operands with x in two parts
+// gave the same accuracy but cost nine operations for eight codes against three, and this kernel
+// is bound by instruction issue: 22.2 us against 14 at 4 x 4096 x 36864.)
 //
 // Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
 // of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
@@ -136,15 +137,17 @@ struct Q4Plan {
 };
 template <int NT>
 struct Q4Smem {
-  static constexpr int R = NT == 4 ? 16 : 32;   // tiles at a time
-  static constexpr int SUMS = NT * 2 * 32 * 4;  // bytes of one tile's sums
+  static constexpr int MC = 2 * NT;             // rows of x
+  static constexpr int R = NT == 8 ? 16 : 32;   // tiles at a time
+  static constexpr int SUMS = NT * 128;         // bytes of one tile's sums
   static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
-  static constexpr int RECV = R * SUMS;       // [ranks][tiles of the owner], used by clusters
-  static constexpr int X_ROW = 4 * Q4_COLS;   // bytes of x's parts per (row, block)
+  static constexpr int RECV = R * SUMS;         // [ranks][tiles of the owner], used by clusters
   static constexpr int FIXED = SLOTS + RECV;
-  __host__ __device__ static int x_bytes(int kb) { return kb * 4 * NT * (X_ROW + 4); }
+  static constexpr int X_ROW = 4 * Q4_COLS;     // bytes of x's digits per (row, block)
+  // digits, their sums per group (two pairs of digits) and the pairs' weights, per block
+  __host__ __device__ static int x_bytes(int kb, int group) { return kb * MC * (X_ROW + 8 * (Q4_COLS / group) + 8); }
   __host__ __device__ static int total(int kb, int stages, int group) {
-    return FIXED + x_bytes(kb) + Q4_WARPS * stages * q4_block_bytes(group);
+    return FIXED + x_bytes(kb, group) + Q4_WARPS * stages * q4_block_bytes(group);
   }
 };
 
@@ -155,14 +158,15 @@ ENVG_DEV void st_cluster_f2(uint32_t addr, float x, float y) {
 template <int NT, int GROUP>
 __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Plan p) {
   using S = Q4Smem<NT>;
-  constexpr int R = S::R, BLOCK = q4_block_bytes(GROUP), PER = Q4_COLS / GROUP, MC = 4 * NT;
+  constexpr int R = S::R, BLOCK = q4_block_bytes(GROUP), PER = Q4_COLS / GROUP, MC = S::MC;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float* slots = reinterpret_cast<float*>(smem);
   float* recv = reinterpret_cast<float*>(smem + S::SLOTS);
-  uint8_t* xf = smem + S::FIXED;                                         // [kb][word][row][part][t] 16 bytes
-  float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // [kb][row] 2^-e
-  uint8_t* ring = xf + S::x_bytes(p.kb_per) + warp * p.stages * BLOCK;
+  uint8_t* xf = smem + S::FIXED;                                      // [kb][word pair][row][digit][t][word] 8 bytes
+  int* xt = reinterpret_cast<int*>(xf + p.kb_per * MC * S::X_ROW);    // [kb][group][row][digit pair]
+  float* xs = reinterpret_cast<float*>(xt + p.kb_per * PER * MC * 2);  // [kb][row][digit pair] weight
+  uint8_t* ring = xf + S::x_bytes(p.kb_per, GROUP) + warp * p.stages * BLOCK;
 
   const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x / p.splits;
   const int kb0 = rank * p.kb_per, kbn = max(0, min(p.kb_per, a.w.kblocks - kb0));
@@ -204,7 +208,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   griddep_wait();
   griddep_launch_dependents();
 
-  // x of this K range as operand parts: a warp takes 128 columns of a row at a time
+  // x of this K range as digits: a warp takes 128 columns of a row at a time
   constexpr int AHEAD = 8;  // loads of a warp under way at a time
   for (int i0 = warp; i0 < kbn * MC; i0 += AHEAD * Q4_WARPS) {
     float4 in[AHEAD];
@@ -227,42 +231,59 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC;
       if (kb >= kbn) break;
-      float4 v = in[u];
-      float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int e = scale_exp(top);
+      const float4 v = in[u];
+      // magnitudes as integers order as floats do, and keep a NaN on top
+      uint32_t top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                         max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int e = fixed_exp(__uint_as_float(top));
       const float up = pow2(e);
-      v.x *= up, v.y *= up, v.z *= up, v.w *= up;
-      const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
-      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-      const uint32_t l0 = h2_bits(__floats2half2_rn(v.x - b0.x, v.y - b0.y)), l1 = h2_bits(__floats2half2_rn(v.z - b1.x, v.w - b1.y));
-      // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
-      // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+      const uint32_t x0 = digits256(__float2int_rn(v.x * up)), x1 = digits256(__float2int_rn(v.y * up));
+      const uint32_t x2 = digits256(__float2int_rn(v.z * up)), x3 = digits256(__float2int_rn(v.w * up));
+      // A word's columns go in as (0, 2, 4, 6) and (1, 3, 5, 7); lanes 2 i and 2 i + 1 hold columns
+      // 0..3 and 4..7.  The even lane collects digits 0 and 1, the odd one digits 2 and 3.
       const bool odd = lane & 1;
-      const uint32_t s0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
-      const uint32_t a0 = odd ? s0 : h2_bits(h0), a1 = odd ? s1 : h2_bits(h1), c0 = odd ? l0 : s0, c1 = odd ? l1 : s1;
-      uint4 out;
-      out.x = __byte_perm(a0, c0, 0x5410), out.y = __byte_perm(a0, c0, 0x7632);
-      out.z = __byte_perm(a1, c1, 0x5410), out.w = __byte_perm(a1, c1, 0x7632);
+      const uint32_t l0 = __byte_perm(x0, x2, 0x5140), l1 = __byte_perm(x1, x3, 0x5140);  // digits 0, 1
+      const uint32_t h0 = __byte_perm(x0, x2, 0x7362), h1 = __byte_perm(x1, x3, 0x7362);  // digits 2, 3
+      const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? l0 : h0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? l1 : h1, 1);
+      const uint32_t lo0 = odd ? r0 : l0, lo1 = odd ? r1 : l1, hi0 = odd ? h0 : r0, hi1 = odd ? h1 : r1;
       const int word = lane >> 3, tt = (lane >> 1) & 3;
-      *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) = out;
-      if (lane == 0) xs[kb * MC + m] = pow2(-e);
+      uint2* out = reinterpret_cast<uint2*>(xf + (((((kb * 2 + (word >> 1)) * MC + m) * 4 + (odd ? 2 : 0)) * 4 + tt) * 2 + (word & 1)) * 8);
+      out[0] = make_uint2(__byte_perm(lo0, hi0, 0x5410), __byte_perm(lo1, hi1, 0x5410));
+      out[8] = make_uint2(__byte_perm(lo0, hi0, 0x7632), __byte_perm(lo1, hi1, 0x7632));
+      // a block with an infinity or a NaN makes its row's outputs NaN
+      if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? __int_as_float(0x7fc00000) : pow2(-e)) * (lane ? 65536.0f : 1.0f);
     }
   }
   if (p.splits > 1) cluster_sync();  // every CTA of the cluster is there to be written to
   else __syncthreads();
+  // sums of x's digits per group, by products with codes of one
+  for (int kb = warp; kb < kbn; kb += Q4_WARPS)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int d[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint2 b = *reinterpret_cast<const uint2*>(xf + ((((kb * 2 + (w >> 1)) * MC + 2 * nt) * 4 + g) * 8 + t * 2 + (w & 1)) * 8);
+        if (w % (4 / PER) == 0) mma_u8s8<true>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
+        else mma_u8s8<false>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
+        if (w % (4 / PER) == 4 / PER - 1 && g == 0) xt[((kb * PER + w / (4 / PER)) * MC + 2 * nt) * 2 + t] = d[1] * 256 + d[0];
+      }
+    }
+  __syncthreads();
 
-  const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
-  const __half2 c16 = __float2half2_rn(0.0625f);
+  const uint32_t nib = in_register(0x0F0F0F0Fu);
   int at = 0;  // ring offset
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
-    int i = share(r0, warp), j = kbn > 0 ? i / kbn : 0;
-    int more = share(r0, warp + 1) - i;              // blocks of the round left
-    int row = min(more, (j + 1) * kbn - i);          // of them in this tile
-    const uint8_t* xk = xf + (i - j * kbn) * (MC * S::X_ROW) + g * 64 + t * 16;
-    const float* xsk = xs + (i - j * kbn) * MC + t;
+    const int i = share(r0, warp);
+    int j = kbn > 0 ? i / kbn : 0;
+    int more = share(r0, warp + 1) - i;      // blocks of the round left
+    int row = min(more, (j + 1) * kbn - i);  // of them in this tile
+    int kb = i - j * kbn;
+    const uint8_t* xk = xf + kb * (MC * S::X_ROW) + lane * 16;
+    const int* xtk = xt + kb * (PER * MC * 2) + t;
+    const float* xsk = xs + kb * (MC * 2) + t;
     float acc[NT][2] = {};
     for (; more > 0; --more) {
       if (p.stages == 6) copy_groups_wait<5>();
@@ -273,85 +294,76 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
       float sum[NT][2] = {};
+      int d[NT][4];
+      uint4 xw[NT];  // x's digits for two words
 #pragma unroll
-      for (int gi = 0; gi < PER; ++gi) {
-        const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
-        const uint32_t z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
-        // 1024 + z, and -(64 + z) for 16 times the code
-        const __half2 zl0 = bits_h2(z0 * 0x00010001u + magic), zh0 = bits_h2(z0 * 0x00100010u + 0xD400D400u);
-        const __half2 zl1 = bits_h2(z1 * 0x00010001u + magic), zh1 = bits_h2(z1 * 0x00100010u + 0xD400D400u);
-        float d[2][NT][4];  // two chains of products where a group has more than one word
+      for (int w = 0; w < 4; ++w) {
+        const int gi = w / (4 / PER);
+        if (w % 2 == 0)
 #pragma unroll
-        for (int wi = 0; wi < 4 / PER; ++wi) {
-          const int w = gi * (4 / PER) + wi;
-          uint4 xw[NT];  // the word's eight columns of x, for both of its products
+          for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + ((w >> 1) * MC + 2 * nt) * 256);
+        const uint32_t a0 = w0[w] & nib, a1 = w1[w] & nib, a2 = (w0[w] >> 4) & nib, a3 = (w1[w] >> 4) & nib;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + (w * MC + 4 * nt) * 128);
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t b0 = w % 2 ? xw[nt].z : xw[nt].x, b1 = w % 2 ? xw[nt].w : xw[nt].y;
+          if (w % (4 / PER) == 0) mma_u8s8<true>(d[nt], a0, a1, a2, a3, b0, b1);
+          else mma_u8s8<false>(d[nt], a0, a1, a2, a3, b0, b1);
+        }
+        if (w % (4 / PER) == 4 / PER - 1) {
+          const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
+          const int z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t u0 = h ? w0[w] >> 8 : w0[w], u1 = h ? w1[w] >> 8 : w1[w];
-            const uint32_t A0 = h2_bits(__hsub2(bits_h2(and_or(u0, mask0, magic)), zl0));
-            const uint32_t A1 = h2_bits(__hsub2(bits_h2(and_or(u1, mask0, magic)), zl1));
-            const uint32_t A2 = h2_bits(__hfma2(bits_h2(and_or(u0, mask1, magic)), c16, zh0));
-            const uint32_t A3 = h2_bits(__hfma2(bits_h2(and_or(u1, mask1, magic)), c16, zh1));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t bb[2] = {h ? xw[nt].z : xw[nt].x, h ? xw[nt].w : xw[nt].y};
-              if (wi < 2 && h == 0) mma_f16_zero(d[wi & 1][nt], A0, A1, A2, A3, bb);
-              else mma_f16(d[wi & 1][nt], A0, A1, A2, A3, bb);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            const int xsum = xtk[(gi * MC + 2 * nt) * 2];
+            sum[nt][0] = fmaf((float)(d[nt][1] * 256 + d[nt][0] - z0 * xsum), s0, sum[nt][0]);
+            sum[nt][1] = fmaf((float)(d[nt][3] * 256 + d[nt][2] - z1 * xsum), s1, sum[nt][1]);
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i2 = 0; i2 < 2; ++i2) {
-            float v = d[0][nt][2 * i2] + d[0][nt][2 * i2 + 1];
-            if (PER < 4) v += d[1][nt][2 * i2] + d[1][nt][2 * i2 + 1];
-            sum[nt][i2] = fmaf(v, i2 ? s1 : s0, sum[nt][i2]);
-          }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float xsc = xsk[4 * nt];
-        acc[nt][0] = fmaf(sum[nt][0], xsc, acc[nt][0]);
-        acc[nt][1] = fmaf(sum[nt][1], xsc, acc[nt][1]);
+        const float wt = xsk[4 * nt];
+        acc[nt][0] = fmaf(sum[nt][0], wt, acc[nt][0]);
+        acc[nt][1] = fmaf(sum[nt][1], wt, acc[nt][1]);
       }
       __syncwarp();  // every lane has read the stage
       fetch(at);
       at += BLOCK;
       if (at == stage_end) at = 0;
-      xk += MC * S::X_ROW, xsk += MC;
+      xk += MC * S::X_ROW, xtk += PER * MC * 2, xsk += MC * 2;
       if (--row == 0) {  // the warp leaves the tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 64 + 2 * lane) = make_float2(acc[nt][0], acc[nt][1]);
+          const float y0 = acc[nt][0] + __shfl_xor_sync(0xffffffffu, acc[nt][0], 1);
+          const float y1 = acc[nt][1] + __shfl_xor_sync(0xffffffffu, acc[nt][1], 1);
+          if (!(t & 1)) *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 32 + lane) = make_float2(y0, y1);
           acc[nt][0] = acc[nt][1] = 0.0f;
         }
         ++j;
         row = min(more - 1, kbn);
-        xk = xf + g * 64 + t * 16, xsk = xs + t;
+        xk = xf + lane * 16, xtk = xt + t, xsk = xs + t;
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < tiles * NT * 32; i += Q4_THREADS) {
-      const int j = i / (NT * 32), nt = (i / 32) % NT, ln = i & 31;
+    // item: (tile, pair of rows of x, row g of the tile and row of the pair), as the slots hold them
+    for (int it = threadIdx.x; it < tiles * NT * 16; it += Q4_THREADS) {
+      const int jt = it / (NT * 16), nt = (it / 16) % NT, at2 = 2 * (it & 15);
       float2 v = make_float2(0.0f, 0.0f);
       if (kbn > 0) {
         // warp of block b: the last w whose share starts at or before b
-        const int wa = (int)(((int64_t)j * kbn + 1) * Q4_WARPS - 1) / nb, wb = (int)(((int64_t)(j + 1) * kbn) * Q4_WARPS - 1) / nb;
+        const int wa = ((jt * kbn + 1) * Q4_WARPS - 1) / nb, wb = ((jt + 1) * kbn * Q4_WARPS - 1) / nb;
         for (int w = wa; w <= wb; ++w) {
           if (nb * w / Q4_WARPS == nb * (w + 1) / Q4_WARPS) continue;  // a warp without a block
-          const float2 s = *reinterpret_cast<const float2*>(slots + ((j + w) * NT + nt) * 64 + 2 * ln);
+          const float2 s = *reinterpret_cast<const float2*>(slots + ((jt + w) * NT + nt) * 32 + at2);
           v.x += s.x, v.y += s.y;
         }
       }
       if (p.splits == 1) {
-        const int m = 4 * nt + (ln & 3);
-        if (m < mn) q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
+        const int m = 2 * nt + (it & 1);
+        if (m < mn) q4_store(a, r0 + jt, (it & 15) >> 1, m0 + m, v.x, v.y);
       } else {
-        const int owner = j % p.splits, at = rank * (R / p.splits) + j / p.splits;
-        st_cluster_f2(mapa_shared(smem_u32(recv + (at * NT + nt) * 64 + 2 * ln), owner), v.x, v.y);
+        const int owner = jt % p.splits, to = rank * (R / p.splits) + jt / p.splits;
+        st_cluster_f2(mapa_shared(smem_u32(recv + (to * NT + nt) * 32 + at2), owner), v.x, v.y);
       }
     }
     if (p.splits == 1) {
@@ -360,15 +372,15 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     }
     cluster_sync();
     const int each = R / p.splits;
-    for (int i = threadIdx.x; i < each * NT * 32; i += Q4_THREADS) {
-      const int jj = i / (NT * 32), j = jj * p.splits + rank, nt = (i / 32) % NT, ln = i & 31, m = 4 * nt + (ln & 3);
-      if (j >= tiles || m >= mn) continue;
+    for (int it = threadIdx.x; it < each * NT * 16; it += Q4_THREADS) {
+      const int jj = it / (NT * 16), jt = jj * p.splits + rank, nt = (it / 16) % NT, m = 2 * nt + (it & 1);
+      if (jt >= tiles || m >= mn) continue;
       float2 v = make_float2(0.0f, 0.0f);
       for (int q = 0; q < p.splits; ++q) {
-        const float2 s = *reinterpret_cast<const float2*>(recv + ((q * each + jj) * NT + nt) * 64 + 2 * ln);
+        const float2 s = *reinterpret_cast<const float2*>(recv + ((q * each + jj) * NT + nt) * 32 + 2 * (it & 15));
         v.x += s.x, v.y += s.y;
       }
-      q4_store(a, r0 + j, ln >> 2, m0 + m, v.x, v.y);
+      q4_store(a, r0 + jt, (it & 15) >> 1, m0 + m, v.x, v.y);
     }
     if (r0 + R < tile1) cluster_sync();  // the next round's sums may come when all have read these
   }
