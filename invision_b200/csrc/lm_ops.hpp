@@ -107,17 +107,17 @@ int q4_clusters(const Dev* d, int s) {
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)s, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(k_q4<1, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, k_q4<1, 128>, &cfg) != cudaSuccess || n < 1) {
+  if (cudaFuncSetAttribute(k_q4<1, 128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, k_q4<1, 128, false>, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
     n = std::max(1, d->sms / (2 * s));
   }
   return n;
 }
 
-template <int NT>
+template <int NT, bool HALF>
 bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
-  using S = Q4Smem<NT>;
+  using S = Q4Smem<NT, HALF>;
   double least = 0.0;
   bool found = false;
   for (int s = 1; s <= 8; s *= 2) {
@@ -131,21 +131,22 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
     if (found && cost >= least) continue;
     least = cost, found = true;
     best->splits = s, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
+    best->each = w.tiles / clusters, best->rest = w.tiles % clusters;
   }
   return found;
 }
 
-template <int NT, int GROUP>
+template <int NT, int GROUP, bool HALF>
 int launch_q4_t(Dev* d, const Q4Args& a, const Q4Plan& p) {
   static bool attr_set[64] = {};
   if (!attr_set[d->id]) {
-    ENVG_CUDA(cudaFuncSetAttribute(k_q4<NT, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM));
+    ENVG_CUDA(cudaFuncSetAttribute(k_q4<NT, GROUP, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4_SMEM));
     attr_set[d->id] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.clusters * p.splits), (unsigned)cdiv(a.M, Q4Smem<NT>::MC));
+  cfg.gridDim = dim3((unsigned)(p.clusters * p.splits), (unsigned)cdiv(a.M, Q4Smem<NT, HALF>::MC));
   cfg.blockDim = dim3(Q4_THREADS);
-  cfg.dynamicSmemBytes = Q4Smem<NT>::total(p.kb_per, p.stages, GROUP);
+  cfg.dynamicSmemBytes = Q4Smem<NT, HALF>::total(p.kb_per, p.stages, GROUP);
   cfg.stream = stream_of(d);
   cudaLaunchAttribute at[2];
   int n = 0;
@@ -161,17 +162,17 @@ int launch_q4_t(Dev* d, const Q4Args& a, const Q4Plan& p) {
   }
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)n;
-  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_q4<NT, GROUP>, a, p));
+  ENVG_CUDA(cudaLaunchKernelEx(&cfg, k_q4<NT, GROUP, HALF>, a, p));
   d->st.kernel_launches++;
   return ENVG_OK;
 }
 
-template <int NT>
+template <int NT, bool HALF>
 int launch_q4_n(Dev* d, const Q4Args& a, const Q4Plan& p) {
   switch (a.w.group) {
-    case 32: return launch_q4_t<NT, 32>(d, a, p);
-    case 64: return launch_q4_t<NT, 64>(d, a, p);
-    default: return launch_q4_t<NT, 128>(d, a, p);
+    case 32: return launch_q4_t<NT, 32, HALF>(d, a, p);
+    case 64: return launch_q4_t<NT, 64, HALF>(d, a, p);
+    default: return launch_q4_t<NT, 128, HALF>(d, a, p);
   }
 }
 
@@ -180,11 +181,11 @@ int launch_q4(Dev* d, const Q4Args& a) {
   ProfScope ps(stream_of(d), KID_Q4, 2.0 * a.M * (double)a.w.N * (double)a.w.K, bytes);
   Q4Plan p{};
   p.vec = f4_ok(a.x, a.ldx);
-  // 16, 8, 4 or 2 rows at a time: as many as there are, fewer where K leaves no room for their digits
-  if (a.M > 8 && q4_plan<8>(d, a.w, &p)) return launch_q4_n<8>(d, a, p);
-  if (a.M > 4 && q4_plan<4>(d, a.w, &p)) return launch_q4_n<4>(d, a, p);
-  if (a.M > 2 && q4_plan<2>(d, a.w, &p)) return launch_q4_n<2>(d, a, p);
-  if (q4_plan<1>(d, a.w, &p)) return launch_q4_n<1>(d, a, p);
+  // 16, 8, 4 or 2 rows at a time: as many as there are, fewer where K leaves no room for their parts
+  if (a.M > 8 && q4_plan<4, true>(d, a.w, &p)) return launch_q4_n<4, true>(d, a, p);
+  if (a.M > 4 && q4_plan<2, true>(d, a.w, &p)) return launch_q4_n<2, true>(d, a, p);
+  if (a.M > 2 && q4_plan<2, false>(d, a.w, &p)) return launch_q4_n<2, false>(d, a, p);
+  if (q4_plan<1, false>(d, a.w, &p)) return launch_q4_n<1, false>(d, a, p);
   return fail(ENVG_ERR_UNSUPPORTED, "linear_q4: K=%lld is too long", (long long)a.w.K);
 }
 

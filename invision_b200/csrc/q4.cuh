@@ -106,17 +106,24 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
   }
 }
 
-// k_q4: y = x . W^T over the 4-bit blocks, 2 NT rows of x per launch row.
+// k_q4: y = x . W^T over the 4-bit blocks, MC rows of x per launch row.
 //
-// Mathematics.  Of a block, group gi adds s[n][gi] sum_k (c[n][k] - z[n][gi]) x[m][k].  The sums run
-// on the tensor cores as 8-bit integer m16n8k32 products, exactly: codes are the unsigned 16-row
-// operand (two logic operations unpack four of them); x, held per (row, block) as a fixed-point
-// number of 31 bits relative to its largest value, is the 8-column one, in four signed digits to
-// the base 256, a row's in adjacent columns.  A thread joins its two digits' sums and takes off
-// z sum(x) in integers, converts once and multiplies by the group's scale and the digits' weight;
-// the two threads of a row are added when the tile is left.  (fp16 operands with x in two parts
-// gave the same accuracy but cost nine operations for eight codes against three, and this kernel
-// is bound by instruction issue: 22.2 us against 14 at 4 x 4096 x 36864.)
+// Mathematics.  Of a block, group gi adds s[n][gi] sum_k (c[n][k] - z[n][gi]) x[m][k].  The codes are
+// the 16-row operand of the tensor cores' products, x the 8-column one, in as many parts as fp32
+// accuracy takes; a group's sum starts from zero and is multiplied by its scale in fp32.  Two forms:
+//   integers (HALF false): codes as unsigned bytes (two logic operations unpack four), x per (row,
+//     block) as a 31-bit fixed-point number in four signed digits to the base 256, a row's digits in
+//     four adjacent columns, two rows to a product.  The 32-bit sums are exact; a thread joins its two
+//     digits, takes off z sum(x) in integers, converts once; a row's two threads are added when the
+//     tile is left.
+//   halves (HALF true): c - z exact as an fp16 (put into the mantissa of 1024, then one subtraction
+//     or multiply-add; a bare c would be a subnormal, which the cores align by its nominal exponent
+//     and so lose up to ten low bits of x), x in two fp16 parts in adjacent columns, scaled by a power
+//     of two per (row, block), four rows to a product.
+// The integer form unpacks a block in 24 operations against 72, the other form spends 4 per group on
+// four rows against 18; the kernel is bound by instruction issue before it is by HBM, so few rows
+// take integers and many rows halves.  Measured, us: 1 x 2560 x 19456, groups of 64: 8.3 / 10.7;
+// 4 x 4096 x 36864, groups of 128: 20.3 / 22.2; 16 x 9728 x 2560, groups of 32: 20.0 / 16.2.
 //
 // Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
 // of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
@@ -134,18 +141,22 @@ struct Q4Plan {
   int kb_per;         // blocks of K per CTA
   int stages;         // ring depth: 6, 4 or 3
   int vec;            // rows of x are 16-byte aligned
+  int each, rest;     // tiles per cluster; the first `rest` clusters take one more
 };
-template <int NT>
+template <int NT, bool HALF>
 struct Q4Smem {
-  static constexpr int MC = 2 * NT;             // rows of x
-  static constexpr int R = NT == 8 ? 16 : 32;   // tiles at a time
-  static constexpr int SUMS = NT * 128;         // bytes of one tile's sums
+  static constexpr int RT = HALF ? 4 : 2;       // rows of x to a product
+  static constexpr int MC = RT * NT;
+  static constexpr int R = MC == 16 ? 16 : 32;  // tiles at a time
+  static constexpr int SUMS = MC * 64;          // bytes of one tile's sums
   static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
   static constexpr int RECV = R * SUMS;         // [ranks][tiles of the owner], used by clusters
   static constexpr int FIXED = SLOTS + RECV;
-  static constexpr int X_ROW = 4 * Q4_COLS;     // bytes of x's digits per (row, block)
-  // digits, their sums per group (two pairs of digits) and the pairs' weights, per block
-  __host__ __device__ static int x_bytes(int kb, int group) { return kb * MC * (X_ROW + 8 * (Q4_COLS / group) + 8); }
+  static constexpr int X_ROW = 4 * Q4_COLS;     // bytes of x's parts per (row, block)
+  // parts and their weights (one, or one to a pair of digits), digits' sums per group and pair
+  __host__ __device__ static int x_bytes(int kb, int group) {
+    return (int)((kb * MC * (X_ROW + (HALF ? 4 : 8 + 8 * (Q4_COLS / group))) + 15) & ~15);
+  }
   __host__ __device__ static int total(int kb, int stages, int group) {
     return FIXED + x_bytes(kb, group) + Q4_WARPS * stages * q4_block_bytes(group);
   }
@@ -155,22 +166,23 @@ ENVG_DEV void st_cluster_f2(uint32_t addr, float x, float y) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
 }
 
-template <int NT, int GROUP>
+template <int NT, int GROUP, bool HALF>
 __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Plan p) {
-  using S = Q4Smem<NT>;
-  constexpr int R = S::R, BLOCK = q4_block_bytes(GROUP), PER = Q4_COLS / GROUP, MC = S::MC;
+  using S = Q4Smem<NT, HALF>;
+  constexpr int R = S::R, RT = S::RT, BLOCK = q4_block_bytes(GROUP), PER = Q4_COLS / GROUP, MC = S::MC;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float* slots = reinterpret_cast<float*>(smem);
   float* recv = reinterpret_cast<float*>(smem + S::SLOTS);
-  uint8_t* xf = smem + S::FIXED;                                      // [kb][word pair][row][digit][t][word] 8 bytes
-  int* xt = reinterpret_cast<int*>(xf + p.kb_per * MC * S::X_ROW);    // [kb][group][row][digit pair]
-  float* xs = reinterpret_cast<float*>(xt + p.kb_per * PER * MC * 2);  // [kb][row][digit pair] weight
+  // integers: [kb][word pair][row][digit][t][word] 8 bytes; halves: [kb][word][row][part][t] 16 bytes
+  uint8_t* xf = smem + S::FIXED;
+  float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // weights: [kb][row][digit pair], [kb][row]
+  int* xt = reinterpret_cast<int*>(xs + p.kb_per * MC * 2);             // sums of digits: [kb][group][row][digit pair]
   uint8_t* ring = xf + S::x_bytes(p.kb_per, GROUP) + warp * p.stages * BLOCK;
 
   const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x / p.splits;
   const int kb0 = rank * p.kb_per, kbn = max(0, min(p.kb_per, a.w.kblocks - kb0));
-  const int tile0 = (int)((int64_t)a.w.tiles * cl / p.clusters), tile1 = (int)((int64_t)a.w.tiles * (cl + 1) / p.clusters);
+  const int tile0 = cl * p.each + min(cl, p.rest), tile1 = tile0 + p.each + (cl < p.rest ? 1 : 0);
   const int m0 = blockIdx.y * MC, mn = min(MC, a.M - m0);
 
   // the warp's blocks: of each round (R tiles), an even share of its (tile, block) pairs
@@ -208,8 +220,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   griddep_wait();
   griddep_launch_dependents();
 
-  // x of this K range as digits: a warp takes 128 columns of a row at a time
-  constexpr int AHEAD = 8;  // loads of a warp under way at a time
+  // x of this K range in parts: a warp takes 128 columns of a row at a time
+  constexpr int AHEAD = 10;  // loads of a warp under way at a time
   for (int i0 = warp; i0 < kbn * MC; i0 += AHEAD * Q4_WARPS) {
     float4 in[AHEAD];
 #pragma unroll
@@ -236,43 +248,61 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       uint32_t top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
                          max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
       top = __reduce_max_sync(0xffffffffu, top);
-      const int e = fixed_exp(__uint_as_float(top));
-      const float up = pow2(e);
-      const uint32_t x0 = digits256(__float2int_rn(v.x * up)), x1 = digits256(__float2int_rn(v.y * up));
-      const uint32_t x2 = digits256(__float2int_rn(v.z * up)), x3 = digits256(__float2int_rn(v.w * up));
-      // A word's columns go in as (0, 2, 4, 6) and (1, 3, 5, 7); lanes 2 i and 2 i + 1 hold columns
-      // 0..3 and 4..7.  The even lane collects digits 0 and 1, the odd one digits 2 and 3.
       const bool odd = lane & 1;
-      const uint32_t l0 = __byte_perm(x0, x2, 0x5140), l1 = __byte_perm(x1, x3, 0x5140);  // digits 0, 1
-      const uint32_t h0 = __byte_perm(x0, x2, 0x7362), h1 = __byte_perm(x1, x3, 0x7362);  // digits 2, 3
-      const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? l0 : h0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? l1 : h1, 1);
-      const uint32_t lo0 = odd ? r0 : l0, lo1 = odd ? r1 : l1, hi0 = odd ? h0 : r0, hi1 = odd ? h1 : r1;
       const int word = lane >> 3, tt = (lane >> 1) & 3;
-      uint2* out = reinterpret_cast<uint2*>(xf + (((((kb * 2 + (word >> 1)) * MC + m) * 4 + (odd ? 2 : 0)) * 4 + tt) * 2 + (word & 1)) * 8);
-      out[0] = make_uint2(__byte_perm(lo0, hi0, 0x5410), __byte_perm(lo1, hi1, 0x5410));
-      out[8] = make_uint2(__byte_perm(lo0, hi0, 0x7632), __byte_perm(lo1, hi1, 0x7632));
-      // a block with an infinity or a NaN makes its row's outputs NaN
-      if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? __int_as_float(0x7fc00000) : pow2(-e)) * (lane ? 65536.0f : 1.0f);
+      const float nan = __int_as_float(0x7fc00000);  // an infinity or a NaN makes its row's outputs NaN
+      if (HALF) {
+        const int e = scale_exp(__uint_as_float(top));
+        const float up = pow2(e), y0 = v.x * up, y1 = v.y * up, y2 = v.z * up, y3 = v.w * up;
+        const __half2 h0 = __floats2half2_rn(y0, y1), h1 = __floats2half2_rn(y2, y3);
+        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+        const uint32_t l0 = h2_bits(__floats2half2_rn(y0 - b0.x, y1 - b0.y)), l1 = h2_bits(__floats2half2_rn(y2 - b1.x, y3 - b1.y));
+        // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
+        // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
+        const uint32_t a0 = odd ? r0 : h2_bits(h0), a1 = odd ? r1 : h2_bits(h1), c0 = odd ? l0 : r0, c1 = odd ? l1 : r1;
+        *reinterpret_cast<uint4*>(xf + ((((kb * 4 + word) * MC + m) * 2 + (odd ? 1 : 0)) * 4 + tt) * 16) =
+            make_uint4(__byte_perm(a0, c0, 0x5410), __byte_perm(a0, c0, 0x7632), __byte_perm(a1, c1, 0x5410), __byte_perm(a1, c1, 0x7632));
+        if (lane == 0) xs[kb * MC + m] = top >= 0x7f800000u ? nan : pow2(-e);
+      } else {
+        const int e = fixed_exp(__uint_as_float(top));
+        const float up = pow2(e);
+        const uint32_t x0 = digits256(__float2int_rn(v.x * up)), x1 = digits256(__float2int_rn(v.y * up));
+        const uint32_t x2 = digits256(__float2int_rn(v.z * up)), x3 = digits256(__float2int_rn(v.w * up));
+        // A word's columns go in as (0, 2, 4, 6) and (1, 3, 5, 7); lanes 2 i and 2 i + 1 hold columns
+        // 0..3 and 4..7.  The even lane collects digits 0 and 1, the odd one digits 2 and 3.
+        const uint32_t l0 = __byte_perm(x0, x2, 0x5140), l1 = __byte_perm(x1, x3, 0x5140);  // digits 0, 1
+        const uint32_t h0 = __byte_perm(x0, x2, 0x7362), h1 = __byte_perm(x1, x3, 0x7362);  // digits 2, 3
+        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? l0 : h0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? l1 : h1, 1);
+        const uint32_t lo0 = odd ? r0 : l0, lo1 = odd ? r1 : l1, hi0 = odd ? h0 : r0, hi1 = odd ? h1 : r1;
+        uint2* out = reinterpret_cast<uint2*>(xf + (((((kb * 2 + (word >> 1)) * MC + m) * 4 + (odd ? 2 : 0)) * 4 + tt) * 2 + (word & 1)) * 8);
+        out[0] = make_uint2(__byte_perm(lo0, hi0, 0x5410), __byte_perm(lo1, hi1, 0x5410));
+        out[8] = make_uint2(__byte_perm(lo0, hi0, 0x7632), __byte_perm(lo1, hi1, 0x7632));
+        if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? nan : pow2(-e)) * (lane ? 65536.0f : 1.0f);
+      }
     }
   }
   if (p.splits > 1) cluster_sync();  // every CTA of the cluster is there to be written to
   else __syncthreads();
-  // sums of x's digits per group, by products with codes of one
-  for (int kb = warp; kb < kbn; kb += Q4_WARPS)
+  if (!HALF) {
+    // sums of x's digits per group, by products with codes of one
+    for (int kb = warp; kb < kbn; kb += Q4_WARPS)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      int d[4];
+      for (int nt = 0; nt < NT; ++nt) {
+        int d[4];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint2 b = *reinterpret_cast<const uint2*>(xf + ((((kb * 2 + (w >> 1)) * MC + 2 * nt) * 4 + g) * 8 + t * 2 + (w & 1)) * 8);
-        if (w % (4 / PER) == 0) mma_u8s8<true>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
-        else mma_u8s8<false>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
-        if (w % (4 / PER) == 4 / PER - 1 && g == 0) xt[((kb * PER + w / (4 / PER)) * MC + 2 * nt) * 2 + t] = d[1] * 256 + d[0];
+        for (int w = 0; w < 4; ++w) {
+          const uint2 b = *reinterpret_cast<const uint2*>(xf + ((((kb * 2 + (w >> 1)) * MC + 2 * nt) * 4 + g) * 8 + t * 2 + (w & 1)) * 8);
+          if (w % (4 / PER) == 0) mma_u8s8<true>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
+          else mma_u8s8<false>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
+          if (w % (4 / PER) == 4 / PER - 1 && g == 0) xt[((kb * PER + w / (4 / PER)) * MC + 2 * nt) * 2 + t] = d[1] * 256 + d[0];
+        }
       }
-    }
-  __syncthreads();
+    __syncthreads();
+  }
 
-  const uint32_t nib = in_register(0x0F0F0F0Fu);
+  const uint32_t nib = in_register(0x0F0F0F0Fu), mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
+  const __half2 c16 = __float2half2_rn(0.0625f);
   int at = 0;  // ring offset
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
@@ -283,7 +313,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     int kb = i - j * kbn;
     const uint8_t* xk = xf + kb * (MC * S::X_ROW) + lane * 16;
     const int* xtk = xt + kb * (PER * MC * 2) + t;
-    const float* xsk = xs + kb * (MC * 2) + t;
+    const float* xsk = xs + kb * (HALF ? MC : MC * 2) + t;
     float acc[NT][2] = {};
     for (; more > 0; --more) {
       if (p.stages == 6) copy_groups_wait<5>();
@@ -294,29 +324,70 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
       float sum[NT][2] = {};
-      int d[NT][4];
-      uint4 xw[NT];  // x's digits for two words
+      if constexpr (HALF) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int gi = w / (4 / PER);
-        if (w % 2 == 0)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + ((w >> 1) * MC + 2 * nt) * 256);
-        const uint32_t a0 = w0[w] & nib, a1 = w1[w] & nib, a2 = (w0[w] >> 4) & nib, a3 = (w1[w] >> 4) & nib;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t b0 = w % 2 ? xw[nt].z : xw[nt].x, b1 = w % 2 ? xw[nt].w : xw[nt].y;
-          if (w % (4 / PER) == 0) mma_u8s8<true>(d[nt], a0, a1, a2, a3, b0, b1);
-          else mma_u8s8<false>(d[nt], a0, a1, a2, a3, b0, b1);
-        }
-        if (w % (4 / PER) == 4 / PER - 1) {
+        for (int gi = 0; gi < PER; ++gi) {
           const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
-          const int z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
+          const uint32_t z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
+          // 1024 + z, and -(64 + z) for 16 times the code
+          const __half2 zl0 = bits_h2(z0 * 0x00010001u + magic), zh0 = bits_h2(z0 * 0x00100010u + 0xD400D400u);
+          const __half2 zl1 = bits_h2(z1 * 0x00010001u + magic), zh1 = bits_h2(z1 * 0x00100010u + 0xD400D400u);
+          float d[2][NT][4];  // two chains of products where a group has more than one word
+#pragma unroll
+          for (int wi = 0; wi < 4 / PER; ++wi) {
+            const int w = gi * (4 / PER) + wi;
+            uint4 xw[NT];  // the word's eight columns of x, for both of its products
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + (w * MC + 4 * nt) * 128);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t u0 = h ? w0[w] >> 8 : w0[w], u1 = h ? w1[w] >> 8 : w1[w];
+              const uint32_t a0 = h2_bits(__hsub2(bits_h2(and_or(u0, mask0, magic)), zl0));
+              const uint32_t a1 = h2_bits(__hsub2(bits_h2(and_or(u1, mask0, magic)), zl1));
+              const uint32_t a2 = h2_bits(__hfma2(bits_h2(and_or(u0, mask1, magic)), c16, zh0));
+              const uint32_t a3 = h2_bits(__hfma2(bits_h2(and_or(u1, mask1, magic)), c16, zh1));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t bb[2] = {h ? xw[nt].z : xw[nt].x, h ? xw[nt].w : xw[nt].y};
+                if (wi < 2 && h == 0) mma_f16_zero(d[wi & 1][nt], a0, a1, a2, a3, bb);
+                else mma_f16(d[wi & 1][nt], a0, a1, a2, a3, bb);
+              }
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i2 = 0; i2 < 2; ++i2) {
+              float v = d[0][nt][2 * i2] + d[0][nt][2 * i2 + 1];
+              if (PER < 4) v += d[1][nt][2 * i2] + d[1][nt][2 * i2 + 1];
+              sum[nt][i2] = fmaf(v, i2 ? s1 : s0, sum[nt][i2]);
+            }
+        }
+      } else {
+        int d[NT][4];
+        uint4 xw[NT];  // x's digits for two words
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int gi = w / (4 / PER);
+          if (w % 2 == 0)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) xw[nt] = *reinterpret_cast<const uint4*>(xk + ((w >> 1) * MC + 2 * nt) * 256);
+          const uint32_t a0 = w0[w] & nib, a1 = w1[w] & nib, a2 = (w0[w] >> 4) & nib, a3 = (w1[w] >> 4) & nib;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const int xsum = xtk[(gi * MC + 2 * nt) * 2];
-            sum[nt][0] = fmaf((float)(d[nt][1] * 256 + d[nt][0] - z0 * xsum), s0, sum[nt][0]);
-            sum[nt][1] = fmaf((float)(d[nt][3] * 256 + d[nt][2] - z1 * xsum), s1, sum[nt][1]);
+            const uint32_t b0 = w % 2 ? xw[nt].z : xw[nt].x, b1 = w % 2 ? xw[nt].w : xw[nt].y;
+            if (w % (4 / PER) == 0) mma_u8s8<true>(d[nt], a0, a1, a2, a3, b0, b1);
+            else mma_u8s8<false>(d[nt], a0, a1, a2, a3, b0, b1);
+          }
+          if (w % (4 / PER) == 4 / PER - 1) {
+            const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
+            const int z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int xsum = xtk[(gi * MC + 2 * nt) * 2];
+              sum[nt][0] = fmaf((float)(d[nt][1] * 256 + d[nt][0] - z0 * xsum), s0, sum[nt][0]);
+              sum[nt][1] = fmaf((float)(d[nt][3] * 256 + d[nt][2] - z1 * xsum), s1, sum[nt][1]);
+            }
           }
         }
       }
@@ -330,13 +401,18 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       fetch(at);
       at += BLOCK;
       if (at == stage_end) at = 0;
-      xk += MC * S::X_ROW, xtk += PER * MC * 2, xsk += MC * 2;
+      xk += MC * S::X_ROW, xtk += PER * MC * 2, xsk += HALF ? MC : MC * 2;
       if (--row == 0) {  // the warp leaves the tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float y0 = acc[nt][0] + __shfl_xor_sync(0xffffffffu, acc[nt][0], 1);
-          const float y1 = acc[nt][1] + __shfl_xor_sync(0xffffffffu, acc[nt][1], 1);
-          if (!(t & 1)) *reinterpret_cast<float2*>(slots + ((j + warp) * NT + nt) * 32 + lane) = make_float2(y0, y1);
+          float* slot = slots + (j + warp) * (MC * 16) + nt * (RT * 16);
+          if (HALF) {
+            *reinterpret_cast<float2*>(slot + 2 * lane) = make_float2(acc[nt][0], acc[nt][1]);
+          } else {
+            const float y0 = acc[nt][0] + __shfl_xor_sync(0xffffffffu, acc[nt][0], 1);
+            const float y1 = acc[nt][1] + __shfl_xor_sync(0xffffffffu, acc[nt][1], 1);
+            if (!(t & 1)) *reinterpret_cast<float2*>(slot + lane) = make_float2(y0, y1);
+          }
           acc[nt][0] = acc[nt][1] = 0.0f;
         }
         ++j;
@@ -345,25 +421,26 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       }
     }
     __syncthreads();
-    // item: (tile, pair of rows of x, row g of the tile and row of the pair), as the slots hold them
-    for (int it = threadIdx.x; it < tiles * NT * 16; it += Q4_THREADS) {
-      const int jt = it / (NT * 16), nt = (it / 16) % NT, at2 = 2 * (it & 15);
+    // item: (tile, product's rows of x, row g of the tile and row of x), as the slots hold them
+    constexpr int ITEMS = MC * 8;  // of a tile
+    for (int it = threadIdx.x; it < tiles * ITEMS; it += Q4_THREADS) {
+      const int jt = it / ITEMS, q = it % ITEMS;
       float2 v = make_float2(0.0f, 0.0f);
       if (kbn > 0) {
         // warp of block b: the last w whose share starts at or before b
         const int wa = ((jt * kbn + 1) * Q4_WARPS - 1) / nb, wb = ((jt + 1) * kbn * Q4_WARPS - 1) / nb;
         for (int w = wa; w <= wb; ++w) {
           if (nb * w / Q4_WARPS == nb * (w + 1) / Q4_WARPS) continue;  // a warp without a block
-          const float2 s = *reinterpret_cast<const float2*>(slots + ((jt + w) * NT + nt) * 32 + at2);
+          const float2 s = *reinterpret_cast<const float2*>(slots + (jt + w) * (MC * 16) + 2 * q);
           v.x += s.x, v.y += s.y;
         }
       }
       if (p.splits == 1) {
-        const int m = 2 * nt + (it & 1);
-        if (m < mn) q4_store(a, r0 + jt, (it & 15) >> 1, m0 + m, v.x, v.y);
+        const int m = q / (8 * RT) * RT + q % RT;
+        if (m < mn) q4_store(a, r0 + jt, q % (8 * RT) / RT, m0 + m, v.x, v.y);
       } else {
         const int owner = jt % p.splits, to = rank * (R / p.splits) + jt / p.splits;
-        st_cluster_f2(mapa_shared(smem_u32(recv + (to * NT + nt) * 32 + at2), owner), v.x, v.y);
+        st_cluster_f2(mapa_shared(smem_u32(recv + to * (MC * 16) + 2 * q), owner), v.x, v.y);
       }
     }
     if (p.splits == 1) {
@@ -372,15 +449,15 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     }
     cluster_sync();
     const int each = R / p.splits;
-    for (int it = threadIdx.x; it < each * NT * 16; it += Q4_THREADS) {
-      const int jj = it / (NT * 16), jt = jj * p.splits + rank, nt = (it / 16) % NT, m = 2 * nt + (it & 1);
+    for (int it = threadIdx.x; it < each * ITEMS; it += Q4_THREADS) {
+      const int jj = it / ITEMS, jt = jj * p.splits + rank, q = it % ITEMS, m = q / (8 * RT) * RT + q % RT;
       if (jt >= tiles || m >= mn) continue;
       float2 v = make_float2(0.0f, 0.0f);
-      for (int q = 0; q < p.splits; ++q) {
-        const float2 s = *reinterpret_cast<const float2*>(recv + ((q * each + jj) * NT + nt) * 32 + 2 * (it & 15));
+      for (int r = 0; r < p.splits; ++r) {
+        const float2 s = *reinterpret_cast<const float2*>(recv + (r * each + jj) * (MC * 16) + 2 * q);
         v.x += s.x, v.y += s.y;
       }
-      q4_store(a, r0 + jt, (it & 15) >> 1, m0 + m, v.x, v.y);
+      q4_store(a, r0 + jt, q % (8 * RT) / RT, m0 + m, v.x, v.y);
     }
     if (r0 + R < tile1) cluster_sync();  // the next round's sums may come when all have read these
   }
