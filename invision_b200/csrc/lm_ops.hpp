@@ -130,7 +130,7 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
     const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
     if (found && cost >= least) continue;
     least = cost, found = true;
-    best->splits = s, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
+    best->splits = s, best->log_splits = s == 1 ? 0 : s == 2 ? 1 : s == 4 ? 2 : 3, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
     best->each = w.tiles / clusters, best->rest = w.tiles % clusters;
   }
   return found;

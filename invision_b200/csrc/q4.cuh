@@ -136,7 +136,7 @@ constexpr int Q4_WARPS = 16, Q4_THREADS = 32 * Q4_WARPS;
 constexpr int Q4_SMEM = 227 * 1024;
 
 struct Q4Plan {
-  int splits;         // CTAs of a cluster: K ranges
+  int splits, log_splits;  // CTAs of a cluster, a power of two: K ranges
   int clusters;       // runs of tiles
   int kb_per;         // blocks of K per CTA
   int stages;         // ring depth: 6, 4 or 3
@@ -147,11 +147,11 @@ template <int NT, bool HALF>
 struct Q4Smem {
   static constexpr int RT = HALF ? 4 : 2;       // rows of x to a product
   static constexpr int MC = RT * NT;
-  static constexpr int R = MC == 16 ? 16 : 32;  // tiles at a time
+  static constexpr int R = 32;                  // tiles at a time
   static constexpr int SUMS = MC * 64;          // bytes of one tile's sums
   static constexpr int SLOTS = (R + Q4_WARPS) * SUMS;
   static constexpr int RECV = R * SUMS;         // [ranks][tiles of the owner], used by clusters
-  static constexpr int FIXED = SLOTS + RECV;
+  static constexpr int FIXED = SLOTS + RECV + R * 8;  // and each tile's first and last warp
   static constexpr int X_ROW = 4 * Q4_COLS;     // bytes of x's parts per (row, block)
   // parts and their weights (one, or one to a pair of digits), digits' sums per group and pair
   __host__ __device__ static int x_bytes(int kb, int group) {
@@ -174,13 +174,14 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float* slots = reinterpret_cast<float*>(smem);
   float* recv = reinterpret_cast<float*>(smem + S::SLOTS);
+  int2* ends = reinterpret_cast<int2*>(smem + S::SLOTS + S::RECV);
   // integers: [kb][word pair][row][digit][t][word] 8 bytes; halves: [kb][word][row][part][t] 16 bytes
   uint8_t* xf = smem + S::FIXED;
   float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // weights: [kb][row][digit pair], [kb][row]
   int* xt = reinterpret_cast<int*>(xs + p.kb_per * MC * 2);             // sums of digits: [kb][group][row][digit pair]
   uint8_t* ring = xf + S::x_bytes(p.kb_per, GROUP) + warp * p.stages * BLOCK;
 
-  const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x / p.splits;
+  const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x >> p.log_splits;
   const int kb0 = rank * p.kb_per, kbn = max(0, min(p.kb_per, a.w.kblocks - kb0));
   const int tile0 = cl * p.each + min(cl, p.rest), tile1 = tile0 + p.each + (cl < p.rest ? 1 : 0);
   const int m0 = blockIdx.y * MC, mn = min(MC, a.M - m0);
@@ -306,6 +307,10 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   int at = 0;  // ring offset
   for (int r0 = tile0; r0 < tile1; r0 += R) {
     const int tiles = min(R, tile1 - r0), nb = tiles * kbn;
+    if (threadIdx.x < tiles && kbn > 0) {  // warp of block b: the last w whose share starts at or before b
+      const int b = threadIdx.x * kbn;
+      ends[threadIdx.x] = make_int2(((b + 1) * Q4_WARPS - 1) / nb, ((b + kbn) * Q4_WARPS - 1) / nb);
+    }
     const int i = share(r0, warp);
     int j = kbn > 0 ? i / kbn : 0;
     int more = share(r0, warp + 1) - i;      // blocks of the round left
@@ -427,9 +432,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       const int jt = it / ITEMS, q = it % ITEMS;
       float2 v = make_float2(0.0f, 0.0f);
       if (kbn > 0) {
-        // warp of block b: the last w whose share starts at or before b
-        const int wa = ((jt * kbn + 1) * Q4_WARPS - 1) / nb, wb = ((jt + 1) * kbn * Q4_WARPS - 1) / nb;
-        for (int w = wa; w <= wb; ++w) {
+        const int2 e = ends[jt];
+        for (int w = e.x; w <= e.y; ++w) {
           if (nb * w / Q4_WARPS == nb * (w + 1) / Q4_WARPS) continue;  // a warp without a block
           const float2 s = *reinterpret_cast<const float2*>(slots + (jt + w) * (MC * 16) + 2 * q);
           v.x += s.x, v.y += s.y;
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         const int m = q / (8 * RT) * RT + q % RT;
         if (m < mn) q4_store(a, r0 + jt, q % (8 * RT) / RT, m0 + m, v.x, v.y);
       } else {
-        const int owner = jt % p.splits, to = rank * (R / p.splits) + jt / p.splits;
+        const int owner = jt & (p.splits - 1), to = rank * (R >> p.log_splits) + (jt >> p.log_splits);
         st_cluster_f2(mapa_shared(smem_u32(recv + to * (MC * 16) + 2 * q), owner), v.x, v.y);
       }
     }
@@ -448,9 +452,9 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       continue;
     }
     cluster_sync();
-    const int each = R / p.splits;
+    const int each = R >> p.log_splits;
     for (int it = threadIdx.x; it < each * ITEMS; it += Q4_THREADS) {
-      const int jj = it / ITEMS, jt = jj * p.splits + rank, q = it % ITEMS, m = q / (8 * RT) * RT + q % RT;
+      const int jj = it / ITEMS, jt = (jj << p.log_splits) + rank, q = it % ITEMS, m = q / (8 * RT) * RT + q % RT;
       if (jt >= tiles || m >= mn) continue;
       float2 v = make_float2(0.0f, 0.0f);
       for (int r = 0; r < p.splits; ++r) {
