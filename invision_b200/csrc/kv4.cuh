@@ -6,12 +6,13 @@
 // group holds m = fp16(min x), s = fp16((max x - min x) / 15) and codes
 // c = clamp(rint((x - m) / s), 0, 15); it stands for the values m + s c.  The codes of 16 tokens
 // lie together in one tile, tiles of a (page, kv head) follow one another:
-//   tile = K codes [16][hd / 2 bytes] | V codes [16][hd / 2 bytes] | scales [16][K s.., K m.., V s.., V m..] fp16
-// A 32-bit word holds 8 consecutive channels 64 gi + 8 r + j (nibble j, r = 0..7).  In a K row,
-// word (gi, r) stands at byte (r / 2) * hd / 8 + (2 gi + r % 2) * 4, so that lane t of a quad
-// finds the words of its 16-channel pieces side by side; in a V row at byte r * hd / 16 + 4 gi.
-// Token 8 a + 2 c + b of a tile takes V row 8 a + 4 b + c: lane t of a quad multiplies tokens 2 t,
-// 2 t + 1, 2 t + 8 and 2 t + 9, and the quad's four lanes read the rows of each side by side.
+//   tile = K codes [16][hd / 2 bytes] | V codes [hd / 64][32][16 bytes] | scales [16][K s.., K m.., V s.., V m..] fp16
+// A K row's 32-bit word holds 8 consecutive channels 64 gi + 8 r + j (nibble j, r = 0..7) and stands
+// at byte (r / 2) * hd / 8 + (2 gi + r % 2) * 4, so that lane t of a quad finds the words of its
+// 16-channel pieces side by side.  V is held the way the products over tokens take it: the 16 bytes
+// of lane 4 r + t hold channels 64 gi + 8 r .. + 7 of tokens 2 t, 2 t + 8, 2 t + 1 and 2 t + 9, byte
+// 4 i + b the two channels 2 i and 2 i + 1 of the b-th of these tokens.  A byte belongs to one
+// token, so that appending never reads what is there.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -150,9 +151,9 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(const NormRopeArgs a) {
 ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) {
   return tok * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4;
 }
-ENVG_DEV uint32_t kv_v_word(int hd, int tok, int gi, int r) {
-  const int row = (tok & 8) + 4 * (tok & 1) + ((tok >> 1) & 3);
-  return KV_TILE * (hd / 2) + row * (hd / 2) + r * (hd / 16) + 4 * gi;
+// First of the four bytes (4 apart) of V's channels 64 gi + 8 r .. + 7 of a token.
+ENVG_DEV uint32_t kv_v_byte(int hd, int tok, int gi, int r) {
+  return KV_TILE * (hd / 2) + gi * 512 + (4 * r + ((tok & 7) >> 1)) * 16 + (tok >> 3) + 2 * (tok & 1);
 }
 // Byte offset of the scale of (token, K or V, group); its minimum stands hd / 64 halves further.
 ENVG_DEV uint32_t kv_scale_at(int hd, int tok, int v, int gi) { return KV_TILE * hd + tok * (hd / 8) + v * (hd / 16) + 2 * gi; }
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
   const int tile_bytes = kv_tile_bytes(a.hd);
   uint8_t* tile = pos >= 0 ? kv_tile(a.c, b, h, pos, tile_bytes) : nullptr;
   const int tok = pos >= 0 ? pos % KV_TILE : 0;
-  const uint32_t word_at = isv ? kv_v_word(a.hd, tok, gi, r) : kv_k_word(a.hd, tok, gi, r);
+  const uint32_t word_at = isv ? kv_v_byte(a.hd, tok, gi, r) : kv_k_word(a.hd, tok, gi, r);
   const uint32_t scale_at = kv_scale_at(a.hd, tok, isv, gi);
   float* rows = isv ? a.v + row * a.ldv : a.k + row * a.ldk;
   rows += (int64_t)h * a.hd + gi * KV_GROUP + 8 * r;
@@ -197,7 +198,9 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
     if (!work) return;
     float x[8] = {};
     if (tile) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + word_at);
+      uint32_t w;
+      if (isv) w = tile[word_at] | tile[word_at + 4] << 8 | tile[word_at + 8] << 16 | (uint32_t)tile[word_at + 12] << 24;
+      else w = *reinterpret_cast<const uint32_t*>(tile + word_at);
       const float2 sm = kv_scale(tile, scale_at, a.hd);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = fmaf(sm.x, (float)((w >> (4 * j)) & 15u), sm.y);
@@ -232,7 +235,12 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
         w |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * j);
       }
     }
-    *reinterpret_cast<uint32_t*>(tile + word_at) = w;
+    if (isv) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[word_at + 4 * i] = (uint8_t)(w >> (8 * i));
+    } else {
+      *reinterpret_cast<uint32_t*>(tile + word_at) = w;
+    }
     if (r == 0) {
       __half* p = reinterpret_cast<__half*>(tile + scale_at);
       p[0] = hs, p[G] = hm;
@@ -251,7 +259,7 @@ struct KvAttnArgs {
   int64_t ldq, ldo;
   int batch, q_len, heads, hd, window, sinks;
   float sl2;  // softmax scale * log2 e
-  int vec;    // rows of q are 16-byte aligned
+  int vec, vec_out;  // rows of q, of out are 16-byte aligned
   uint64_t wait_cap_ns;
 };
 
@@ -260,14 +268,16 @@ struct KvAttnArgs {
 // Mathematics.  The rows are (query token, head) pairs that read the same kv head.  A row's score
 // of token j is sum_g s_jg (q_g . c_jg) + m_jg sum(q_g) over its groups of 64 channels, and its
 // output sum_j p_j (s_jg (c_jg - 8) + (m_jg + 8 s_jg)).  Both products with codes run on the
-// tensor cores as m16n8k16 with fp16 operands and fp32 sums, exactly in the codes, which go in as
-// c - 8 (centred: the positive codes' sums would be far larger than the result and cost its last
-// bits), so that the minimum becomes the middle m + 8 s.  The codes are the 16-row operand
-// (16 tokens of K, 16 channels of V^T), so a code is unpacked once for all rows; q and p s are the
-// 8-column one, each split into two fp16 parts in adjacent columns, so that fp32 accuracy costs no
-// further instruction.  q is scaled by a power of two per row, p s by the row maximum and by the
-// largest s seen (both folded into the exponent).  Scores come out as [token][row]; an 8 x 8
-// transpose in registers (movmatrix) makes the P operand of them.
+// tensor cores as 8-bit integer m16n8k32 products, whose 32-bit sums are exact.  The codes are the
+// unsigned 16-row operand (16 tokens of K, 16 channels of V^T), four of them unpacked by one or two
+// logic operations, once for all rows.  The other factor is the 8-column one, a fixed-point number
+// cut into digits to the base 256: q with 31 bits of its row's largest value in four signed
+// digits (two products of two adjacent columns a row), p s with 22 bits of the unit's largest in
+// three unsigned ones.  A thread joins its digits' sums, which are one row's, in integers and
+// converts once.  The c - 8 of the output comes from a start of the sums at -8 sum(p s), itself a
+// product (sums of the positive codes would be far larger than the result and cost its last bits).
+// Scores come out as [token][row]; an 8 x 8 transpose in registers (movmatrix) makes the p s operand
+// of them.
 //
 // Split.  Tokens are taken in units of two 16-token tiles, dealt out over the warps of a cluster
 // of CTAs (one cluster per sequence, kv head and 4 NB rows).  Each warp runs a one-pass softmax
@@ -360,9 +370,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   const int w_hi = n_sink + (p_lo + 1) / KV_TILE - first, w_sink = min(n_sink, a.sinks / KV_TILE);
   const int w_lo = n_sink + (a.window > 0 ? max(0, p_hi - a.window) / KV_TILE + 1 - first : 0);
 
-  // q: column g of an operand is part g % 2 of row g / 2, scaled to [2^14, 2^15) before the split,
-  // in the order of the K words' nibbles; a thread's scores are those of row t
-  uint32_t qb[NB][4 * G][2];
+  // q: columns g of the two operands are digits g % 2 and 2 + g % 2 of row g / 2, in the order of
+  // the K words' nibbles; a thread's scores are those of row t
+  uint32_t qb[NB][2 * G][2][2];
   float qs[NB][G], cq[NB];
   int pos[NB];
 #pragma unroll
@@ -371,19 +381,21 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     const bool have = rr < rows;
     const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
     const float* src = a.q + ((int64_t)b * a.q_len + qi) * a.ldq + (int64_t)qh * HD + 16 * t;
-    float x[16 * G], top = 0.0f;
+    float x[16 * G];
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4 * G; ++i) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (have) v = ld_f4(src + 64 * (i / 4) + 4 * (i % 4), a.vec != 0);
       x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[4 * i + j]) & 0x7fffffffu);
     }
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = scale_exp(top);
+    for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = fixed_exp(__uint_as_float(top));
     const float up = pow2(e);
-    const int from = 8 * t;                            // a lane whose g / 2 is this thread's t
+    const int from = 8 * t;  // a lane whose g / 2 is this thread's t
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
       float sum = 0.0f;
@@ -393,25 +405,25 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
     }
-    cq[nb] = pow2(-__shfl_sync(0xffffffffu, e, from)) * a.sl2;
+    // a row with an infinity or a NaN gives NaN
+    cq[nb] = __shfl_sync(0xffffffffu, top >= 0x7f800000u ? __int_as_float(0x7fc00000) : pow2(-e), from) * a.sl2;
     const int mr = row0 + 4 * nb + t;
     pos[nb] = mr < rows ? len - a.q_len + mr / per_kv : -1;
+    const uint32_t pick[2] = {(g & 1) ? 0x0051u : 0x0040u, (g & 1) ? 0x0073u : 0x0062u};
 #pragma unroll
-    for (int j = 0; j < 16 * G; ++j) {
-      const float v = x[j] * up;
-      const __half hi = __float2half_rn(v);
-      x[j] = (g & 1) ? v - __half2float(hi) : v;
+    for (int w = 0; w < 2 * G; ++w) {
+      uint32_t d[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = digits256(__float2int_rn(x[8 * w + j] * up));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)  // nibbles 0, 2, 4, 6 and 1, 3, 5, 7
+          qb[nb][w][n][h] = __byte_perm(__byte_perm(d[h], d[2 + h], pick[n]), __byte_perm(d[4 + h], d[6 + h], pick[n]), 0x5410);
     }
-#pragma unroll
-    for (int w = 0; w < 2 * G; ++w)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // nibbles (0, 4), (1, 5) and (2, 6), (3, 7)
-        const float* v = x + 8 * w + 2 * h;
-        qb[nb][2 * w + h][0] = h2_bits(__floats2half2_rn(v[0], v[4]));
-        qb[nb][2 * w + h][1] = h2_bits(__floats2half2_rn(v[1], v[5]));
-      }
   }
 
+  // sums of a row are held relative to 2^m, m its largest score so far rounded up to a whole power
   float o[NB][4 * G][2], m[NB], l[NB], pm[NB][G];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -421,12 +433,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
 #pragma unroll
     for (int i = 0; i < 4 * G; ++i) o[nb][i][0] = o[nb][i][1] = 0.0f;
   }
-  float rexp = -32.0f, rscale = 0.0f;  // no V scale seen is above rscale = 2^rexp
   const WaitCtl wc{a.wait_cap_ns, a.c.status, abort_s, 0};
-  // c into the mantissa of 1024, then - 1032; 16 c, then x 1/16 - 72 (a bare c would be a subnormal,
-  // which the cores align by its nominal exponent and so lose up to ten low bits of the other factor)
-  const uint32_t mask0 = in_register(0x000F000Fu), mask1 = in_register(0x00F000F0u), magic = in_register(0x64006400u);
-  const __half2 c1032 = __float2half2_rn(-1032.0f), c72 = __float2half2_rn(-72.0f), c16 = __float2half2_rn(0.0625f);
+  const uint32_t nib = in_register(0x0F0F0F0Fu);
   bool fine = true;
   int st = 0;
   uint32_t phase = 0;
@@ -442,7 +450,6 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     const uint32_t vote = (there >> (2 * (n & 15))) & 3u;
     // scores of tokens g and g + 8 of each tile, log2 units
     float x[NB][2][2], vs[2][2][G], vm[2][2][G];
-    __half2 smax = bits_h2(0u);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       const uint8_t* tile = stage + tt * S::TILE;
@@ -458,53 +465,41 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           const float2 f2 = __half22float2(bits_h2(u.z)), f3 = __half22float2(bits_h2(u.w));
           ks[i][0] = f0.x, ks[i][G - 1] = f0.y, km[i][0] = f1.x, km[i][G - 1] = f1.y;
           vs[tt][i][0] = f2.x, vs[tt][i][G - 1] = f2.y, vm[tt][i][0] = f3.x, vm[tt][i][G - 1] = f3.y;
-          smax = __hmax2(smax, bits_h2(u.z));
           const uint4 k4 = *reinterpret_cast<const uint4*>(pk);
           kw[i][0] = k4.x, kw[i][1] = k4.y, kw[i][2 * G - 2] = k4.z, kw[i][2 * G - 1] = k4.w;
         } else {
           const uint2 u = *reinterpret_cast<const uint2*>(p);
           const float2 f0 = __half22float2(bits_h2(u.x)), f1 = __half22float2(bits_h2(u.y));
           ks[i][0] = f0.x, km[i][0] = f0.y, vs[tt][i][0] = f1.x, vm[tt][i][0] = f1.y;
-          smax = __hmax2(smax, bits_h2((u.y & 0xffffu) * 0x10001u));
           const uint2 k2 = *reinterpret_cast<const uint2*>(pk);
           kw[i][0] = k2.x, kw[i][1] = k2.y;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) km[i][gi] = fmaf(8.0f, ks[i][gi], km[i][gi]);
       float mn[NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) x[nb][tt][0] = x[nb][tt][1] = mn[nb][0] = mn[nb][1] = 0.0f;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        // two chains of two products, added in rounded fp32 (see the outputs below)
-        float d[2][NB][4];
+        int d[NB][2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int w = 2 * gi + h;
+          const uint32_t a0 = kw[0][w] & nib, a1 = kw[1][w] & nib, a2 = (kw[0][w] >> 4) & nib, a3 = (kw[1][w] >> 4) & nib;
 #pragma unroll
-          for (int b8 = 0; b8 < 2; ++b8) {
-            const uint32_t u0 = b8 ? kw[0][w] >> 8 : kw[0][w], u1 = b8 ? kw[1][w] >> 8 : kw[1][w];
-            const uint32_t a0 = h2_bits(__hadd2(bits_h2(and_or(u0, mask0, magic)), c1032));
-            const uint32_t a1 = h2_bits(__hadd2(bits_h2(and_or(u1, mask0, magic)), c1032));
-            const uint32_t a2 = h2_bits(__hfma2(bits_h2(and_or(u0, mask1, magic)), c16, c72));
-            const uint32_t a3 = h2_bits(__hfma2(bits_h2(and_or(u1, mask1, magic)), c16, c72));
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              if (b8 == 0) mma_f16_zero(d[h][nb], a0, a1, a2, a3, qb[nb][2 * w]);
-              else mma_f16(d[h][nb], a0, a1, a2, a3, qb[nb][2 * w + 1]);
+            for (int k = 0; k < 2; ++k) {
+              if (h == 0) mma_u8s8<true>(d[nb][k], a0, a1, a2, a3, qb[nb][w][k][0], qb[nb][w][k][1]);
+              else mma_u8s8<false>(d[nb][k], a0, a1, a2, a3, qb[nb][w][k][0], qb[nb][w][k][1]);
             }
-          }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float sum = (d[0][nb][2 * i] + d[1][nb][2 * i]) + (d[0][nb][2 * i + 1] + d[1][nb][2 * i + 1]);
-            x[nb][tt][i] = fmaf(sum, ks[i][gi], x[nb][tt][i]);
-            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);  // km: the middle
+            const float dot = fmaf((float)(d[nb][1][2 * i + 1] * 256 + d[nb][1][2 * i]), 65536.0f, (float)(d[nb][0][2 * i + 1] * 256 + d[nb][0][2 * i]));
+            x[nb][tt][i] = fmaf(dot, ks[i][gi], x[nb][tt][i]);
+            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);
           }
       }
 #pragma unroll
@@ -516,7 +511,6 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     // score; its scale and minimum are dropped where no row sees it (they may hold anything there).
     const bool whole = vote == 3u && ((2 * unit >= w_lo && 2 * unit + 1 < w_hi) || 2 * unit + 1 < w_sink);
     if (!whole) {
-      smax = bits_h2(0u);
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -530,14 +524,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
             any |= see;
           }
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
+          for (int gi = 0; gi < G; ++gi)
             if (!any) vs[tt][i][gi] = vm[tt][i][gi] = 0.0f;
-            smax = __hmax2(smax, __float2half2_rn(vs[tt][i][gi]));
-          }
         }
     }
-    // a larger score or a larger V scale moves the exponent's reference; the scale's power of two
-    // is shared by the warp so that all rows move together
     float top[NB];
     bool moves = false;
 #pragma unroll
@@ -545,19 +535,13 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       top[nb] = fmaxf(fmaxf(x[nb][0][0], x[nb][0][1]), fmaxf(x[nb][1][0], x[nb][1][1]));
       moves |= top[nb] > m[nb];
     }
-    const float sm = fmaxf(__low2float(smax), __high2float(smax));
-    moves |= sm > rscale;
-    if (__any_sync(0xffffffffu, moves)) {
-      float need = rexp;
-      if (sm > 0.0f) need = fmaxf(need, (float)(ilogbf(sm) + 1));
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, off));
+    if (__any_sync(0xffffffffu, moves)) {  // a larger score: the sums so far are scaled down to it
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top[nb] = fmaxf(top[nb], __shfl_xor_sync(0xffffffffu, top[nb], off));
-        const float m2 = fmaxf(m[nb], top[nb]);
-        const float alpha = m[nb] == -INFINITY ? 0.0f : ex2((m[nb] + rexp) - (m2 + need));
+        const float m2 = fmaxf(m[nb], ceilf(top[nb]));
+        const float alpha = m[nb] == -INFINITY ? 0.0f : ex2(m[nb] - m2);
         m[nb] = m2;
         l[nb] *= alpha;
 #pragma unroll
@@ -565,16 +549,16 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
 #pragma unroll
         for (int i = 0; i < 4 * G; ++i) o[nb][i][0] *= alpha, o[nb][i][1] *= alpha;
       }
-      rexp = need;
-      rscale = __int_as_float((127 + (int)need) << 23);
     }
-    uint32_t pb[NB][2][G][2];
+    uint32_t pb[NB][G][2][2];  // [operand][tile]
+    float f[NB];               // what one unit of the weights' fixed-point numbers stands for
     // a token that one thread's row sees may be hidden from its other rows: 0 x NaN must not come
     // through there (with one row to a thread, what it does not see is zero already)
     auto hidden = [&](float p) { return NB > 1 && !whole && p == 0.0f; };
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] + rexp - 14.0f;
+      const float ref = m[nb] == -INFINITY ? 0.0f : m[nb];
+      float v[2][2][G], most = 0.0f;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -583,55 +567,53 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
           l[nb] += p;
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
-            const float w = hidden(p) ? 0.0f : p * vs[tt][i][gi];
             pm[nb][gi] = fmaf(p, hidden(p) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
-            // one conversion rounds w to its high part again beside the low part
-            pb[nb][tt][gi][i] = transpose_8x8(h2_bits(__floats2half2_rn(w, w - __half2float(__float2half_rn(w)))));
+            v[tt][i][gi] = hidden(p) ? 0.0f : p * vs[tt][i][gi];
+            most = fmaxf(most, v[tt][i][gi]);
           }
+        }
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+      // scaled so that the largest is in [2^21, 2^22); added to 2^23, the integer stands in the low bits
+      const int field = max(22, (int)(__float_as_uint(most) >> 23));
+      const float up = __int_as_float((275 - field) << 23);
+      f[nb] = __int_as_float((field - 21) << 23);
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          const uint32_t v0 = __float_as_uint(fmaf(v[tt][0][gi], up, 8388608.0f)), v1 = __float_as_uint(fmaf(v[tt][1][gi], up, 8388608.0f));
+          pb[nb][gi][0][tt] = transpose_8x8(__byte_perm(v0, v1, 0x5140));
+          pb[nb][gi][1][tt] = transpose_8x8(__byte_perm(v0, v1, 0x7362));  // its second column is not used
         }
     }
-    uint32_t vw[2][4][G];
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+    for (int gi = 0; gi < G; ++gi) {
+      uint32_t vw[2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = stage + tt * S::TILE + KV_TILE * (HD / 2) + (t + 4 * i) * (HD / 2) + g * (HD / 16);
-        if (G == 2) {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          vw[tt][i][0] = u.x, vw[tt][i][G - 1] = u.y;
-        } else {
-          vw[tt][i][0] = *reinterpret_cast<const uint32_t*>(p);
+      for (int tt = 0; tt < 2; ++tt) {
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + tt * S::TILE + KV_TILE * (HD / 2) + gi * 512 + lane * 16);
+        vw[tt][0] = u.x, vw[tt][1] = u.y, vw[tt][2] = u.z, vw[tt][3] = u.w;
+      }
+      int minus[NB][2][4];  // -8 times the sums of the weights' digits
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) mma_s8u8_zero(minus[nb][k], 0xF8F8F8F8u, pb[nb][gi][k][0], pb[nb][gi][k][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // channels 8 g + 2 i and 2 i + 1 of the group
+        const uint32_t a0 = vw[0][i] & nib, a1 = (vw[0][i] >> 4) & nib, a2 = vw[1][i] & nib, a3 = (vw[1][i] >> 4) & nib;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          int d[2][4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) mma_u8u8(d[k], a0, a1, a2, a3, pb[nb][gi][k][0], pb[nb][gi][k][1], minus[nb][k]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            o[nb][4 * gi + i][c] = fmaf((float)(d[1][2 * c] * 65536 + d[0][2 * c + 1] * 256 + d[0][2 * c]), f[nb], o[nb][4 * gi + i][c]);
         }
       }
-    // The tensor cores cut off what a product adds below the accumulator's last bit, always
-    // towards zero; over a long context that bias would reach 1e-5.  So each unit's two products
-    // start from zero and are added, high and low part together, in rounded fp32.
-#pragma unroll
-    for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {  // channels 8 g + j and j + 1 of the group, j = 4 half + 2 pr
-          float d[NB][4];
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt) {
-            uint32_t ab = __byte_perm(vw[tt][0][gi], vw[tt][1][gi], half ? 0x7632 : 0x5410);
-            uint32_t cd = __byte_perm(vw[tt][2][gi], vw[tt][3][gi], half ? 0x7632 : 0x5410);
-            if (pr) ab >>= 8, cd >>= 8;
-            const uint32_t a0 = h2_bits(__hadd2(bits_h2(and_or(ab, mask0, magic)), c1032));
-            const uint32_t a1 = h2_bits(__hfma2(bits_h2(and_or(ab, mask1, magic)), c16, c72));
-            const uint32_t a2 = h2_bits(__hadd2(bits_h2(and_or(cd, mask0, magic)), c1032));
-            const uint32_t a3 = h2_bits(__hfma2(bits_h2(and_or(cd, mask1, magic)), c16, c72));
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              if (tt == 0) mma_f16_zero(d[nb], a0, a1, a2, a3, pb[nb][tt][gi]);
-              else mma_f16(d[nb], a0, a1, a2, a3, pb[nb][tt][gi]);
-            }
-          }
-          const int i = 4 * gi + 2 * half + pr;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[nb][i][0] += d[nb][0] + d[nb][1], o[nb][i][1] += d[nb][2] + d[nb][3];
-        }
+    }
     __syncwarp();  // every lane has read the stage
     if (n + KVA_STAGES < mine) issue(n + KVA_STAGES, st);
     if (++st == KVA_STAGES) st = 0, phase ^= 1;
@@ -663,31 +645,39 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       }
     if (g == 0) {
       // a row of NaN scores has no maximum, but its sum is NaN and has to come through
-      ml[warp * 2 * ROWS + 4 * nb + t] = m[nb] > -INFINITY ? m[nb] + rexp : l[nb] == l[nb] ? -INFINITY : 0.0f;
+      ml[warp * 2 * ROWS + 4 * nb + t] = m[nb] > -INFINITY ? m[nb] : l[nb] == l[nb] ? -INFINITY : 0.0f;
       ml[warp * 2 * ROWS + ROWS + 4 * nb + t] = l[nb];
     }
   }
   __syncthreads();
   float* cout = reinterpret_cast<float*>(smem) + KVA_WARPS * ROWS * S::OUT_LD;
-  for (int i = threadIdx.x; i < ROWS * HD; i += KVA_THREADS) {
-    const int r = i / HD, c = i % HD, q = row0 + r;
-    if (q >= rows) break;
-    float top = -INFINITY, sum = 0.0f, y = 0.0f;
+  constexpr int QUADS = HD / 4;  // four outputs at a time
+  auto put = [&](int r, int c, float4 y, float sum, bool none) {
+    const int q = row0 + r;
+    const float by = none ? 0.0f : 1.0f / sum;
+    st_f4(a.out + ((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c,
+          none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * by, y.y * by, y.z * by, y.w * by), a.vec_out != 0);
+  };
+  for (int i = threadIdx.x; i < ROWS * QUADS; i += KVA_THREADS) {
+    const int r = i / QUADS, c = 4 * (i % QUADS);
+    if (row0 + r >= rows) break;
+    float top = -INFINITY, sum = 0.0f, mw[KVA_WARPS];
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < KVA_WARPS; ++w) top = fmaxf(top, ml[w * 2 * ROWS + r]);
+    for (int w = 0; w < KVA_WARPS; ++w) mw[w] = ml[w * 2 * ROWS + r], top = fmaxf(top, mw[w]);
 #pragma unroll
     for (int w = 0; w < KVA_WARPS; ++w) {
-      const float mw = ml[w * 2 * ROWS + r], f = mw == -INFINITY ? 0.0f : ex2(mw - top);
-      if (f > 0.0f) {
-        sum = fmaf(f, ml[w * 2 * ROWS + ROWS + r], sum);
-        y = fmaf(f, reinterpret_cast<float*>(smem)[(w * ROWS + r) * S::OUT_LD + c], y);
+      const float e = mw[w] == -INFINITY ? 0.0f : ex2(mw[w] - top);
+      if (e > 0.0f) {
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + (w * ROWS + r) * S::OUT_LD + c);
+        sum = fmaf(e, ml[w * 2 * ROWS + ROWS + r], sum);
+        y.x = fmaf(e, v.x, y.x), y.y = fmaf(e, v.y, y.y), y.z = fmaf(e, v.z, y.z), y.w = fmaf(e, v.w, y.w);
       }
     }
     if (splits == 1) {
-      a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
-          top == -INFINITY ? 0.0f : y / sum;
+      put(r, c, y, sum, top == -INFINITY);
     } else {
-      cout[r * S::OUT_LD + c] = y;
+      *reinterpret_cast<float4*>(cout + r * S::OUT_LD + c) = y;
       if (c == 0) ml[KVA_WARPS * 2 * ROWS + r] = top, ml[KVA_WARPS * 2 * ROWS + ROWS + r] = sum;
     }
   }
@@ -695,21 +685,31 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   // join the CTAs of the cluster, each writing its share of the outputs
   cluster_sync();
   const uint32_t cout_s = sbase + KVA_WARPS * ROWS * S::OUT_LD * 4, ml_s = sbase + S::ML + KVA_WARPS * 2 * ROWS * 4;
-  for (int i = rank * KVA_THREADS + threadIdx.x; i < ROWS * HD; i += splits * KVA_THREADS) {
-    const int r = i / HD, c = i % HD, q = row0 + r;
-    if (q >= rows) break;
-    float top = -INFINITY, sum = 0.0f, y = 0.0f;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, ld_cluster_f32(mapa_shared(ml_s + r * 4, s)));
-    for (int s = 0; s < splits; ++s) {
-      const float ms = ld_cluster_f32(mapa_shared(ml_s + r * 4, s));
-      const float f = ms == -INFINITY ? 0.0f : ex2(ms - top);
-      if (f > 0.0f) {
-        sum = fmaf(f, ld_cluster_f32(mapa_shared(ml_s + ROWS * 4 + r * 4, s)), sum);
-        y = fmaf(f, ld_cluster_f32(mapa_shared(cout_s + (r * S::OUT_LD + c) * 4, s)), y);
+  for (int i = rank * KVA_THREADS + threadIdx.x; i < ROWS * QUADS; i += splits * KVA_THREADS) {
+    const int r = i / QUADS, c = 4 * (i % QUADS);
+    if (row0 + r >= rows) break;
+    float top = -INFINITY, sum = 0.0f, ms[8], ls[8];
+    float4 v[8], y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      ms[s] = -INFINITY;
+      if (s < splits) {
+        ms[s] = ld_cluster_f32(mapa_shared(ml_s + r * 4, s));
+        ls[s] = ld_cluster_f32(mapa_shared(ml_s + ROWS * 4 + r * 4, s));
+        v[s] = ld_cluster_f4(mapa_shared(cout_s + (r * S::OUT_LD + c) * 4, s));
       }
     }
-    a.out[((int64_t)b * a.q_len + q / per_kv) * a.ldo + (int64_t)(kvh * per_kv + q % per_kv) * HD + c] =
-        top == -INFINITY ? 0.0f : y / sum;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) top = fmaxf(top, ms[s]);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float e = ms[s] == -INFINITY ? 0.0f : ex2(ms[s] - top);
+      if (e > 0.0f) {
+        sum = fmaf(e, ls[s], sum);
+        y.x = fmaf(e, v[s].x, y.x), y.y = fmaf(e, v[s].y, y.y), y.z = fmaf(e, v[s].z, y.z), y.w = fmaf(e, v[s].w, y.w);
+      }
+    }
+    put(r, c, y, sum, top == -INFINITY);
   }
   cluster_sync();  // no CTA leaves while others read its shared memory
 }

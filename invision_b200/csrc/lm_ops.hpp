@@ -709,7 +709,7 @@ int envg_attention_kv4(const envg_attention_kv4_args* r, int flags) {
   a.window = window, a.sinks = sinks;
   a.sl2 = scale * 1.4426950408889634f;
   a.wait_cap_ns = d->wait_cap_ns;
-  a.vec = f4_ok(a.q, a.ldq);
+  a.vec = f4_ok(a.q, a.ldq), a.vec_out = f4_ok(a.out, a.ldo);
   const int64_t most = table_stride * cache->page_size;
   ENVG_TRY(launch_kv4_attn(d, a, (int)(max_ctx > 0 ? std::min<int64_t>(max_ctx, most) : most)));
   if (!devp) ENVG_TRY(st.out(io, dst, ldo, rows, width));

@@ -1,5 +1,5 @@
 // mma16.cuh -- warp-level pieces that the 4-bit kernels share: m16n8k16 products with fp16 operands
-// and fp32 sums, an 8 x 8 transpose in registers, unpacking, untiled bulk copies and reads of a
+// and fp32 sums, m16n8k32 products of bytes with 32-bit sums, an 8 x 8 transpose in registers, unpacking, untiled bulk copies and reads of a
 // cluster's shared memory.
 //
 // mma.sync rather than tcgen05: a code has to be unpacked in registers and its group's scale has to
@@ -76,6 +76,18 @@ ENVG_DEV void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with the 8-column operand unsigned, from the accumulator c; and with a signed 16-row
+// operand from zero.
+ENVG_DEV void mma_u8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+ENVG_DEV void mma_s8u8_zero(int (&d)[4], uint32_t a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%7,%7,%7,%7};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a), "r"(b0), "r"(b1), "r"(0));
+}
 // A fixed-point value as four signed digits to the base 256, one to a byte.
 ENVG_DEV uint32_t digits256(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
 // The power of two e that takes a row's largest magnitude to [2^29, 2^30), where it and all smaller
@@ -87,6 +99,11 @@ ENVG_DEV int fixed_exp(float top) {
 ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+ENVG_DEV float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
