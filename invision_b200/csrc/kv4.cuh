@@ -43,6 +43,7 @@ struct Kv4View {
   uint8_t* base;
   int64_t pages;
   int page_size, kv_heads;
+  FastDiv page_tiles;       // by the tiles of a page
   const int32_t* table;     // [batch][table_stride] page ids
   int64_t table_stride;
   const int32_t* ctx_lens;  // [batch] tokens held, this call's q_len new ones among them
@@ -62,20 +63,25 @@ ENVG_DEV int kv_len(const Kv4View& c, int b) {
 
 // Tile of token `pos` of sequence b and kv head h; nullptr where the table names no page.
 ENVG_DEV uint8_t* kv_tile(const Kv4View& c, int b, int h, int pos, int tile_bytes) {
-  const int32_t page = __ldg(c.table + (int64_t)b * c.table_stride + pos / c.page_size);
+  const uint32_t tile = (uint32_t)pos / KV_TILE, at = c.page_tiles.div(tile);
+  const int32_t page = __ldg(c.table + (int64_t)b * c.table_stride + at);
   if (page < 0 || page >= c.pages) {
     kv_flag(c.status, SITE_KV_PAGE);
     return nullptr;
   }
-  const int64_t per_page = c.page_size / KV_TILE;
-  return c.base + (((int64_t)page * c.kv_heads + h) * per_page + (pos % c.page_size) / KV_TILE) * tile_bytes;
+  const int per_page = (int)c.page_tiles.d;
+  return c.base + (((int64_t)page * c.kv_heads + h) * per_page + (int)(tile - at * per_page)) * tile_bytes;
 }
 
 // ---- norm of queries and keys per head + position rotation ------------------------------------
 // y = rot(x w / sqrt(mean x^2 + eps)); rot turns the pair (a, b) of channels into
 // (a cos - b sin, b cos + a sin).  A pair is (i, i + hd/2), or (2i, 2i + 1) when interleaved.
-// One thread holds four pairs (8 channels) of one head, so that a head's pairs never leave their
-// thread and the norm is one shuffle tree over hd / 8 threads (rounded up to a power of two).
+// A thread holds eight channels (four pairs) of NR_HEADS heads of one token: a head's pairs never
+// leave their thread, the norm is one shuffle tree over hd / 8 threads (rounded up to a power of
+// two), and weights and angles are read once for the heads.  HBM bounds it: every load is issued
+// before the first use (with one head to a thread it was bound by instructions and by L1, at 51 us
+// for 4608 x 48 heads of 128).
+constexpr int NR_HEADS = 4;
 struct NormRopeArgs {
   float *qd, *kd;
   const float *q, *k;
@@ -85,8 +91,10 @@ struct NormRopeArgs {
   const int32_t* positions;
   int64_t pos0, tokens;
   int heads, kv_heads, hd;
-  float eps;
+  float eps, by_hd;  // by_hd: 1 / hd
   int interleaved, vec;
+  int q_runs;         // runs of NR_HEADS heads of q; k's follow
+  FastDiv per_token;  // by the runs of a token
   int* status;
 };
 
@@ -94,60 +102,85 @@ template <int LANES>
 __global__ void __launch_bounds__(256) k_qk_norm_rope(const NormRopeArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const int all = a.heads + a.kv_heads;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const uint32_t item = (blockIdx.x * 256u + threadIdx.x) / LANES;  // (token, run of heads)
   const int li = threadIdx.x % LANES;
-  const int64_t tok = item / all;
-  const int h = (int)(item - tok * all);
-  const bool work = tok < a.tokens && 8 * li < a.hd;
-  const bool isq = h < a.heads;
-  const bool vec = a.vec != 0;
-  float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
-  const int i0 = a.interleaved ? 8 * li : 4 * li;                 // first channels of the thread
-  const int i1 = a.interleaved ? 8 * li + 4 : a.hd / 2 + 4 * li;  // and the other four
-  if (work) {
-    const float* src = isq ? a.q + tok * a.ldq + (int64_t)h * a.hd : a.k + tok * a.ldk + (int64_t)(h - a.heads) * a.hd;
-    x0 = ld_f4(src + i0, vec);
-    x1 = ld_f4(src + i1, vec);
-  }
-  float ss = x0.x * x0.x;
-  ss = fmaf(x0.y, x0.y, ss), ss = fmaf(x0.z, x0.z, ss), ss = fmaf(x0.w, x0.w, ss);
-  ss = fmaf(x1.x, x1.x, ss), ss = fmaf(x1.y, x1.y, ss), ss = fmaf(x1.z, x1.z, ss), ss = fmaf(x1.w, x1.w, ss);
+  const uint32_t tk = a.per_token.div(item);
+  const int64_t tok = tk;
+  const int run = (int)(item - tk * a.per_token.d);
+  const bool isq = run < a.q_runs, vec = a.vec != 0;
+  const int h0 = (isq ? run : run - a.q_runs) * NR_HEADS, left = (isq ? a.heads : a.kv_heads) - h0;
+  const int n = tok < a.tokens && 8 * li < a.hd ? min(left, NR_HEADS) : 0;  // heads of this thread
+  // channels 4 li .. + 3 and hd / 2 + 4 li .. + 3: four pairs (i, i + hd / 2), or two and two pairs
+  // (2 i, 2 i + 1) when interleaved
+  const int i0 = 4 * li, i1 = a.hd / 2 + 4 * li;
+  const float* src = isq ? a.q + tok * a.ldq : a.k + tok * a.ldk;
+  float4 x0[NR_HEADS], x1[NR_HEADS];
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (!work) return;
-  const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-  const float* w = isq ? a.wq : a.wk;
-  float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0;
-  if (w) w0 = ld_f4(w + i0, vec), w1 = ld_f4(w + i1, vec);
-  x0 = make_float4(x0.x * inv * w0.x, x0.y * inv * w0.y, x0.z * inv * w0.z, x0.w * inv * w0.w);
-  x1 = make_float4(x1.x * inv * w1.x, x1.y * inv * w1.y, x1.z * inv * w1.z, x1.w * inv * w1.w);
-  if (a.cos) {
-    int64_t pos = a.positions ? (int64_t)__ldg(a.positions + tok) : a.pos0 + tok;
-    if (pos < 0 || pos >= a.table_rows) {
-      kv_flag(a.status, SITE_ROPE_POS);
-      pos = pos < 0 ? 0 : a.table_rows - 1;
-    }
-    const float4 c = ld_f4(a.cos + pos * (a.hd / 2) + 4 * li, vec);
-    const float4 s = ld_f4(a.sin + pos * (a.hd / 2) + 4 * li, vec);
-    if (a.interleaved) {
-      x0 = make_float4(x0.x * c.x - x0.y * s.x, x0.y * c.x + x0.x * s.x, x0.z * c.y - x0.w * s.y, x0.w * c.y + x0.z * s.y);
-      x1 = make_float4(x1.x * c.z - x1.y * s.z, x1.y * c.z + x1.x * s.z, x1.z * c.w - x1.w * s.w, x1.w * c.w + x1.z * s.w);
-    } else {
-      const float4 p = x0;
-      x0 = make_float4(p.x * c.x - x1.x * s.x, p.y * c.y - x1.y * s.y, p.z * c.z - x1.z * s.z, p.w * c.w - x1.w * s.w);
-      x1 = make_float4(x1.x * c.x + p.x * s.x, x1.y * c.y + p.y * s.y, x1.z * c.z + p.z * s.z, x1.w * c.w + p.w * s.w);
+  for (int j = 0; j < NR_HEADS; ++j) {
+    x0[j] = x1[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j < n) x0[j] = ld_f4(src + (int64_t)(h0 + j) * a.hd + i0, vec), x1[j] = ld_f4(src + (int64_t)(h0 + j) * a.hd + i1, vec);
+  }
+  float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0, c = w0, s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (n > 0) {
+    const float* w = isq ? a.wq : a.wk;
+    if (w) w0 = ld_f4(w + i0, vec), w1 = ld_f4(w + i1, vec);
+    if (a.cos) {
+      int64_t pos = a.positions ? (int64_t)__ldg(a.positions + tok) : a.pos0 + tok;
+      if (pos < 0 || pos >= a.table_rows) {
+        kv_flag(a.status, SITE_ROPE_POS);
+        pos = pos < 0 ? 0 : a.table_rows - 1;
+      }
+      const float *cp = a.cos + pos * (a.hd / 2), *sp = a.sin + pos * (a.hd / 2);
+      if (!a.interleaved) {
+        c = ld_f4(cp + 4 * li, vec), s = ld_f4(sp + 4 * li, vec);
+      } else {  // pairs 2 li, 2 li + 1 and hd / 4 + 2 li, + 1
+        const int f0 = 2 * li, f1 = a.hd / 4 + 2 * li;
+        c = make_float4(cp[f0], cp[f0 + 1], cp[f1], cp[f1 + 1]);
+        s = make_float4(sp[f0], sp[f0 + 1], sp[f1], sp[f1 + 1]);
+      }
     }
   }
-  float* dst = isq ? a.qd + tok * a.ldqd + (int64_t)h * a.hd : a.kd + tok * a.ldkd + (int64_t)(h - a.heads) * a.hd;
-  st_f4(dst + i0, x0, vec);
-  st_f4(dst + i1, x1, vec);
+  float ss[NR_HEADS];
+#pragma unroll
+  for (int j = 0; j < NR_HEADS; ++j) {
+    const float4 u = x0[j], v = x1[j];
+    float q = u.x * u.x;
+    q = fmaf(u.y, u.y, q), q = fmaf(u.z, u.z, q), q = fmaf(u.w, u.w, q);
+    q = fmaf(v.x, v.x, q), q = fmaf(v.y, v.y, q), q = fmaf(v.z, v.z, q), q = fmaf(v.w, v.w, q);
+    ss[j] = q;
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < NR_HEADS; ++j) ss[j] += __shfl_xor_sync(0xffffffffu, ss[j], o);
+  float* dst = isq ? a.qd + tok * a.ldqd : a.kd + tok * a.ldkd;
+#pragma unroll
+  for (int j = 0; j < NR_HEADS; ++j) {
+    if (j >= n) break;
+    const float inv = 1.0f / sqrtf(ss[j] * a.by_hd + a.eps);
+    float4 u = x0[j], v = x1[j];
+    u = make_float4(u.x * inv * w0.x, u.y * inv * w0.y, u.z * inv * w0.z, u.w * inv * w0.w);
+    v = make_float4(v.x * inv * w1.x, v.y * inv * w1.y, v.z * inv * w1.z, v.w * inv * w1.w);
+    if (a.cos) {
+      if (a.interleaved) {
+        u = make_float4(u.x * c.x - u.y * s.x, u.y * c.x + u.x * s.x, u.z * c.y - u.w * s.y, u.w * c.y + u.z * s.y);
+        v = make_float4(v.x * c.z - v.y * s.z, v.y * c.z + v.x * s.z, v.z * c.w - v.w * s.w, v.w * c.w + v.z * s.w);
+      } else {
+        const float4 p = u;
+        u = make_float4(p.x * c.x - v.x * s.x, p.y * c.y - v.y * s.y, p.z * c.z - v.z * s.z, p.w * c.w - v.w * s.w);
+        v = make_float4(v.x * c.x + p.x * s.x, v.y * c.y + p.y * s.y, v.z * c.z + p.z * s.z, v.w * c.w + p.w * s.w);
+      }
+    }
+    st_f4(dst + (int64_t)(h0 + j) * a.hd + i0, u, vec);
+    st_f4(dst + (int64_t)(h0 + j) * a.hd + i1, v, vec);
+  }
 }
 
 // ---- cache: write and read ----------------------------------------------------------------------
 // Eight threads hold one group of 64 channels, eight consecutive channels (one word of codes)
-// each; the group's minimum and maximum are one shuffle tree.  Every rounding is IEEE (no
-// contraction), so equal inputs give equal codes on any path that uses the formula.
+// each; the group's minimum and maximum are one shuffle tree.  Codes are those of the IEEE quotient
+// rounded to nearest even, so equal inputs give equal codes on any path that uses the formula; the
+// quotient itself is taken only where a product with the reciprocal comes near a half.
 ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) {
   return tok * (hd / 2) + (r >> 1) * (hd / 8) + (2 * gi + (r & 1)) * 4;
 }
@@ -165,35 +198,38 @@ ENVG_DEV float2 kv_scale(const uint8_t* tile, uint32_t at, int hd) {
 struct KvRowsArgs {
   Kv4View c;
   float *k, *v;  // [batch * q_len, ld], read by the append and written by the read
-  int64_t ldk, ldv, items;
+  int64_t ldk, ldv, rows;
   int hd, batch, q_len, vec;
+  int rows_per;            // rows of a block
+  FastDiv per_row, queue;  // by a row's threads (eight for each K or V, head and group), by q_len
 };
 
 template <bool READ>
 __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const int G = a.hd / KV_GROUP;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 8;
+  const int G = a.hd / KV_GROUP, lg = G - 1;
+  // a block takes as many whole rows as it has threads for, or a part of one (blockIdx.y)
+  const uint32_t in_block = blockIdx.y * 256u + threadIdx.x, rb = a.per_row.div(in_block);
+  const int64_t row0 = (int64_t)blockIdx.x * a.rows_per + rb;
+  const bool work = rb < (uint32_t)a.rows_per && row0 < a.rows;
+  const int64_t row = work ? row0 : 0;
+  const int unit = work ? (int)(in_block - rb * a.per_row.d) / 8 : 0;
   const int r = threadIdx.x % 8;
-  const bool work = item < a.items;
-  int64_t n = work ? item : a.items - 1;
-  const int gi = (int)(n % G);
-  n /= G;
-  const int isv = (int)(n & 1);
-  n >>= 1;
-  const int h = (int)(n % a.c.kv_heads);
-  const int64_t row = n / a.c.kv_heads;
-  const int b = (int)(row / a.q_len);
-  const int pos = kv_len(a.c, b) - a.q_len + (int)(row % a.q_len);
+  const int isv = unit >= a.c.kv_heads * G ? 1 : 0, n = unit - isv * a.c.kv_heads * G;
+  const int gi = n & lg, h = n >> lg;
+  const bool vec = a.vec != 0;
+  float* rows = isv ? a.v + row * a.ldv : a.k + row * a.ldk;
+  rows += (int64_t)h * a.hd + gi * KV_GROUP + 8 * r;
+  float4 p0, p1;
+  if (!READ) p0 = ld_f4(rows, vec), p1 = ld_f4(rows + 4, vec);  // under way while the page is looked up
+  const int b = (int)a.queue.div((uint32_t)row);
+  const int pos = kv_len(a.c, b) - a.q_len + (int)((uint32_t)row - (uint32_t)b * a.queue.d);
   const int tile_bytes = kv_tile_bytes(a.hd);
   uint8_t* tile = pos >= 0 ? kv_tile(a.c, b, h, pos, tile_bytes) : nullptr;
   const int tok = pos >= 0 ? pos % KV_TILE : 0;
   const uint32_t word_at = isv ? kv_v_byte(a.hd, tok, gi, r) : kv_k_word(a.hd, tok, gi, r);
   const uint32_t scale_at = kv_scale_at(a.hd, tok, isv, gi);
-  float* rows = isv ? a.v + row * a.ldv : a.k + row * a.ldk;
-  rows += (int64_t)h * a.hd + gi * KV_GROUP + 8 * r;
-  const bool vec = a.vec != 0;
   if (READ) {
     if (!work) return;
     float x[8] = {};
@@ -203,24 +239,25 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
       else w = *reinterpret_cast<const uint32_t*>(tile + word_at);
       const float2 sm = kv_scale(tile, scale_at, a.hd);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(sm.x, (float)((w >> (4 * j)) & 15u), sm.y);
+      for (int j = 0; j < 8; ++j) {  // a code in the low bits of 2^23
+        const float c = __uint_as_float(and_or(w >> (4 * j), 15u, 0x4B000000u)) - 8388608.0f;
+        x[j] = fmaf(sm.x, c, sm.y);
+      }
     }
     st_f4(rows, make_float4(x[0], x[1], x[2], x[3]), vec);
     st_f4(rows + 4, make_float4(x[4], x[5], x[6], x[7]), vec);
   } else {
-    const float4 p0 = ld_f4(rows, vec), p1 = ld_f4(rows + 4, vec);
     const float x[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
     float lo = x[0], hi = x[0];
     bool nan = x[0] != x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), nan |= x[j] != x[j];
-    int any = nan ? 1 : 0;
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      any |= __shfl_xor_sync(0xffffffffu, any, o);
     }
+    const uint32_t any = (__ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24)) & 0xffu;
     if (!work || !tile) return;
     if (any) lo = hi = __int_as_float(0x7fc00000);  // a group with a NaN holds NaN
     const float low = lo < -KV_HALF_MAX ? -KV_HALF_MAX : lo > KV_HALF_MAX ? KV_HALF_MAX : lo;
@@ -229,11 +266,22 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
     const float s = __half2float(hs), m = __half2float(hm);
     uint32_t w = 0;
     if (s > 0.0f) {
+      const float inv = __frcp_rn(s), whole = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
+      bool near = false;
+      uint32_t c[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = rintf(__fdiv_rn(__fsub_rn(x[j], m), s));
-        w |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * j);
+        const float q = fminf(fmaxf(__fsub_rn(x[j], m) * inv, 0.0f), 15.0f), y = __fadd_rn(q, whole);
+        c[j] = __float_as_uint(y);
+        // the product is within 15 x 2^-22 of the quotient: near a half, divide
+        near |= fabsf(__fsub_rn(q, __fsub_rn(y, whole))) > 0.5f - 1e-5f;
       }
+      if (near)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          c[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(x[j], m), s), 0.0f), 15.0f), whole));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w |= (c[j] & 15u) << (4 * j);
     }
     if (isv) {
 #pragma unroll

@@ -193,8 +193,8 @@ int launch_norm_rope(Dev* d, const NormRopeArgs& a) {
   const int all = a.heads + a.kv_heads;
   int lanes = 1;
   while (lanes * 8 < a.hd) lanes *= 2;
-  const int64_t blocks = cdiv(a.tokens * all * lanes, 256);
-  if (blocks > INT32_MAX) return fail(ENVG_ERR_ARG, "qk_norm_rope: %lld tokens are too many", (long long)a.tokens);
+  const int64_t runs = cdiv(a.heads, NR_HEADS) + cdiv(a.kv_heads, NR_HEADS), blocks = cdiv(a.tokens * runs * lanes, 256);
+  if (blocks * 256 > UINT32_MAX) return fail(ENVG_ERR_ARG, "qk_norm_rope: %lld tokens are too many", (long long)a.tokens);
   ProfScope ps(stream_of(d), KID_NORM_ROPE, 0.0, 8.0 * (double)a.tokens * all * a.hd + 4.0 * (double)a.tokens * a.hd);
   const dim3 g((unsigned)blocks), b(256);
   switch (lanes) {
@@ -245,6 +245,7 @@ Kv4View kv_view(Dev* d, envg_kv4 c, const int32_t* table, int64_t stride, const 
   v.pages = c->pages;
   v.page_size = c->page_size;
   v.kv_heads = c->kv_heads;
+  v.page_tiles = FastDiv((uint32_t)(c->page_size / KV_TILE));
   v.table = table;
   v.table_stride = stride;
   v.ctx_lens = lens;
@@ -291,15 +292,18 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   a.c = kv_view(d, c, table, stride, lens);
   a.k = dk, a.v = dv, a.ldk = lk, a.ldv = lv;
   a.hd = c->head_dim, a.batch = batch, a.q_len = q_len;
-  a.items = rows * c->kv_heads * 2 * (c->head_dim / KV_GROUP);
+  a.rows = rows;
+  const int row_threads = c->kv_heads * 2 * (c->head_dim / KV_GROUP) * 8;
+  a.rows_per = std::max(1, 256 / row_threads);
+  a.per_row = FastDiv((uint32_t)row_threads);
+  a.queue = FastDiv((uint32_t)q_len);
   a.vec = f4_ok(dk, lk) && f4_ok(dv, lv);
-  const int64_t blocks = cdiv(a.items * 8, 256);
-  if (blocks > INT32_MAX) return fail(ENVG_ERR_ARG, "%s: too many rows", what);
+  const dim3 grid((unsigned)cdiv(rows, a.rows_per), (unsigned)cdiv(row_threads, 256));
   {
     ProfScope ps(stream_of(d), read ? KID_KV4_READ : KID_KV4_APPEND, 0.0,
                  (double)rows * c->kv_heads * (8.0 * c->head_dim + c->head_dim + 8 * (c->head_dim / KV_GROUP)));
-    if (read) ENVG_TRY(launch_pdl(d, k_kv4_rows<true>, dim3((unsigned)blocks), dim3(256), 0, a));
-    else ENVG_TRY(launch_pdl(d, k_kv4_rows<false>, dim3((unsigned)blocks), dim3(256), 0, a));
+    if (read) ENVG_TRY(launch_pdl(d, k_kv4_rows<true>, grid, dim3(256), 0, a));
+    else ENVG_TRY(launch_pdl(d, k_kv4_rows<false>, grid, dim3(256), 0, a));
     d->st.kernel_launches++;
   }
   if (!devp && read) {
@@ -576,6 +580,9 @@ int envg_qk_norm_rope(const envg_qk_norm_rope_args* r, int flags) {
   a.wq = q_weight, a.wk = k_weight, a.cos = cos_table, a.sin = sin_table, a.table_rows = table_rows;
   a.positions = positions, a.pos0 = pos0, a.tokens = tokens;
   a.heads = heads, a.kv_heads = kv_heads, a.hd = head_dim, a.eps = eps, a.interleaved = interleaved ? 1 : 0;
+  a.by_hd = 1.0f / (float)head_dim;
+  a.q_runs = (int)cdiv(heads, NR_HEADS);
+  a.per_token = FastDiv((uint32_t)(a.q_runs + cdiv(kv_heads, NR_HEADS)));
   a.status = d->d_status;
   LmStage st(d);
   const bool devp = (flags & ENVG_DEVICE_PTRS) != 0;

@@ -115,6 +115,20 @@ ENVG_DEV int scale_exp(float top) {
 }
 ENVG_DEV float pow2(int e) { return __int_as_float((127 + e) << 23); }
 
+// n / d for 0 <= n < 2^32 by a multiplication (Granlund and Montgomery, PLDI 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  __host__ explicit FastDiv(uint32_t by) : d(by), mul(0), shift(0) {
+    while (shift < 32 && (1ull << shift) < by) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  ENVG_DEV uint32_t div(uint32_t n) const {
+    const uint32_t t = __umulhi(mul, n);
+    return shift ? (t + ((n - t) >> 1)) >> (shift - 1) : n;
+  }
+};
+
 // Four consecutive floats, as one access where `vec` (the address is 16-byte aligned).
 ENVG_DEV float4 ld_f4(const float* p, bool vec) {
   if (vec) return *reinterpret_cast<const float4*>(p);
