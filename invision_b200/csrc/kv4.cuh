@@ -6,13 +6,14 @@
 // group holds m = fp16(min x), s = fp16((max x - min x) / 15) and codes
 // c = clamp(rint((x - m) / s), 0, 15); it stands for the values m + s c.  The codes of 16 tokens
 // lie together in one tile, tiles of a (page, kv head) follow one another:
-//   tile = K codes [16][hd / 2 bytes] | V codes [hd / 64][32][16 bytes] | scales [16][K s.., K m.., V s.., V m..] fp16
+//   tile = K codes [16][hd / 2 bytes] | V codes [hd / 64][4][8][16 bytes] | scales [16][K s.., K m.., V s.., V m..] fp16
 // A K row's 32-bit word holds 8 consecutive channels 64 gi + 8 r + j (nibble j, r = 0..7) and stands
 // at byte (r / 2) * hd / 8 + (2 gi + r % 2) * 4, so that lane t of a quad finds the words of its
-// 16-channel pieces side by side.  V is held the way the products over tokens take it: the 16 bytes
-// of lane 4 r + t hold channels 64 gi + 8 r .. + 7 of tokens 2 t, 2 t + 8, 2 t + 1 and 2 t + 9, byte
+// 16-channel pieces side by side.  V is held the way the products over tokens take it: piece (t, r)
+// of 16 bytes holds channels 64 gi + 8 r .. + 7 of tokens 2 t, 2 t + 8, 2 t + 1 and 2 t + 9, byte
 // 4 i + b the two channels 2 i and 2 i + 1 of the b-th of these tokens.  A byte belongs to one
-// token, so that appending never reads what is there.
+// token, so that appending never reads what is there.  The piece stands at t * 128 + (r ^ 2 t) * 16:
+// a token's bytes share one line of 128, and a quarter warp's pieces (two r, four t) all banks.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -186,112 +187,123 @@ ENVG_DEV uint32_t kv_k_word(int hd, int tok, int gi, int r) {
 }
 // First of the four bytes (4 apart) of V's channels 64 gi + 8 r .. + 7 of a token.
 ENVG_DEV uint32_t kv_v_byte(int hd, int tok, int gi, int r) {
-  return KV_TILE * (hd / 2) + gi * 512 + (4 * r + ((tok & 7) >> 1)) * 16 + (tok >> 3) + 2 * (tok & 1);
+  const int t = (tok & 7) >> 1;
+  return KV_TILE * (hd / 2) + gi * 512 + t * 128 + ((r ^ (2 * t)) * 16) + (tok >> 3) + 2 * (tok & 1);
 }
 // Byte offset of the scale of (token, K or V, group); its minimum stands hd / 64 halves further.
 ENVG_DEV uint32_t kv_scale_at(int hd, int tok, int v, int gi) { return KV_TILE * hd + tok * (hd / 8) + v * (hd / 16) + 2 * gi; }
-ENVG_DEV float2 kv_scale(const uint8_t* tile, uint32_t at, int hd) {
-  const __half* p = reinterpret_cast<const __half*>(tile + at);
-  return make_float2(__half2float(p[0]), __half2float(p[hd / KV_GROUP]));
-}
 
 struct KvRowsArgs {
   Kv4View c;
   float *k, *v;  // [batch * q_len, ld], read by the append and written by the read
-  int64_t ldk, ldv, rows;
+  int64_t ldk, ldv;
   int hd, batch, q_len, vec;
-  int rows_per;            // rows of a block
-  FastDiv per_row, queue;  // by a row's threads (eight for each K or V, head and group), by q_len
+  int runs, runs_per;    // runs of ROWS new tokens in all, and of a block
+  FastDiv per_run, seq;  // by a run's threads (eight for each K or V, head and group), by a sequence's runs
 };
 
-template <bool READ>
+// A thread takes ROWS consecutive tokens, so that most find their tile where the last one's was
+// (one token to a thread spent two thirds of its instructions on finding it).
+template <bool READ, int ROWS>
 __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int G = a.hd / KV_GROUP, lg = G - 1;
-  // a block takes as many whole rows as it has threads for, or a part of one (blockIdx.y)
-  const uint32_t in_block = blockIdx.y * 256u + threadIdx.x, rb = a.per_row.div(in_block);
-  const int64_t row0 = (int64_t)blockIdx.x * a.rows_per + rb;
-  const bool work = rb < (uint32_t)a.rows_per && row0 < a.rows;
-  const int64_t row = work ? row0 : 0;
-  const int unit = work ? (int)(in_block - rb * a.per_row.d) / 8 : 0;
+  // a block takes as many whole runs as it has threads for, or a part of one (blockIdx.y)
+  const uint32_t in_block = blockIdx.y * 256u + threadIdx.x, rb = a.per_run.div(in_block);
+  const int run0 = blockIdx.x * a.runs_per + (int)rb;
+  const bool work = rb < (uint32_t)a.runs_per && run0 < a.runs;
+  const uint32_t run = work ? run0 : 0;
+  const int unit = work ? (int)(in_block - rb * a.per_run.d) / 8 : 0;
   const int r = threadIdx.x % 8;
   const int isv = unit >= a.c.kv_heads * G ? 1 : 0, n = unit - isv * a.c.kv_heads * G;
   const int gi = n & lg, h = n >> lg;
+  const int b = (int)a.seq.div(run);
+  const int i0 = (int)(run - (uint32_t)b * a.seq.d) * ROWS, rows = work ? min(ROWS, a.q_len - i0) : 0;
   const bool vec = a.vec != 0;
-  float* rows = isv ? a.v + row * a.ldv : a.k + row * a.ldk;
-  rows += (int64_t)h * a.hd + gi * KV_GROUP + 8 * r;
-  float4 p0, p1;
-  if (!READ) p0 = ld_f4(rows, vec), p1 = ld_f4(rows + 4, vec);  // under way while the page is looked up
-  const int b = (int)a.queue.div((uint32_t)row);
-  const int pos = kv_len(a.c, b) - a.q_len + (int)((uint32_t)row - (uint32_t)b * a.queue.d);
+  const int64_t ld = isv ? a.ldv : a.ldk;
+  float* at = (isv ? a.v : a.k) + ((int64_t)b * a.q_len + i0) * ld + (int64_t)h * a.hd + gi * KV_GROUP + 8 * r;
+  float4 p0[ROWS], p1[ROWS];
+  if (!READ) {  // under way while the page is looked up
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      p0[i] = p1[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < rows) p0[i] = ld_f4(at + i * ld, vec), p1[i] = ld_f4(at + i * ld + 4, vec);
+    }
+  }
+  const int pos0 = kv_len(a.c, b) - a.q_len + i0;
   const int tile_bytes = kv_tile_bytes(a.hd);
-  uint8_t* tile = pos >= 0 ? kv_tile(a.c, b, h, pos, tile_bytes) : nullptr;
-  const int tok = pos >= 0 ? pos % KV_TILE : 0;
-  const uint32_t word_at = isv ? kv_v_byte(a.hd, tok, gi, r) : kv_k_word(a.hd, tok, gi, r);
-  const uint32_t scale_at = kv_scale_at(a.hd, tok, isv, gi);
-  if (READ) {
-    if (!work) return;
-    float x[8] = {};
-    if (tile) {
-      uint32_t w;
-      if (isv) w = tile[word_at] | tile[word_at + 4] << 8 | tile[word_at + 8] << 16 | (uint32_t)tile[word_at + 12] << 24;
-      else w = *reinterpret_cast<const uint32_t*>(tile + word_at);
-      const float2 sm = kv_scale(tile, scale_at, a.hd);
+  uint8_t* tile = nullptr;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {  // a code in the low bits of 2^23
-        const float c = __uint_as_float(and_or(w >> (4 * j), 15u, 0x4B000000u)) - 8388608.0f;
-        x[j] = fmaf(sm.x, c, sm.y);
+  for (int i = 0; i < ROWS; ++i) {
+    const int pos = pos0 + i, tok = pos & (KV_TILE - 1);
+    const bool on = i < rows && pos >= 0;
+    if (on && (i == 0 || tok == 0 || pos == 0)) tile = kv_tile(a.c, b, h, pos, tile_bytes);
+    uint8_t* codes = tile + (isv ? kv_v_byte(a.hd, tok, gi, r) : kv_k_word(a.hd, tok, gi, r));
+    uint8_t* scale = tile + kv_scale_at(a.hd, tok, isv, gi);
+    if (READ) {
+      if (i >= rows) return;
+      float x[8] = {};
+      if (on && tile) {
+        uint32_t w;
+        if (isv) w = codes[0] | codes[4] << 8 | codes[8] << 16 | (uint32_t)codes[12] << 24;
+        else w = *reinterpret_cast<const uint32_t*>(codes);
+        const __half* sp = reinterpret_cast<const __half*>(scale);
+        const float s = __half2float(sp[0]), m = __half2float(sp[G]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)  // a code in the low bits of 2^23
+          x[j] = fmaf(s, __uint_as_float(and_or(w >> (4 * j), 15u, 0x4B000000u)) - 8388608.0f, m);
       }
-    }
-    st_f4(rows, make_float4(x[0], x[1], x[2], x[3]), vec);
-    st_f4(rows + 4, make_float4(x[4], x[5], x[6], x[7]), vec);
-  } else {
-    const float x[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-    float lo = x[0], hi = x[0];
-    bool nan = x[0] != x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), nan |= x[j] != x[j];
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const uint32_t any = (__ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24)) & 0xffu;
-    if (!work || !tile) return;
-    if (any) lo = hi = __int_as_float(0x7fc00000);  // a group with a NaN holds NaN
-    const float low = lo < -KV_HALF_MAX ? -KV_HALF_MAX : lo > KV_HALF_MAX ? KV_HALF_MAX : lo;
-    const float step = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    const __half hs = __float2half_rn(step > KV_HALF_MAX ? KV_HALF_MAX : step), hm = __float2half_rn(low);
-    const float s = __half2float(hs), m = __half2float(hm);
-    uint32_t w = 0;
-    if (s > 0.0f) {
-      const float inv = __frcp_rn(s), whole = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
-      bool near = false;
-      uint32_t c[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = fminf(fmaxf(__fsub_rn(x[j], m) * inv, 0.0f), 15.0f), y = __fadd_rn(q, whole);
-        c[j] = __float_as_uint(y);
-        // the product is within 15 x 2^-22 of the quotient: near a half, divide
-        near |= fabsf(__fsub_rn(q, __fsub_rn(y, whole))) > 0.5f - 1e-5f;
-      }
-      if (near)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          c[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(x[j], m), s), 0.0f), 15.0f), whole));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w |= (c[j] & 15u) << (4 * j);
-    }
-    if (isv) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tile[word_at + 4 * i] = (uint8_t)(w >> (8 * i));
+      st_f4(at + i * ld, make_float4(x[0], x[1], x[2], x[3]), vec);
+      st_f4(at + i * ld + 4, make_float4(x[4], x[5], x[6], x[7]), vec);
     } else {
-      *reinterpret_cast<uint32_t*>(tile + word_at) = w;
-    }
-    if (r == 0) {
-      __half* p = reinterpret_cast<__half*>(tile + scale_at);
-      p[0] = hs, p[G] = hm;
+      const float x[8] = {p0[i].x, p0[i].y, p0[i].z, p0[i].w, p1[i].x, p1[i].y, p1[i].z, p1[i].w};
+      float lo = x[0], hi = x[0];
+      bool nan = x[0] != x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), nan |= x[j] != x[j];
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const uint32_t any = (__ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24)) & 0xffu;
+      if (on && tile) {
+        if (any) lo = hi = __int_as_float(0x7fc00000);  // a group with a NaN holds NaN
+        const float low = lo < -KV_HALF_MAX ? -KV_HALF_MAX : lo > KV_HALF_MAX ? KV_HALF_MAX : lo;
+        const float step = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+        const __half hs = __float2half_rn(step > KV_HALF_MAX ? KV_HALF_MAX : step), hm = __float2half_rn(low);
+        const float s = __half2float(hs), m = __half2float(hm);
+        uint32_t w = 0;
+        if (s > 0.0f) {
+          const float inv = __frcp_rn(s), whole = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
+          bool near = false;
+          uint32_t c[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float q = fminf(fmaxf(__fsub_rn(x[j], m) * inv, 0.0f), 15.0f), y = __fadd_rn(q, whole);
+            c[j] = __float_as_uint(y);
+            // the product is within 15 x 2^-22 of the quotient: near a half, divide
+            near |= fabsf(__fsub_rn(q, __fsub_rn(y, whole))) > 0.5f - 1e-5f;
+          }
+          if (near)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              c[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(x[j], m), s), 0.0f), 15.0f), whole));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w |= (c[j] & 15u) << (4 * j);
+        }
+        if (isv) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) codes[4 * j] = (uint8_t)(w >> (8 * j));
+        } else {
+          *reinterpret_cast<uint32_t*>(codes) = w;
+        }
+        if (r == 0) {
+          __half* sp = reinterpret_cast<__half*>(scale);
+          sp[0] = hs, sp[G] = hm;
+        }
+      }
     }
   }
 }
@@ -640,7 +652,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
       uint32_t vw[2][4];
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        const uint4 u = *reinterpret_cast<const uint4*>(stage + tt * S::TILE + KV_TILE * (HD / 2) + gi * 512 + lane * 16);
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + tt * S::TILE + KV_TILE * (HD / 2) + gi * 512 + t * 128 + ((g ^ (2 * t)) << 4));
         vw[tt][0] = u.x, vw[tt][1] = u.y, vw[tt][2] = u.z, vw[tt][3] = u.w;
       }
       int minus[NB][2][4];  // -8 times the sums of the weights' digits

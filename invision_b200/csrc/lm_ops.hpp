@@ -292,18 +292,21 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   a.c = kv_view(d, c, table, stride, lens);
   a.k = dk, a.v = dv, a.ldk = lk, a.ldv = lv;
   a.hd = c->head_dim, a.batch = batch, a.q_len = q_len;
-  a.rows = rows;
-  const int row_threads = c->kv_heads * 2 * (c->head_dim / KV_GROUP) * 8;
-  a.rows_per = std::max(1, 256 / row_threads);
-  a.per_row = FastDiv((uint32_t)row_threads);
-  a.queue = FastDiv((uint32_t)q_len);
+  // four tokens to a thread once they fill the GPU's threads all the same
+  const int run_threads = c->kv_heads * 2 * (c->head_dim / KV_GROUP) * 8;
+  const bool four = q_len >= 4 && rows * run_threads >= (int64_t)d->sms * 2048 * 4;
+  const int runs_seq = (int)cdiv(q_len, four ? 4 : 1);
+  a.runs = batch * runs_seq;
+  a.runs_per = std::max(1, 256 / run_threads);
+  a.per_run = FastDiv((uint32_t)run_threads);
+  a.seq = FastDiv((uint32_t)runs_seq);
   a.vec = f4_ok(dk, lk) && f4_ok(dv, lv);
-  const dim3 grid((unsigned)cdiv(rows, a.rows_per), (unsigned)cdiv(row_threads, 256));
+  const dim3 grid((unsigned)cdiv(a.runs, a.runs_per), (unsigned)cdiv(run_threads, 256));
   {
     ProfScope ps(stream_of(d), read ? KID_KV4_READ : KID_KV4_APPEND, 0.0,
                  (double)rows * c->kv_heads * (8.0 * c->head_dim + c->head_dim + 8 * (c->head_dim / KV_GROUP)));
-    if (read) ENVG_TRY(launch_pdl(d, k_kv4_rows<true>, grid, dim3(256), 0, a));
-    else ENVG_TRY(launch_pdl(d, k_kv4_rows<false>, grid, dim3(256), 0, a));
+    ENVG_TRY(read ? (four ? launch_pdl(d, k_kv4_rows<true, 4>, grid, dim3(256), 0, a) : launch_pdl(d, k_kv4_rows<true, 1>, grid, dim3(256), 0, a))
+                  : (four ? launch_pdl(d, k_kv4_rows<false, 4>, grid, dim3(256), 0, a) : launch_pdl(d, k_kv4_rows<false, 1>, grid, dim3(256), 0, a)));
     d->st.kernel_launches++;
   }
   if (!devp && read) {
