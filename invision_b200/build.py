@@ -19,6 +19,32 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std
          "-Xcompiler", "-fPIC,-O3", "-shared"]
 
 
+# The torch side of the Python binding (operand checks in one step); the library itself needs no torch.
+VIEWS_SRC = os.path.join(HERE, "csrc", "views.cpp")
+VIEWS = os.path.join(HERE, "lib", "_views.so")
+
+
+def build_views(force=False, verbose=True):
+    """Builds lib/_views.so against the torch of this interpreter (returns None where there is none)."""
+    if not force and os.path.exists(VIEWS) and os.path.getmtime(VIEWS) > os.path.getmtime(VIEWS_SRC):
+        return VIEWS
+    try:
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError:
+        return None
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"]] + ["-I" + p for p in include_paths()]
+    cmd += [VIEWS_SRC, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", VIEWS]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return VIEWS
+
+
 def needs_build():
     if not os.path.exists(OUT):
         return True
@@ -27,9 +53,10 @@ def needs_build():
 
 
 def build(force=False, verbose=True):
+    os.makedirs(os.path.dirname(OUT), exist_ok=True)
+    build_views(force, verbose)
     if not force and not needs_build():
         return OUT
-    os.makedirs(os.path.dirname(OUT), exist_ok=True)
     cmd = [NVCC] + FLAGS + SRC + ["-o", OUT]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -343,7 +343,7 @@ struct KvAttnArgs {
 // of CTAs (one cluster per sequence, kv head and 4 NB rows).  Each warp runs a one-pass softmax
 // with its own ring of bulk copies; the warps' (max, sum, output) are joined in shared memory, the
 // CTAs' through distributed shared memory in rank order: no workspace, no atomics, one launch.
-constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 3;
+constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 2;
 constexpr int SITE_KVA_RING = 60;  // status[1] of a ring wait that ran out
 
 template <int HD, int NB>
@@ -360,7 +360,7 @@ struct KvaSmem {
 };
 
 template <int HD, int NB>
-__global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 128 ? 2 : 3) k_kv4_attn(const KvAttnArgs a) {
+__global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const KvAttnArgs a) {
   using S = KvaSmem<HD, NB>;
   constexpr int G = HD / KV_GROUP;  // groups per head
   constexpr int ROWS = S::ROWS;
@@ -381,6 +381,21 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   const int splits = gridDim.x, rank = blockIdx.x, b = blockIdx.z;
   const int per_kv = a.heads / a.c.kv_heads, rows = per_kv * a.q_len;
   const int kvh = blockIdx.y % a.c.kv_heads, row0 = (blockIdx.y / a.c.kv_heads) * ROWS;
+  // q first: its loads are under way while the lengths and the page table are looked up
+  float x[NB][16 * G];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int rr = row0 + 4 * nb + (g >> 1);
+    const bool have = rr < rows;
+    const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
+    const float* src = a.q + ((int64_t)b * a.q_len + qi) * a.ldq + (int64_t)qh * HD + 16 * t;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (have) v = ld_f4(src + 64 * (i / 4) + 4 * (i % 4), a.vec != 0);
+      x[nb][4 * i] = v.x, x[nb][4 * i + 1] = v.y, x[nb][4 * i + 2] = v.z, x[nb][4 * i + 3] = v.w;
+    }
+  }
   const int len = kv_len(a.c, b);
   // tiles that some row of the CTA sees: the first n_sink ones, then [first, last]
   const int p_lo = len - a.q_len + row0 / per_kv, p_hi = len - a.q_len + min(rows - 1, row0 + ROWS - 1) / per_kv;
@@ -437,20 +452,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
   int pos[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int rr = row0 + 4 * nb + (g >> 1);
-    const bool have = rr < rows;
-    const int qi = have ? rr / per_kv : 0, qh = kvh * per_kv + (have ? rr - qi * per_kv : 0);
-    const float* src = a.q + ((int64_t)b * a.q_len + qi) * a.ldq + (int64_t)qh * HD + 16 * t;
-    float x[16 * G];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (have) v = ld_f4(src + 64 * (i / 4) + 4 * (i % 4), a.vec != 0);
-      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[4 * i + j]) & 0x7fffffffu);
-    }
+    for (int j = 0; j < 16 * G; ++j) top = max(top, __float_as_uint(x[nb][j]) & 0x7fffffffu);
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int e = fixed_exp(__uint_as_float(top));
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     for (int gi = 0; gi < G; ++gi) {
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += x[16 * gi + j];
+      for (int j = 0; j < 16; ++j) sum += x[nb][16 * gi + j];
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : NB == 4 && HD == 12
     for (int w = 0; w < 2 * G; ++w) {
       uint32_t d[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = digits256(__float2int_rn(x[8 * w + j] * up));
+      for (int j = 0; j < 8; ++j) d[j] = digits256(__float2int_rn(x[nb][8 * w + j] * up));
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll

@@ -316,11 +316,20 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   return finish_call(d, flags);
 }
 
-// CTAs that share one (sequence, kv head, row tile): enough for two waves of three CTAs per SM,
-// as long as each warp keeps a unit of two tiles.  A power of two up to 8 (the portable cluster).
+// CTAs that share one (sequence, kv head, row tile), a power of two up to 8 (the portable cluster).
+// A CTA costs about as much as eight units of two tiles a warp, so a GPU that is full takes more
+// CTAs only while they keep that (measured, us: 16 sequences of 8192 to 16384 tokens, 128 groups:
+// 122 / 75 / 65 / 59 at 1 / 2 / 4 / 8; 32 windows of 1024, 256 groups: 16.4 / 18 / 24 / 37); one that
+// is not takes them down to one unit a warp (512 tokens, 8 groups: 6.9 / 6.4 / 5.6 / 5.9).
 int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
+  const int64_t units = cdiv(tokens, 2 * KV_TILE);
   int s = 1;
-  while (s < 8 && groups * s * 2 <= (int64_t)d->sms * 6 && cdiv(tokens, 2 * KV_TILE) >= (int64_t)s * 2 * KVA_WARPS) s *= 2;
+  while (s < 8) {
+    const int64_t each = units / (2 * s * KVA_WARPS);  // units a warp keeps
+    const bool more = groups * s < d->sms ? each >= 1 : groups * s * 2 <= (int64_t)d->sms * 8 && each >= 8;
+    if (!more) break;
+    s *= 2;
+  }
   return s;
 }
 
@@ -363,13 +372,12 @@ int launch_kv4_attn(Dev* d, const KvAttnArgs& a, int max_ctx) {
   const double seen = a.window > 0 ? std::min<double>(max_ctx, (double)a.window + a.sinks + a.q_len) : max_ctx;
   ProfScope ps(stream_of(d), KID_KV4_ATTN, 4.0 * a.hd * a.heads * (double)rows * seen,
                seen * a.batch * a.c.kv_heads * (a.hd + 8 * (a.hd / KV_GROUP)) + 8.0 * (double)rows * a.heads * a.hd);
-  // rows that read one kv head: 4, 8 or 16 at a time
+  // rows that read one kv head: 4 or 8 at a time (16 took 255 registers and was no faster)
   const int64_t shared = (int64_t)(a.heads / a.c.kv_heads) * a.q_len;
-  const int nb = shared <= 4 ? 1 : shared <= 8 ? 2 : 4;
-  const int splits = kv4_splits(d, cdiv(shared, 4 * nb) * a.c.kv_heads * a.batch, (int64_t)seen);
-  if (a.hd == 128)
-    return nb == 1 ? launch_kv4_attn_t<128, 1>(d, a, splits) : nb == 2 ? launch_kv4_attn_t<128, 2>(d, a, splits) : launch_kv4_attn_t<128, 4>(d, a, splits);
-  return nb == 1 ? launch_kv4_attn_t<64, 1>(d, a, splits) : nb == 2 ? launch_kv4_attn_t<64, 2>(d, a, splits) : launch_kv4_attn_t<64, 4>(d, a, splits);
+  const bool four = shared <= 4;
+  const int splits = kv4_splits(d, cdiv(shared, four ? 4 : 8) * a.c.kv_heads * a.batch, (int64_t)seen);
+  if (a.hd == 128) return four ? launch_kv4_attn_t<128, 1>(d, a, splits) : launch_kv4_attn_t<128, 2>(d, a, splits);
+  return four ? launch_kv4_attn_t<64, 1>(d, a, splits) : launch_kv4_attn_t<64, 2>(d, a, splits);
 }
 
 }  // namespace

@@ -575,7 +575,9 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
 # ---------------------------------------------------------------------------------------------
 
 _torch = None  # the torch module, once a tensor has been passed
+_views = None  # lib/_views.so: a CUDA tensor's checks in one step
 _TORCH_DTYPES = {}
+_CODES = {"float32": 0, "int32": 1, "uint8": 2}
 _NP_DTYPES = {"float32": np.dtype(np.float32), "int32": np.dtype(np.int32), "uint8": np.dtype(np.uint8)}
 # the argument structures of the C ABI (native alignment)
 _LINEAR_Q4 = struct.Struct("PqPqPPPqqqi")
@@ -595,11 +597,28 @@ def _side(a):
 
         _TORCH_DTYPES.update(float32=torch.float32, int32=torch.int32, uint8=torch.uint8)
         _torch = torch
+        _load_views()
     if not (isinstance(a, _torch.Tensor) and a.is_cuda):
         raise TypeError("operands must be numpy arrays (host) or CUDA tensors (device)")
     if _follow_torch_stream:
         lib().envg_set_stream(_raw_stream(a.get_device()) or CUDA_STREAM_LEGACY)
     return DEVICE_PTRS
+
+
+def _load_views():
+    global _views
+    path = os.path.join(HERE, "lib", "_views.so")
+    if os.path.exists(path):
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_loader
+
+        try:
+            spec = spec_from_loader("_views", ExtensionFileLoader("_views", path))
+            found = module_from_spec(spec)
+            spec.loader.exec_module(found)
+            _views = found
+        except ImportError:  # built for another torch: the checks are made attribute by attribute
+            pass
 
 
 def _raw_stream(device):
@@ -619,10 +638,10 @@ def _matrix(a, rows, cols, name, mode, dtype="float32"):
     """(pointer, row stride in elements) of a 2-D array [rows, >= cols] whose columns are adjacent."""
     if a is None:
         return 0, 0
-    if mode == DEVICE_PTRS and type(a) is _torch.Tensor and a.dim() == 2:  # the usual case, checked at once
-        (r, c), (s0, s1) = a.shape, a.stride()
-        if a.is_cuda and a.dtype is _TORCH_DTYPES[dtype] and r == rows and c >= cols and s1 == 1 and s0 >= c:
-            return a.data_ptr(), s0
+    if mode == DEVICE_PTRS and _views is not None:
+        got = _views.matrix(a, rows, cols, _CODES[dtype])
+        if got is not None:
+            return got
     host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
         raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")
@@ -644,6 +663,10 @@ def _matrix(a, rows, cols, name, mode, dtype="float32"):
 def _vector(a, n, name, mode, dtype="float32"):
     if a is None:
         return 0
+    if mode == DEVICE_PTRS and _views is not None:
+        got = _views.vector(a, n, _CODES[dtype])
+        if got is not None:
+            return got
     host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
         raise TypeError(f"{name}: expected {dtype}, got {a.dtype}")

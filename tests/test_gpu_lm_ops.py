@@ -515,3 +515,42 @@ def test_attention_kv4_beyond_4_gib_strides_streams_repeats(gpu):
         ref, tol = R.attention(q[b, 3 : 3 + H * hd].reshape(1, H, hd), kk, vv, [lens[b] - 1], 0, 0, hd ** -0.5)
         y = got[0][b, 1 : 1 + H * hd].reshape(1, H, hd)
         assert (np.abs(y - ref) <= tol).all() and R.rel(y, ref) <= 4 * REL
+
+
+# ---- all of them together ------------------------------------------------------------------------
+
+def test_decode_example_matches_plain_layers(gpu):
+    """examples/decode_q4.py at a small size: each layer within fp32 rounding of its plain form.  A key
+    whose rounding falls the other way in the two forms cannot occur: both read the cache's values."""
+    import importlib.util
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("decode_q4", os.path.join(root, "examples", "decode_q4.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    worst, _ = ex.run(layers=2, batch=3, steps=3, hidden=256, heads=6, kv_heads=2, head_dim=64, mlp=384, page=16, prompt=20)
+    assert worst <= 2e-5, worst
+
+
+def test_random_shapes_against_formulas(gpu):
+    """A sweep of drawn sizes over all four operators, odd ones among them."""
+    rng = np.random.default_rng(77)
+    for _ in range(12):
+        group = int(rng.choice([32, 64, 128]))
+        M, K, half = int(rng.integers(1, 70)), int(rng.integers(1, 3000)), int(rng.integers(1, 300))
+        codes, scales, z = _q4(2 * half, K, group, bool(rng.integers(2)), int(rng.integers(1 << 30)))
+        x = rng.standard_normal((M, K)).astype(np.float32)
+        gu = bool(rng.integers(2))
+        W = gpu.Q4Weight(codes, scales, z, K=K, group=group, layout=gpu.LAYOUT_GATE_UP if gu else gpu.LAYOUT_PLAIN)
+        y = np.full((M, half if gu else 2 * half), np.nan, np.float32)
+        gpu.linear_q4(y, x, W)
+        ref, tol = R.linear(x, R.q4_weight(codes, scales, z, K, group), gate_up=gu, groups=-(-K // group))
+        assert np.isfinite(y).all() and (np.abs(y - ref) - tol).max() <= 0 and R.rel(y, ref) <= 2 * REL, (M, K, half, group, gu)
+    for _ in range(12):
+        hd, KVH, per = int(rng.choice([64, 128])), int(rng.integers(1, 5)), int(rng.integers(1, 10))
+        B, q_len, page = int(rng.integers(1, 5)), int(rng.integers(1, 12)), int(rng.choice([16, 48, 80]))
+        lens = [int(v) for v in rng.integers(0, 400, B)]
+        window = int(rng.choice([0, 1, 20, 130]))
+        c, table, ks, vs = _held(gpu, rng, lens, page, KVH, hd)
+        _check_attention(gpu, rng, c, table, ks, vs, lens, q_len, KVH * per, hd, window, int(rng.integers(0, 40)) if window else 0)
