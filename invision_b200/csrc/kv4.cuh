@@ -319,7 +319,8 @@ struct KvAttnArgs {
   int64_t ldq, ldo;
   int batch, q_len, heads, hd, window, sinks;
   float sl2;  // softmax scale * log2 e
-  int vec, vec_out;  // rows of q, of out are 16-byte aligned
+  int vec, vec_out;        // rows of q, of out are 16-byte aligned
+  int splits, log_splits;  // CTAs of a cluster, a power of two: parts of the tokens
   uint64_t wait_cap_ns;
 };
 
@@ -378,9 +379,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
   griddep_launch_dependents();
   __syncthreads();
 
-  const int splits = gridDim.x, rank = blockIdx.x, b = blockIdx.z;
+  const int splits = a.splits, rank = blockIdx.x & (splits - 1), row_tile = blockIdx.x >> a.log_splits, b = blockIdx.y;
   const int per_kv = a.heads / a.c.kv_heads, rows = per_kv * a.q_len;
-  const int kvh = blockIdx.y % a.c.kv_heads, row0 = (blockIdx.y / a.c.kv_heads) * ROWS;
+  const int kvh = row_tile % a.c.kv_heads, row0 = (row_tile / a.c.kv_heads) * ROWS;
   // q first: its loads are under way while the lengths and the page table are looked up
   float x[NB][16 * G];
 #pragma unroll

@@ -116,7 +116,7 @@ int q4_clusters(const Dev* d, int s) {
 }
 
 template <int NT, bool HALF>
-bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
+bool q4_plan(const Dev* d, const Q4View& w, int M, Q4Plan* best) {
   using S = Q4Smem<NT, HALF>;
   double least = 0.0;
   bool found = false;
@@ -126,8 +126,12 @@ bool q4_plan(const Dev* d, const Q4View& w, Q4Plan* best) {
     int stages = room / (Q4_WARPS * q4_block_bytes(w.group));
     stages = stages >= 6 ? 6 : stages >= 4 ? 4 : stages;
     if (stages < 3 || kb * (s - 1) >= w.kblocks) continue;  // (every CTA has work)
-    const int clusters = (int)std::min<int64_t>(w.tiles, q4_clusters(d, s));
-    const double cost = (double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + (s > 1 ? 4.0 : 0.0);
+    // the launch rows of more than MC rows of x share the GPU: one wave of CTAs with more tiles each
+    // rather than several waves (a CTA's start costs as much as about 64 blocks)
+    const int held = q4_clusters(d, s), chunks = (int)cdiv(M, S::MC);
+    const int clusters = (int)std::min<int64_t>(w.tiles, std::max(1, held / chunks));
+    const double waves = (double)cdiv((int64_t)clusters * chunks, held);
+    const double cost = waves * ((double)cdiv(w.tiles, clusters) * kb / Q4_WARPS + 4.0 + (s > 1 ? 4.0 : 0.0));
     if (found && cost >= least) continue;
     least = cost, found = true;
     best->splits = s, best->log_splits = s == 1 ? 0 : s == 2 ? 1 : s == 4 ? 2 : 3, best->clusters = clusters, best->kb_per = kb, best->stages = stages;
@@ -182,10 +186,10 @@ int launch_q4(Dev* d, const Q4Args& a) {
   Q4Plan p{};
   p.vec = f4_ok(a.x, a.ldx);
   // 16, 8, 4 or 2 rows at a time: as many as there are, fewer where K leaves no room for their parts
-  if (a.M > 8 && q4_plan<4, true>(d, a.w, &p)) return launch_q4_n<4, true>(d, a, p);
-  if (a.M > 4 && q4_plan<2, true>(d, a.w, &p)) return launch_q4_n<2, true>(d, a, p);
-  if (a.M > 2 && q4_plan<2, false>(d, a.w, &p)) return launch_q4_n<2, false>(d, a, p);
-  if (q4_plan<1, false>(d, a.w, &p)) return launch_q4_n<1, false>(d, a, p);
+  if (a.M > 8 && q4_plan<4, true>(d, a.w, a.M, &p)) return launch_q4_n<4, true>(d, a, p);
+  if (a.M > 4 && q4_plan<2, true>(d, a.w, a.M, &p)) return launch_q4_n<2, true>(d, a, p);
+  if (a.M > 2 && q4_plan<2, false>(d, a.w, a.M, &p)) return launch_q4_n<2, false>(d, a, p);
+  if (q4_plan<1, false>(d, a.w, a.M, &p)) return launch_q4_n<1, false>(d, a, p);
   return fail(ENVG_ERR_UNSUPPORTED, "linear_q4: K=%lld is too long", (long long)a.w.K);
 }
 
@@ -334,7 +338,7 @@ int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
 }
 
 template <int HD, int NB>
-int launch_kv4_attn_t(Dev* d, const KvAttnArgs& a, int splits) {
+int launch_kv4_attn_t(Dev* d, KvAttnArgs a, int splits) {
   using S = KvaSmem<HD, NB>;
   static bool attr_set[64] = {};
   if (!attr_set[d->id]) {
@@ -342,9 +346,11 @@ int launch_kv4_attn_t(Dev* d, const KvAttnArgs& a, int splits) {
     attr_set[d->id] = true;
   }
   const int64_t tiles = cdiv((int64_t)(a.heads / a.c.kv_heads) * a.q_len, S::ROWS) * a.c.kv_heads;
-  if (tiles > 65535 || a.batch > 65535) return fail(ENVG_ERR_UNSUPPORTED, "attention_kv4: batch %d x %lld row tiles is too large", a.batch, (long long)tiles);
+  if (tiles * splits > INT32_MAX || a.batch > 65535)
+    return fail(ENVG_ERR_UNSUPPORTED, "attention_kv4: %d sequences of %lld row tiles are too many", a.batch, (long long)tiles);
+  a.splits = splits, a.log_splits = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)splits, (unsigned)tiles, (unsigned)a.batch);
+  cfg.gridDim = dim3((unsigned)(splits * tiles), (unsigned)a.batch);
   cfg.blockDim = dim3(KVA_THREADS);
   cfg.dynamicSmemBytes = S::TOTAL;
   cfg.stream = stream_of(d);
@@ -724,11 +730,12 @@ int envg_attention_kv4(const envg_attention_kv4_args* r, int flags) {
   }
   a.c = kv_view(d, cache, table, table_stride, ctx_lens);
   a.batch = batch, a.q_len = q_len, a.heads = heads, a.hd = cache->head_dim;
-  a.window = window, a.sinks = sinks;
   a.sl2 = scale * 1.4426950408889634f;
   a.wait_cap_ns = d->wait_cap_ns;
   a.vec = f4_ok(a.q, a.ldq), a.vec_out = f4_ok(a.out, a.ldo);
   const int64_t most = table_stride * cache->page_size;
+  a.window = window < most ? window : 0;  // a window over all that a table row names hides nothing
+  a.sinks = (int)std::min<int64_t>(sinks, most);
   ENVG_TRY(launch_kv4_attn(d, a, (int)(max_ctx > 0 ? std::min<int64_t>(max_ctx, most) : most)));
   if (!devp) ENVG_TRY(st.out(io, dst, ldo, rows, width));
   return finish_call(d, flags);
