@@ -122,8 +122,10 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
 //     of two per (row, block), four rows to a product.
 // The integer form unpacks a block in 24 operations against 72, the other form spends 4 per group on
 // four rows against 18; the kernel is bound by instruction issue before it is by HBM, so few rows
-// take integers and many rows halves.  Measured, us: 1 x 2560 x 19456, groups of 64: 8.3 / 10.7;
-// 4 x 4096 x 36864, groups of 128: 20.3 / 22.2; 16 x 9728 x 2560, groups of 32: 20.0 / 16.2.
+// take integers and many rows halves.  Measured, us (integers / halves): 1 x 2560 x 19456, groups of
+// 64: 7.9 / 13.2; 4 x 4096 x 36864, groups of 128: 20.1 / 28.2 (4.0 TB/s; one row: 17.4, 4.6 TB/s,
+// and 6.5 TB/s for every block past the first wave); 4 x 9728 x 2560, groups of 32: 9.6 / 10.2;
+// 16 x 9728 x 2560, groups of 32: 20.0 / 14.1.
 //
 // Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
 // of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
