@@ -37,8 +37,9 @@ def build_views(force=False, verbose=True):
         return None
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I" + sysconfig.get_paths()["include"]] + ["-I" + p for p in include_paths()]
-    cmd += [VIEWS_SRC, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", VIEWS]
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    cmd += ["-I" + p for p in include_paths()]
+    cmd += [VIEWS_SRC, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-o", VIEWS]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)

@@ -575,15 +575,21 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
 # ---------------------------------------------------------------------------------------------
 
 _torch = None  # the torch module, once a tensor has been passed
-_views = None  # lib/_views.so: a CUDA tensor's checks in one step
+_views = None   # lib/_views.so: a CUDA tensor's checks, or a whole call, in one step
+_Tensor = None  # torch.Tensor, where _views is there
+_ADDRESSES = {}
 _TORCH_DTYPES = {}
 _CODES = {"float32": 0, "int32": 1, "uint8": 2}
 _NP_DTYPES = {"float32": np.dtype(np.float32), "int32": np.dtype(np.int32), "uint8": np.dtype(np.uint8)}
-# the argument structures of the C ABI (native alignment)
-_LINEAR_Q4 = struct.Struct("PqPqPPPqqqi")
-_QK_NORM_ROPE = struct.Struct("PqPqPqPqPPPPqPqqiiifi")
-_KV4_ROWS = struct.Struct("PPqPqPqPii")
-_ATTENTION_KV4 = struct.Struct("PqPqPPqPiiiiiif")
+# the argument structures of the C ABI (native alignment), as _views.call spells them: M, E a matrix and
+# its row stride; V, I, P, J a pointer to a vector or a contiguous matrix
+_LINEAR_Q4_SPEC = "MEpVVqqqi"
+_QK_NORM_ROPE_SPEC = "MMMMVVPPqIqqiiifi"
+_KV4_ROWS_SPEC = "pMMJqIii"
+_ATTENTION_KV4_SPEC = "MMpJqIiiiiiif"
+_LINEAR_Q4, _QK_NORM_ROPE, _KV4_ROWS, _ATTENTION_KV4 = (
+    struct.Struct(spec.translate(str.maketrans({"M": "Pq", "E": "Pq", "V": "P", "I": "P", "J": "P", "p": "P"})))
+    for spec in (_LINEAR_Q4_SPEC, _QK_NORM_ROPE_SPEC, _KV4_ROWS_SPEC, _ATTENTION_KV4_SPEC))
 
 
 def _side(a):
@@ -606,7 +612,7 @@ def _side(a):
 
 
 def _load_views():
-    global _views
+    global _views, _Tensor
     path = os.path.join(HERE, "lib", "_views.so")
     if os.path.exists(path):
         from importlib.machinery import ExtensionFileLoader
@@ -616,9 +622,27 @@ def _load_views():
             spec = spec_from_loader("_views", ExtensionFileLoader("_views", path))
             found = module_from_spec(spec)
             spec.loader.exec_module(found)
-            _views = found
+            _views, _Tensor = found, _torch.Tensor
         except ImportError:  # built for another torch: the checks are made attribute by attribute
             pass
+
+
+def _call(name, sync, spec, *operands):
+    """envg_`name` on CUDA tensors by _views.call, its status checked: False, and no call, where an
+    operand is not what `spec` says (the caller then finds out what is wrong)."""
+    if lib() is not _ADDRESSES.get(None):
+        _ADDRESSES.clear()
+        _ADDRESSES[None] = lib()
+    fn = _ADDRESSES.get(name)
+    if fn is None:
+        for k in (name, "envg_set_stream"):
+            _ADDRESSES[k] = ctypes.cast(getattr(lib(), k), _vp).value
+        fn = _ADDRESSES[name]
+    rc = _views.call(fn, _ADDRESSES["envg_set_stream"] if _follow_torch_stream else 0, DEVICE_PTRS if sync else DEVICE_PTRS | ASYNC,
+                     spec, *operands)
+    if rc:
+        _check(rc)
+    return rc is not None
 
 
 def _raw_stream(device):
@@ -743,6 +767,11 @@ def linear_q4(dst, x, W, bias=None, epilogue=None, gate=None, sync=True):
     """dst = epilogue(x . W^T) for a Q4Weight: envg_linear_q4.  x [M, K]; dst [M, N] (N/2 for SILU_GATE)."""
     if epilogue is None:
         epilogue = EPI_SILU_GATE if W.layout == LAYOUT_GATE_UP else (EPI_BIAS if bias is not None else EPI_NONE)
+    if type(x) is _Tensor and x.dim() == 2:
+        M, N = x.size(0), W.N
+        if _call("envg_linear_q4", sync, _LINEAR_Q4_SPEC, dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, x, M, W.K,
+                 _handle(W), bias, N, gate, N, M, W.K, N, epilogue):
+            return OK
     mode = _side(x)
     M, N = x.shape[0], W.N
     px, ldx = _matrix(x, M, W.K, "x", mode)
@@ -761,6 +790,13 @@ def qk_norm_rope(q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, heads, kv_hea
     q [T, heads * hd], k [T, kv_heads * hd] (either may be None with 0 heads); cos / sin
     [P, hd / 2] or None (the norm alone); positions int32 [T], or None for pos0 + t."""
     first = q if q is not None else k
+    if type(first) is _Tensor and first.dim() == 2 and (cos is None or (type(cos) is _Tensor and cos.dim() == 2)):
+        T, wq, wk, half = first.size(0), heads * head_dim, kv_heads * head_dim, head_dim // 2
+        rows = cos.size(0) if cos is not None else 0
+        if _call("envg_qk_norm_rope", sync, _QK_NORM_ROPE_SPEC, q_dst, T, wq, k_dst, T, wk, q, T, wq, k, T, wk,
+                 q_weight, head_dim, k_weight, head_dim, cos, rows, half, sin, rows, half, rows, positions, T,
+                 pos0, T, heads, kv_heads, head_dim, eps, 1 if interleaved else 0):
+            return OK
     mode = _side(first)
     T, wq, wk, half = first.shape[0], heads * head_dim, kv_heads * head_dim, head_dim // 2
     rows = cos.shape[0] if cos is not None else 0
@@ -794,20 +830,25 @@ class KV4Cache:
         _check(lib().envg_kv4_create(pages, page_size, kv_heads, head_dim, ctypes.byref(h)))
         self.pages, self.page_size, self.kv_heads, self.head_dim, self.h = pages, page_size, kv_heads, head_dim, h
 
-    def _rows(self, call, k, v, table, ctx_lens, q_len, sync):
+    def _rows(self, name, k, v, table, ctx_lens, q_len, sync):
+        if type(k) is _Tensor and type(ctx_lens) is _Tensor and type(table) is _Tensor and table.dim() == 2:
+            B, width, pages = ctx_lens.numel(), self.kv_heads * self.head_dim, table.size(1)
+            if _call(name, sync, _KV4_ROWS_SPEC, _handle(self), k, B * q_len, width, v, B * q_len, width, table, B, pages, pages,
+                     ctx_lens, B, B, q_len):
+                return OK
         mode = _side(k)
         B, width = ctx_lens.shape[0], self.kv_heads * self.head_dim
-        return _check(call(_KV4_ROWS.pack(_handle(self), *_matrix(k, B * q_len, width, "k", mode),
+        return _check(getattr(lib(), name)(_KV4_ROWS.pack(_handle(self), *_matrix(k, B * q_len, width, "k", mode),
                                           *_matrix(v, B * q_len, width, "v", mode), *_table(table, ctx_lens, B, mode),
                                           B, q_len), _flags(mode, sync)))
 
     def append(self, k, v, table, ctx_lens, q_len=1, sync=True):
         """Write the newest ``q_len`` tokens of each sequence; k, v [B * q_len, kv_heads * hd]: envg_kv4_append."""
-        return self._rows(lib().envg_kv4_append, k, v, table, ctx_lens, q_len, sync)
+        return self._rows("envg_kv4_append", k, v, table, ctx_lens, q_len, sync)
 
     def read(self, k, v, table, ctx_lens, q_len=1, sync=True):
         """The values held for the newest ``q_len`` tokens of each sequence, into k and v: envg_kv4_read."""
-        return self._rows(lib().envg_kv4_read, k, v, table, ctx_lens, q_len, sync)
+        return self._rows("envg_kv4_read", k, v, table, ctx_lens, q_len, sync)
 
     def free(self):
         if self.h is not None and self.h.value:
@@ -826,10 +867,15 @@ def attention_kv4(dst, q, cache, table, ctx_lens, heads, q_len=1, max_ctx=0, win
 
     q, dst [B * q_len, heads * hd]; causal, with ``window`` > 0 only the last ``window`` tokens and the
     first ``sinks``; ``max_ctx`` (0: unknown) is the largest of ctx_lens and only plans the launch."""
-    mode = _side(q)
-    B, width = ctx_lens.shape[0], heads * cache.head_dim
     if scale is None:
         scale = cache.head_dim ** -0.5
+    if type(q) is _Tensor and type(ctx_lens) is _Tensor and type(table) is _Tensor and table.dim() == 2:
+        B, width, pages = ctx_lens.numel(), heads * cache.head_dim, table.size(1)
+        if _call("envg_attention_kv4", sync, _ATTENTION_KV4_SPEC, dst, B * q_len, width, q, B * q_len, width, _handle(cache),
+                 table, B, pages, pages, ctx_lens, B, B, q_len, max_ctx, heads, window, sinks, scale):
+            return OK
+    mode = _side(q)
+    B, width = ctx_lens.shape[0], heads * cache.head_dim
     return _check(lib().envg_attention_kv4(
         _ATTENTION_KV4.pack(*_matrix(dst, B * q_len, width, "dst", mode), *_matrix(q, B * q_len, width, "q", mode),
                             _handle(cache), *_table(table, ctx_lens, B, mode), B, q_len, max_ctx, heads, window, sinks,
