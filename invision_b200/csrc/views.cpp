@@ -139,10 +139,21 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// A tensor without plain storage (nested, functional, ..) throws where it is asked for its sizes or
+// its memory: it is one of those that the binding looks at again.
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  try {
+    return F(self, args, n);
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
 PyMethodDef methods[] = {
-    {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr},
-    {"matrix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(matrix)), METH_FASTCALL, nullptr},
-    {"vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(vector)), METH_FASTCALL, nullptr},
+    {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<call>)), METH_FASTCALL, nullptr},
+    {"matrix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<matrix>)), METH_FASTCALL, nullptr},
+    {"vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<vector>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_views", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

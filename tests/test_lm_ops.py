@@ -101,3 +101,30 @@ def test_packed_structures_match_the_header(tmp_path):
     subprocess.check_call(["gcc", "-I", os.path.dirname(envg.HEADER_PATH), str(src), "-o", str(tmp_path / "s")])
     sizes = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()
     assert [int(v) for v in sizes] == [st.size for st in names.values()]
+
+
+def test_one_step_calls_leave_other_tensors_to_the_binding():
+    """_views.call makes no call with a tensor that is not the CUDA matrix its spec asks for, nor with
+    numbers that a field does not hold; it never throws through the interpreter."""
+    import ctypes
+
+    torch = pytest.importorskip("torch")
+    with pytest.raises(TypeError, match="CUDA"):
+        envg._side(torch.zeros(1))
+    if envg._views is None:
+        pytest.skip("the torch extension was not built for this torch")
+    calls = []
+    fn = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int)(lambda p, f: calls.append(f) or 0)
+    at, call = ctypes.cast(fn, ctypes.c_void_p).value, envg._views.call
+    nested = torch.nested.as_nested_tensor([torch.zeros(2, 2), torch.zeros(3, 2)], layout=torch.strided)
+    for t in (torch.zeros(2, 2), torch.empty(2, 2, device="meta"), nested, np.zeros((2, 2), np.float32), "x", None):
+        assert call(at, 0, 0, "M", t, 2, 2) is None
+        if t is not None:
+            assert envg._views.matrix(t, 2, 2, 0) is None and envg._views.vector(t, 2, 0) is None
+    for spec, operands, error in (("M", (), TypeError), ("q", (1, 2), TypeError), ("i", (1 << 40,), OverflowError),
+                                  ("f", (1e300,), OverflowError), ("q", (1.5,), TypeError), ("p", (-1,), OverflowError)):
+        with pytest.raises(error):
+            call(at, 0, 0, spec, *operands)
+    with pytest.raises(TypeError):
+        call(at, 0, 0, "q" * 40, *range(40))  # more than a structure holds
+    assert not calls
