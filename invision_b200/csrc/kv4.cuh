@@ -204,8 +204,8 @@ struct KvRowsArgs {
 
 // A thread takes ROWS consecutive tokens, so that most find their tile where the last one's was
 // (one token to a thread spent two thirds of its instructions on finding it).  4096 tokens, 8 heads
-// of 128, written and read back: 25.9 us, 3.0 TB/s over both kernels, bound by instructions; 33.5
-// with V's bytes of a token in four lines instead of one.
+// of 128, written and read back: 23.9 us, 3.2 TB/s over both kernels, bound by instructions; 7.6 us
+// more with V's bytes of a token in four lines instead of one.
 template <bool READ, int ROWS>
 __global__ void __launch_bounds__(256) k_kv4_rows(const KvRowsArgs a) {
   griddep_wait();

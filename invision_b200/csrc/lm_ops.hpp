@@ -296,10 +296,13 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   a.c = kv_view(d, c, table, stride, lens);
   a.k = dk, a.v = dv, a.ldk = lk, a.ldv = lv;
   a.hd = c->head_dim, a.batch = batch, a.q_len = q_len;
-  // four tokens to a thread once they fill the GPU's threads all the same
+  // two or four tokens to a thread once they fill the GPU's threads all the same (append and read of
+  // 1024 / 2048 / 4096 / 8192 / 16384 tokens, 8 heads of 128, us: 9.7 / 15.2 / 25.8 / - / - with one,
+  // 10.3 / 14.5 / 23.9 / 40.9 / 78.2 with two, - / 18.2 / 25.6 / 42.4 / 75.8 with four)
   const int run_threads = c->kv_heads * 2 * (c->head_dim / KV_GROUP) * 8;
-  const bool four = q_len >= 4 && rows * run_threads >= (int64_t)d->sms * 2048 * 4;
-  const int runs_seq = (int)cdiv(q_len, four ? 4 : 1);
+  const int64_t fill = rows * run_threads / ((int64_t)d->sms * 2048);
+  const int each = q_len >= 4 && fill >= 10 ? 4 : q_len >= 2 && fill >= 1 ? 2 : 1;
+  const int runs_seq = (int)cdiv(q_len, each);
   a.runs = batch * runs_seq;
   a.runs_per = std::max(1, 256 / run_threads);
   a.per_run = FastDiv((uint32_t)run_threads);
@@ -309,8 +312,9 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
   {
     ProfScope ps(stream_of(d), read ? KID_KV4_READ : KID_KV4_APPEND, 0.0,
                  (double)rows * c->kv_heads * (8.0 * c->head_dim + c->head_dim + 8 * (c->head_dim / KV_GROUP)));
-    ENVG_TRY(read ? (four ? launch_pdl(d, k_kv4_rows<true, 4>, grid, dim3(256), 0, a) : launch_pdl(d, k_kv4_rows<true, 1>, grid, dim3(256), 0, a))
-                  : (four ? launch_pdl(d, k_kv4_rows<false, 4>, grid, dim3(256), 0, a) : launch_pdl(d, k_kv4_rows<false, 1>, grid, dim3(256), 0, a)));
+    void (*kernel)(const KvRowsArgs) = read ? (each == 4 ? k_kv4_rows<true, 4> : each == 2 ? k_kv4_rows<true, 2> : k_kv4_rows<true, 1>)
+                                            : (each == 4 ? k_kv4_rows<false, 4> : each == 2 ? k_kv4_rows<false, 2> : k_kv4_rows<false, 1>);
+    ENVG_TRY(launch_pdl(d, kernel, grid, dim3(256), 0, a));
     d->st.kernel_launches++;
   }
   if (!devp && read) {

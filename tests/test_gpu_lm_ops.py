@@ -301,6 +301,13 @@ def test_kv4_append_read_bit_for_bit(gpu, lens, q_len, page, KVH, hd):
         assert np.array_equal(got, ref.astype(np.float32))
 
 
+@pytest.mark.parametrize("lens,q_len,page,KVH,hd", [([1500, 1190], 1201, 48, 8, 128), ([2401], 2401, 16, 16, 64), ([12003], 12001, 64, 8, 128), ([6001, 5999], 6001, 32, 16, 64)])
+def test_kv4_append_read_long_runs(gpu, lens, q_len, page, KVH, hd):
+    """Enough tokens that a thread takes two or four of them: odd lengths, runs that begin inside a tile
+    and before the first token."""
+    test_kv4_append_read_bit_for_bit(gpu, lens, q_len, page, KVH, hd)
+
+
 def test_kv4_append_keeps_its_neighbours_and_holds_nan(gpu):
     """Token by token equals all at once; a NaN stays in its group; device strides."""
     import torch
