@@ -561,3 +561,54 @@ def test_random_shapes_against_formulas(gpu):
         window = int(rng.choice([0, 1, 20, 130]))
         c, table, ks, vs = _held(gpu, rng, lens, page, KVH, hd)
         _check_attention(gpu, rng, c, table, ks, vs, lens, q_len, KVH * per, hd, window, int(rng.integers(0, 40)) if window else 0)
+
+
+def test_torch_operands_are_the_same_by_every_way_of_the_binding(gpu, monkeypatch):
+    """One-step calls, checks of each operand by the extension, checks in Python: equal bits, equal
+    refusals; strided operands, a side stream, a subclass of torch.Tensor."""
+    import torch
+
+    from invision_b200 import envg
+
+    rng = np.random.default_rng(77)
+    H, KVH, hd, B, L = 4, 2, 64, 3, 70
+    table, pages = _tables(rng, [L] * B, 16)
+    w = gpu.Q4Weight(*gpu.quantize_q4(rng.standard_normal((H * hd, 96)).astype(np.float32), 32), K=96, group=32)
+    cud = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    x, bias = cud(rng.standard_normal((B, 96)).astype(np.float32)), cud(rng.standard_normal(H * hd).astype(np.float32))
+    kv = cud(rng.standard_normal((B, 2 * KVH * hd + 5)).astype(np.float32))
+    nw, ang = cud(rng.standard_normal(hd).astype(np.float32)), cud(rng.standard_normal((L, hd // 2)).astype(np.float32))
+    td, pos = cud(table), cud(np.array([0, 7, 69], np.int32))
+    stream = torch.cuda.Stream()
+
+    def layer():
+        cache = gpu.KV4Cache(pages, 16, KVH, hd)
+        lens = cud(np.array([1, 1, 1], np.int32))
+        q, k = torch.empty(B, H * hd + 3, device="cuda"), torch.empty(B, KVH * hd, device="cuda")
+        ko, vo, out = torch.empty_like(k), torch.empty_like(k), torch.empty(B, H * hd, device="cuda")
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            gpu.linear_q4(q[:, : H * hd], x, w, bias=torch.nn.Parameter(bias), sync=False)
+            gpu.qk_norm_rope(q[:, : H * hd], k, q[:, : H * hd], kv[:, : KVH * hd], nw, nw, ang.cos(), ang.sin(), H, KVH, hd, positions=pos, sync=False)
+            cache.append(k, kv[:, KVH * hd : 2 * KVH * hd], td, lens, sync=False)
+            cache.read(ko, vo, td, lens, sync=False)
+            gpu.attention_kv4(out, q[:, : H * hd], cache, td, lens, H, window=5, sinks=1, sync=True)
+        with pytest.raises(ValueError, match="x"):
+            gpu.linear_q4(out, x[:, :95], w)
+        with pytest.raises(TypeError):
+            gpu.linear_q4(out, x.double(), w)
+        with pytest.raises(ValueError, match="ctx_lens|q|dst"):
+            gpu.attention_kv4(out[:2], q[:, : H * hd], cache, td, lens, H)
+        with pytest.raises(TypeError):
+            cache.append(k.cpu(), k, td, lens)
+        return [t.cpu().numpy() for t in (q[:, : H * hd], k, ko, vo, out)]
+
+    ways = [layer()]
+    assert envg._Tensor is torch.Tensor  # the extension is there
+    monkeypatch.setattr(envg, "_Tensor", None)
+    ways.append(layer())
+    monkeypatch.setattr(envg, "_views", None)
+    ways.append(layer())
+    for other in ways[1:]:
+        for a, b in zip(ways[0], other):
+            assert np.isfinite(a).all() and np.array_equal(a, b)
