@@ -335,8 +335,8 @@ struct KvAttnArgs {
 // unsigned 16-row operand (16 tokens of K, 16 channels of V^T), four of them unpacked by one or two
 // logic operations, once for all rows.  The other factor is the 8-column one, a fixed-point number
 // cut into digits to the base 256: q with 31 bits of its row's largest value in four signed
-// digits (two products of two adjacent columns a row), p s with 22 bits of the unit's largest in
-// three unsigned ones.  A thread joins its digits' sums, which are one row's, in integers and
+// digits (two products of two adjacent columns a row), p s with 22 bits of its group's largest in the
+// unit in three unsigned ones.  A thread joins its digits' sums, which are one row's, in integers and
 // converts once.  The c - 8 of the output comes from a start of the sums at -8 sum(p s), itself a
 // product (sums of the positive codes would be far larger than the result and cost its last bits).
 // Scores come out as [token][row]; an 8 x 8 transpose in registers (movmatrix) makes the p s operand
@@ -623,14 +623,14 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
       }
     }
     uint32_t pb[NB][G][2][2];  // [operand][tile]
-    float f[NB];               // what one unit of the weights' fixed-point numbers stands for
+    float f[NB][G];            // what one unit of the weights' fixed-point numbers stands for
     // a token that one thread's row sees may be hidden from its other rows: 0 x NaN must not come
     // through there (with one row to a thread, what it does not see is zero already)
     auto hidden = [&](float p) { return NB > 1 && !whole && p == 0.0f; };
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const float ref = m[nb] == -INFINITY ? 0.0f : m[nb];
-      float v[2][2][G], most = 0.0f;
+      float v[2][2][G], most[G] = {};
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -641,20 +641,27 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
           for (int gi = 0; gi < G; ++gi) {
             pm[nb][gi] = fmaf(p, hidden(p) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
             v[tt][i][gi] = hidden(p) ? 0.0f : p * vs[tt][i][gi];
-            most = fmaxf(most, v[tt][i][gi]);
+            most[gi] = fmaxf(most[gi], v[tt][i][gi]);
           }
         }
+      // Each group has a unit of its own: a group of small values beside one of large values keeps its
+      // bits.  Only the exponents count, so that two groups' largest travel in the halves of a word.
+      uint32_t tops = G == 2 ? __byte_perm(__float_as_uint(most[0]), __float_as_uint(most[G - 1]), 0x7632) : __float_as_uint(most[0]) >> 16;
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+      for (int off = 4; off < 32; off <<= 1) tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, off));
       // scaled so that the largest is in [2^21, 2^22); added to 2^23, the integer stands in the low bits
-      const int field = max(22, (int)(__float_as_uint(most) >> 23));
-      const float up = __int_as_float((275 - field) << 23);
-      f[nb] = __int_as_float((field - 21) << 23);
+      float up[G];
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        const int field = max(22, (int)(gi ? tops >> 23 : (tops >> 7) & 255u));
+        up[gi] = __int_as_float((275 - field) << 23);
+        f[nb][gi] = __int_as_float((field - 21) << 23);
+      }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
-          const uint32_t v0 = __float_as_uint(fmaf(v[tt][0][gi], up, 8388608.0f)), v1 = __float_as_uint(fmaf(v[tt][1][gi], up, 8388608.0f));
+          const uint32_t v0 = __float_as_uint(fmaf(v[tt][0][gi], up[gi], 8388608.0f)), v1 = __float_as_uint(fmaf(v[tt][1][gi], up[gi], 8388608.0f));
           pb[nb][gi][0][tt] = transpose_8x8(__byte_perm(v0, v1, 0x5140));
           pb[nb][gi][1][tt] = transpose_8x8(__byte_perm(v0, v1, 0x7362));  // its second column is not used
         }
@@ -682,7 +689,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
           for (int k = 0; k < 2; ++k) mma_u8u8(d[k], a0, a1, a2, a3, pb[nb][gi][k][0], pb[nb][gi][k][1], minus[nb][k]);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
-            o[nb][4 * gi + i][c] = fmaf((float)(d[1][2 * c] * 65536 + d[0][2 * c + 1] * 256 + d[0][2 * c]), f[nb], o[nb][4 * gi + i][c]);
+            o[nb][4 * gi + i][c] = fmaf((float)(d[1][2 * c] * 65536 + d[0][2 * c + 1] * 256 + d[0][2 * c]), f[nb][gi], o[nb][4 * gi + i][c]);
         }
       }
     }

@@ -100,3 +100,21 @@ def attention(q, k, v, pos, window, sinks, scale):
 def rel(a, b):
     n = np.linalg.norm(b)
     return np.linalg.norm(np.asarray(a, np.float64) - b) / n if n else float(np.abs(a).max())
+
+
+def attention_exact(q, k, v, pos, window, sinks, scale):
+    """One sequence in 64 bits: q [n, H, hd] at positions pos, the values held k [L, KVH, hd], v [L, KVH, dv]."""
+    n, H, _ = q.shape
+    L, KVH = k.shape[:2]
+    j, per = np.arange(L), H // KVH
+    see = j <= np.asarray(pos)[:, None]
+    if window > 0:
+        see &= (j > np.asarray(pos)[:, None] - window) | (j < sinks)
+    out = np.zeros((n, H, v.shape[2]))
+    for h in range(H):
+        x = np.where(see, scale * (q[:, h].astype(np.float64) @ k[:, h // per].astype(np.float64).T), -np.inf)
+        top = x.max(-1, keepdims=True)
+        p = np.exp(x - np.where(top > -np.inf, top, 0.0))
+        total = p.sum(-1, keepdims=True)
+        out[:, h] = (p / np.where(total > 0, total, 1.0)) @ v[:, h // per].astype(np.float64)
+    return out

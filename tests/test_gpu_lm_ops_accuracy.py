@@ -1,0 +1,48 @@
+"""GPU: what the language-model decode operators keep of their operands' bits: groups of channels
+of very different sizes, rows near the ends of fp32's range, NaN that has to come through."""
+import numpy as np
+import pytest
+
+from tests import lm_ref as R
+
+pytestmark = pytest.mark.gpu
+
+# 2-norm of a group's error over the group's own norm, for scores up to 16 in log2 units.  A score is
+# rounded to fp32 about four times at that size (2^-20 / sqrt(12) each, 5.5e-7 together, times ln 2 in
+# the weight), a weight by its exponential (2^-22), its product with V's scale to 22 bits of the
+# group's largest and by up to some tens of fp32 additions (2e-7): together below 1e-6.
+REL_GROUP = 2e-6
+
+
+def _fill(gpu, rng, lens, page, k, v):
+    """A cache holding k and v ([sequences][tokens, KVH, hd]) in shuffled pages: (cache, table)."""
+    KVH, hd = k[0].shape[1:]
+    per = -(-max(lens) // page)
+    table = rng.permutation(len(lens) * per).astype(np.int32).reshape(len(lens), per)
+    c = gpu.KV4Cache(len(lens) * per, page, KVH, hd)
+    for b, n in enumerate(lens):
+        c.append(k[b].reshape(n, -1), v[b].reshape(n, -1), table[b : b + 1], np.array([n], np.int32), q_len=n)
+    return c, table
+
+
+@pytest.mark.parametrize("ratio", [1.0, 1e-1, 1e2, 1e3, 1e-4, 1e6])
+@pytest.mark.parametrize("lens,q_len,H,KVH,window,sinks", [([700, 333], 1, 8, 2, 0, 0), ([700, 333], 1, 16, 2, 0, 0),
+                                                           ([400], 5, 4, 2, 100, 7), ([33], 3, 2, 2, 0, 0)])
+def test_attention_kv4_value_groups_of_different_size(gpu, lens, q_len, H, KVH, window, sinks, ratio):
+    """Channels 0..63 and 64..127 of V differ in size by `ratio`: each keeps its own precision."""
+    hd = 128
+    rng = np.random.default_rng(H + q_len)
+    size = np.repeat([ratio ** 0.5, ratio ** -0.5], 64).astype(np.float32)
+    k = [rng.standard_normal((n, KVH, hd)).astype(np.float32) for n in lens]
+    v = [rng.standard_normal((n, KVH, hd)).astype(np.float32) * size for n in lens]
+    c, table = _fill(gpu, rng, lens, 16, k, v)
+    q = rng.standard_normal((len(lens) * q_len, H * hd)).astype(np.float32)
+    out = np.full_like(q, np.nan)
+    gpu.attention_kv4(out, q, c, table, np.asarray(lens, np.int32), H, q_len=q_len, window=window, sinks=sinks)
+    for b, n in enumerate(lens):
+        rows = slice(b * q_len, (b + 1) * q_len)
+        ref = R.attention_exact(q[rows].reshape(q_len, H, hd), R.kv_hold(k[b]), R.kv_hold(v[b]), n - q_len + np.arange(q_len),
+                                window, sinks, hd ** -0.5)
+        got = out[rows].reshape(q_len, H, hd)
+        for g in (np.s_[..., :64], np.s_[..., 64:]):
+            assert R.rel(got[g], ref[g]) <= REL_GROUP, (b, ratio, R.rel(got[g], ref[g]))
