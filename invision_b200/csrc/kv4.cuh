@@ -625,8 +625,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
     uint32_t pb[NB][G][2][2];  // [operand][tile]
     float f[NB][G];            // what one unit of the weights' fixed-point numbers stands for
     // a token that one thread's row sees may be hidden from its other rows: 0 x NaN must not come
-    // through there (with one row to a thread, what it does not see is zero already)
-    auto hidden = [&](float p) { return NB > 1 && !whole && p == 0.0f; };
+    // through there (with one row to a thread, what it does not see is zero already).  By the score, not
+    // the weight: a token that is seen gives its NaN whatever its weight.
+    auto hidden = [&](float score) { return NB > 1 && !whole && score == -INFINITY; };
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const float ref = m[nb] == -INFINITY ? 0.0f : m[nb];
@@ -639,8 +640,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
           l[nb] += p;
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
-            pm[nb][gi] = fmaf(p, hidden(p) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
-            v[tt][i][gi] = hidden(p) ? 0.0f : p * vs[tt][i][gi];
+            pm[nb][gi] = fmaf(p, hidden(x[nb][tt][i]) ? 0.0f : fmaf(8.0f, vs[tt][i][gi], vm[tt][i][gi]), pm[nb][gi]);
+            v[tt][i][gi] = hidden(x[nb][tt][i]) ? 0.0f : p * vs[tt][i][gi];
             most[gi] = fmaxf(most[gi], v[tt][i][gi]);
           }
         }
@@ -746,8 +747,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
     for (int w = 0; w < KVA_WARPS; ++w) mw[w] = ml[w * 2 * ROWS + r], top = fmaxf(top, mw[w]);
 #pragma unroll
     for (int w = 0; w < KVA_WARPS; ++w) {
-      const float e = mw[w] == -INFINITY ? 0.0f : ex2(mw[w] - top);
-      if (e > 0.0f) {
+      if (mw[w] != -INFINITY) {  // with a weight of zero too: its NaN has to come through
+        const float e = ex2(mw[w] - top);
         const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + (w * ROWS + r) * S::OUT_LD + c);
         sum = fmaf(e, ml[w * 2 * ROWS + ROWS + r], sum);
         y.x = fmaf(e, v.x, y.x), y.y = fmaf(e, v.y, y.y), y.z = fmaf(e, v.z, y.z), y.w = fmaf(e, v.w, y.w);
@@ -782,8 +783,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
     for (int s = 0; s < 8; ++s) top = fmaxf(top, ms[s]);
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const float e = ms[s] == -INFINITY ? 0.0f : ex2(ms[s] - top);
-      if (e > 0.0f) {
+      if (ms[s] != -INFINITY) {
+        const float e = ex2(ms[s] - top);
         sum = fmaf(e, ls[s], sum);
         y.x = fmaf(e, v[s].x, y.x), y.y = fmaf(e, v[s].y, y.y), y.z = fmaf(e, v[s].z, y.z), y.w = fmaf(e, v[s].w, y.w);
       }

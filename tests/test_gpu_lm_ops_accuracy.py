@@ -46,3 +46,35 @@ def test_attention_kv4_value_groups_of_different_size(gpu, lens, q_len, H, KVH, 
         got = out[rows].reshape(q_len, H, hd)
         for g in (np.s_[..., :64], np.s_[..., 64:]):
             assert R.rel(got[g], ref[g]) <= REL_GROUP, (b, ratio, R.rel(got[g], ref[g]))
+
+
+@pytest.mark.parametrize("n,q_len,H,KVH,window", [(2000, 1, 4, 1, 0), (2000, 1, 8, 1, 0), (90, 1, 1, 1, 0), (300, 2, 4, 1, 250), (1600, 3, 4, 2, 1500)])
+@pytest.mark.parametrize("what", ["key", "value", "infinite score"])
+def test_attention_kv4_seen_nan_comes_through_beside_large_scores(gpu, n, q_len, H, KVH, window, what):
+    """A token with a NaN whose weight underflows beside one of a far larger score, whichever warps and
+    CTAs the two fall to: the row (a NaN key) or the channels of its group (a NaN value) are NaN."""
+    hd = 128
+    first = max(0, n - q_len + 1 - window) + q_len if window else 0
+    for at, big in ((first, n - q_len - 1), (n - q_len - 3, first + 2), (first + 7, first + 41), ((first + n) // 2, first + 1)):
+        rng = np.random.default_rng(at)
+        q = rng.standard_normal((q_len, H * hd)).astype(np.float32)
+        k = rng.standard_normal((n, KVH, hd)).astype(np.float32)
+        v = rng.standard_normal((n, KVH, hd)).astype(np.float32)
+        for h in range(H):  # every row scores this token by some hundreds above the others
+            k[big, h // (H // KVH)] += 40.0 * np.sign(q[:, h * hd : (h + 1) * hd]).sum(0)
+        q *= 6.0
+        if what == "key":
+            k[at] = np.nan
+        elif what == "value":
+            v[at, :, 70] = np.nan
+        else:
+            q[:] = np.abs(q) * 1e36
+            k[at] = 3e4
+        c, table = _fill(gpu, rng, [n], 16, [k], [v])
+        out = np.zeros_like(q)
+        gpu.attention_kv4(out, q, c, table, np.array([n], np.int32), H, q_len=q_len, window=window)
+        out = out.reshape(q_len, H, hd)
+        if what == "value":
+            assert np.isfinite(out[..., :64]).all() and np.isnan(out[..., 64:]).all(), (at, big)
+        else:
+            assert np.isnan(out).all(), (at, big)
