@@ -339,7 +339,9 @@ int envg_linear_noalloc(float* dst, const float* x, envg_weight W, const float* 
  * follow the conventions above (fp32 rows, status codes, host or device pointers by `flags`), take
  * a row stride for every matrix and allocate nothing with device pointers.  Arguments that only
  * the device can read (a page table, lengths, positions) are checked there: a value out of range
- * reads and writes nothing out of bounds, and the next synchronising call returns ENVG_ERR_ARG. */
+ * reads and writes nothing out of bounds, and the next synchronising call returns ENVG_ERR_ARG.
+ * Tokens whose page does not exist are left out; of a sequence whose length does not fit the table
+ * nothing is appended, and its rows of a read or of attention are zeros. */
 
 /* Opaque device-resident 4-bit weight. */
 typedef struct envg_q4weight_s* envg_q4weight;

@@ -496,7 +496,7 @@ int check_status(Dev* d) {
     if (st == ENVG_ERR_ARG)
       return fail(st, "a device-side argument was out of range: %s",
                   site == SITE_KV_PAGE    ? "the page table names no page of the cache (its tokens were left out)"
-                  : site == SITE_KV_LEN   ? "a context length does not fit its row of the page table"
+                  : site == SITE_KV_LEN   ? "a context length does not fit its row of the page table (its sequence was left out)"
                   : site == SITE_ROPE_POS ? "a position lies outside the cos / sin tables"
                                           : "a zero point of a 4-bit weight is above 15");
     return fail(st, "device-side wait exceeded its bound (site %d); pipeline abandoned", site);

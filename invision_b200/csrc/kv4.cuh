@@ -51,13 +51,13 @@ struct Kv4View {
   int* status;
 };
 
-// Tokens of sequence b, held to what its row of the table can name.
+// Tokens of sequence b; none where the length is not one that its row of the table can name, so that
+// a wrong length cannot overwrite tokens that are held.
 ENVG_DEV int kv_len(const Kv4View& c, int b) {
-  const int64_t most = c.table_stride * c.page_size;
   const int n = __ldg(c.ctx_lens + b);
-  if (n < 0 || n > most) {
+  if (n < 0 || n > c.table_stride * c.page_size) {
     kv_flag(c.status, SITE_KV_LEN);
-    return n < 0 ? 0 : (int)most;
+    return 0;
   }
   return n;
 }

@@ -612,3 +612,47 @@ def test_torch_operands_are_the_same_by_every_way_of_the_binding(gpu, monkeypatc
     for other in ways[1:]:
         for a, b in zip(ways[0], other):
             assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
+def test_kv4_length_beyond_the_table_leaves_its_sequence_alone(gpu):
+    """A length that only the device can see to be out of range: nothing is appended for its sequence and
+    what the cache holds stays; reads and attention give zeros there; the other sequences are served."""
+    import torch
+
+    rng = np.random.default_rng(4)
+    KVH, hd, page, H, B = 2, 64, 16, 4, 3
+    table = torch.arange(6, dtype=torch.int32, device="cuda").view(B, 2)
+    c = gpu.KV4Cache(6, page, KVH, hd)
+    dev = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    full, some = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([32, 32, 32], [32, 30, 32]))
+
+    def held():
+        k, v = (torch.empty(B * 32, KVH * hd, device="cuda") for _ in range(2))
+        c.read(k, v, table, full, q_len=32)
+        return k.cpu().numpy().reshape(B, 32, -1), v.cpu().numpy().reshape(B, 32, -1)
+
+    c.append(dev(B * 32, KVH * hd), dev(B * 32, KVH * hd), table, full, q_len=32)
+    before = held()
+    q, out, good = dev(B * 3, H * hd), torch.full((B * 3, H * hd), 7.0, device="cuda"), torch.empty(B * 3, H * hd, device="cuda")
+    k, v = dev(B * 3, KVH * hd), dev(B * 3, KVH * hd)
+    for n in (33, 2 ** 31 - 1, -1):
+        lens = torch.tensor([32, n, 32], dtype=torch.int32, device="cuda")
+        gpu.attention_kv4(good, q, c, table, some, H, q_len=3)
+        with pytest.raises(gpu.EnvgError, match="length"):
+            gpu.attention_kv4(out, q, c, table, lens, H, q_len=3)
+        o, g = out.cpu().numpy().reshape(B, 3, -1), good.cpu().numpy().reshape(B, 3, -1)
+        assert (o[1] == 0).all() and np.array_equal(o[[0, 2]], g[[0, 2]])
+        ko, vo = (torch.full((B * 3, KVH * hd), 7.0, device="cuda") for _ in range(2))
+        with pytest.raises(gpu.EnvgError, match="length"):
+            c.read(ko, vo, table, lens, q_len=3)
+        for got, was in zip((ko, vo), before):
+            got = got.cpu().numpy().reshape(B, 3, -1)
+            assert (got[1] == 0).all() and np.array_equal(got[[0, 2]], was[[0, 2], 29:])
+        with pytest.raises(gpu.EnvgError, match="length"):
+            c.append(k, v, table, lens, q_len=3)
+        after = held()
+        for got, was, x in zip(after, before, (k, v)):
+            assert np.array_equal(got[1], was[1]) and np.array_equal(got[[0, 2], :29], was[[0, 2], :29])
+            new = R.kv_hold(x.cpu().numpy().reshape(B, 3, KVH, hd)).reshape(B, 3, -1)
+            assert np.array_equal(got[[0, 2], 29:], new[[0, 2]])
+        before = after
