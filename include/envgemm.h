@@ -473,10 +473,12 @@ int envg_sgemm(int order, int transA, int transB, int64_t M, int64_t N, int64_t 
 
 /* Make the library launch on a caller-owned stream (a cudaStream_t passed as void*), or back on
  * its own non-blocking stream with NULL.  The legacy default stream is cudaStreamLegacy
- * ((void*)1), not NULL.  Lets a PyTorch or CUDA-graph caller order the kernels itself. */
+ * ((void*)1), not NULL.  Lets a PyTorch or CUDA-graph caller order the kernels itself.  The
+ * selection holds for the calling thread; a thread that has selected none since envg_init uses
+ * the one that any thread selected last. */
 int envg_set_stream(void* stream);
 
-/* Wait for all work queued by this thread's calls. */
+/* Wait for all work queued on this thread's stream (see envg_set_stream). */
 int envg_sync(void);
 
 /* Thread-local text of the last error ("" if none). */

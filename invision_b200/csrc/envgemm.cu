@@ -84,8 +84,10 @@ struct Dev {
   bool ready = false;
   int id = -1;
   int sms = 0;
+  uint64_t epoch = 0;             // counts envg_init and envg_shutdown: what a thread selected before is void
   cudaStream_t own = nullptr;
-  cudaStream_t user = nullptr;
+  cudaStream_t user = nullptr;    // selected last by any thread (envg_set_stream)
+  cudaStream_t within = nullptr;  // while set, the stream of a step inside a call
   Buf x, y, xb, wb, part, cnt, bias, gate, act, col, b32, xbatch, ada, xn;
   Buf gn, c1, vec;  // GroupNorm statistics + affine, ResBlock conv1 output, small parameter vectors
   Buf fa, fain;     // attention operands (bf16 Q / K / V^T + key bits), host-call staging
@@ -208,7 +210,21 @@ void resolve_pending() {
 }
 
 Dev* cur() { return (g_cur >= 0 && g_dev[g_cur].ready) ? &g_dev[g_cur] : nullptr; }
-cudaStream_t stream_of(Dev* d) { return d->user ? d->user : d->own; }
+
+// The stream that this thread selected last.  Selecting and calling are two locked steps, so a
+// selection shared by all threads would let one thread's call run on the stream of another.
+struct ThreadStream {
+  uint64_t epoch = 0;
+  cudaStream_t s = nullptr;
+};
+thread_local ThreadStream t_stream[64];
+
+cudaStream_t stream_of(Dev* d) {
+  if (d->within) return d->within;
+  const ThreadStream& t = t_stream[d->id];
+  const cudaStream_t s = t.epoch == d->epoch ? t.s : d->user;
+  return s ? s : d->own;
+}
 
 int ensure(Dev* d, Buf& b, size_t bytes, bool zero = false) {
   if (bytes == 0) bytes = 256;
@@ -1560,6 +1576,7 @@ int envg_init(int ndev, const int* dev_ids) {
   }
   d->st = envg_stats{};
   d->st.device = id;
+  d->epoch++;
   ENVG_TRY(noalloc_preload(d));
   d->ready = true;
   return ENVG_OK;
@@ -1590,6 +1607,7 @@ int envg_shutdown(void) {
   if (d->h_status) cudaFreeHost(d->h_status);
   d->own = nullptr;
   d->user = nullptr;
+  d->epoch++;
   d->h_status = d->d_status = nullptr;
   d->ready = false;
   g_cur = -1;
@@ -1601,6 +1619,8 @@ int envg_set_stream(void* stream) {
   Dev* d = cur();
   if (!d) return fail(ENVG_ERR_STATE, "envg_init has not been called");
   d->user = reinterpret_cast<cudaStream_t>(stream);
+  t_stream[d->id].epoch = d->epoch;
+  t_stream[d->id].s = d->user;
   return ENVG_OK;
 }
 
@@ -2428,7 +2448,6 @@ int batch_core(Dev* d, const envg_linear_desc* descs, const envg_nsplit_desc* ns
   const size_t ncopies = first_use.size();
   ENVG_CUDA(cudaEventRecord(batch_event(d, 0), s));
   ENVG_CUDA(cudaStreamWaitEvent(d->aux, batch_event(d, 0), 0));
-  cudaStream_t saved = d->user;
   size_t next_copy = 0;
   // Producers of copy j: earlier linears whose output overlaps copy j's input.
   auto produces = [&](int p, size_t j) {
@@ -2474,9 +2493,9 @@ int batch_core(Dev* d, const envg_linear_desc* descs, const envg_nsplit_desc* ns
     const envg_linear_desc& q = descs[first_use[j]];
     for (int p = 0; p < first_use[j]; ++p)
       if (produces(p, j)) ENVG_CUDA(cudaStreamWaitEvent(d->aux, batch_event(d, 1 + ncopies + p), 0));
-    d->user = d->aux;
+    d->within = d->aux;
     int rc = launch_cast_rows(d, q.x, q.K, q.M, q.K, q.W->Kp, base + offset[j]);
-    d->user = saved;
+    d->within = nullptr;
     if (rc != ENVG_OK) return rc;
     ENVG_CUDA(cudaEventRecord(batch_event(d, 1 + j), d->aux));
     return ENVG_OK;
