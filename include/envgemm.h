@@ -478,6 +478,10 @@ int envg_sgemm(int order, int transA, int transB, int64_t M, int64_t N, int64_t 
  * the one that any thread selected last. */
 int envg_set_stream(void* stream);
 
+/* For a binding that knows on which device a call's operands live: ENVG_ERR_ARG unless `device` is
+ * the library's current one; then, with `select` non-zero, as envg_set_stream(stream). */
+int envg_use_device(int device, int select, void* stream);
+
 /* Wait for all work queued on this thread's stream (see envg_set_stream). */
 int envg_sync(void);
 

@@ -1624,6 +1624,14 @@ int envg_set_stream(void* stream) {
   return ENVG_OK;
 }
 
+int envg_use_device(int device, int select, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  Dev* d = cur();
+  if (!d) return fail(ENVG_ERR_STATE, "envg_init has not been called");
+  if (device != d->id) return fail(ENVG_ERR_ARG, "operands live on device %d, the library runs on device %d", device, d->id);
+  return select ? envg_set_stream(stream) : ENVG_OK;
+}
+
 int envg_sync(void) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   Dev* d = cur();

@@ -2,19 +2,21 @@
 // torch's headers (a call checks up to a dozen operands and packs a structure, and the attribute
 // reads of that took longer than the smallest kernels).
 //
-//   call(function, set_stream, flags, spec, ...) -> status of function(structure, flags), with the
-//                                   library put on torch's current stream by set_stream (unless 0)
-//                                   and the structure packed from the operands by `spec`, a letter
-//                                   a field: M matrix (tensor, rows, cols) and its row stride, E the
-//                                   same of exactly cols columns, V float vector (tensor, n), I int
-//                                   vector, P contiguous float matrix (tensor, rows, cols), J int
-//                                   matrix, p pointer, q int64, i int32, f float; None is NULL
+//   call(function, use_device, flags, spec, ...) -> status of function(structure, flags), after that
+//                                   of use_device(operands' device, follow, stream) (unless 0): the
+//                                   library has to run there, and with FOLLOW in flags is put on
+//                                   torch's current stream.  The structure is packed from the
+//                                   operands by `spec`, a letter a field: M matrix (tensor, rows,
+//                                   cols) and its row stride, E the same of exactly cols columns, V
+//                                   float vector (tensor, n), I int vector, P contiguous float matrix
+//                                   (tensor, rows, cols), J int matrix, p pointer, q int64, i int32,
+//                                   f float; None is NULL
 //   matrix(t, rows, cols, dtype) -> (pointer, row stride) of a CUDA tensor [rows, >= cols] of that
 //                                   dtype whose columns are adjacent and rows do not overlap
 //   vector(t, n, dtype)          -> pointer of a contiguous CUDA tensor [n] of that dtype
 //
-// dtype: 0 float32, 1 int32, 2 uint8.  None (and no call) where a tensor is anything else; the
-// binding then looks again and says what is wrong.
+// dtype: 0 float32, 1 int32, 2 uint8.  None (and no call) where a tensor is anything else or lives on
+// another device than the first; the binding then looks again and says what is wrong.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -65,9 +67,10 @@ PyObject* vector(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   constexpr Py_ssize_t MOST = 256;  // bytes of a structure
-  if (n < 4) return PyErr_Format(PyExc_TypeError, "call takes a function, a stream setter, flags, a spec and operands");
+  constexpr int FOLLOW = 1 << 16;  // in flags, for this function alone
+  if (n < 4) return PyErr_Format(PyExc_TypeError, "call takes a function, a device check, flags, a spec and operands");
   auto* fn = reinterpret_cast<int (*)(const void*, int)>(PyLong_AsUnsignedLongLong(args[0]));
-  auto* set_stream = reinterpret_cast<int (*)(void*)>(PyLong_AsUnsignedLongLong(args[1]));
+  auto* use_device = reinterpret_cast<int (*)(int, int, void*)>(PyLong_AsUnsignedLongLong(args[1]));
   const int flags = (int)PyLong_AsLong(args[2]);
   const char* spec = PyUnicode_AsUTF8(args[3]);
   if (PyErr_Occurred()) return nullptr;
@@ -115,6 +118,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         ptr = t->data_ptr();
         if (device < 0) device = t->device().index();
+        if (t->device().index() != device) Py_RETURN_NONE;
       }
       put(&ptr, 8);
       if (*spec == 'M' || *spec == 'E') put(&ld, 8);
@@ -127,14 +131,15 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyErr_Format(PyExc_TypeError, "call: the operands do not match the spec");
   }
   void* stream = nullptr;
-  if (set_stream) {
+  const int follow = (flags & FOLLOW) != 0;
+  if (follow) {
     stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
     if (!stream) stream = reinterpret_cast<void*>(1);  // cudaStreamLegacy, by its own name
   }
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  if (set_stream) set_stream(stream);
-  rc = fn(packed, flags);
+  rc = use_device ? use_device(device, follow, stream) : 0;
+  if (rc == 0) rc = fn(packed, flags & ~FOLLOW);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
 }

@@ -121,6 +121,7 @@ def lib():
         L.envg_kv4_create.argtypes = [_i64, _ci, _ci, _ci, ctypes.POINTER(_vp)]
         L.envg_kv4_free.argtypes = [_vp]
         L.envg_set_stream.argtypes = [_vp]
+        L.envg_use_device.argtypes = [_ci, _ci, _vp]
         L.envg_get_stats.argtypes = [ctypes.POINTER(Stats)]
         L.envg_set_wait_cap_ns.argtypes = [ctypes.c_uint64]
         L.envg_selftest_wait_timeout.argtypes = [ctypes.c_uint64]
@@ -575,6 +576,8 @@ def sgemm(order, transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc):
 # ---------------------------------------------------------------------------------------------
 
 _torch = None  # the torch module, once a tensor has been passed
+_device = 0     # the library's device, as the last call with tensors found it
+_FOLLOW = 1 << 16  # flag of _views.call: launch on torch's current stream
 _views = None   # lib/_views.so: a CUDA tensor's checks, or a whole call, in one step
 _Tensor = None  # torch.Tensor, where _views is there
 _ADDRESSES = {}
@@ -594,8 +597,8 @@ _LINEAR_Q4, _QK_NORM_ROPE, _KV4_ROWS, _ATTENTION_KV4 = (
 
 def _side(a):
     """HOST_PTRS for a call whose operand ``a`` is a numpy array; DEVICE_PTRS, with the library put on
-    torch's current stream, for a CUDA tensor."""
-    global _torch
+    torch's current stream, for a CUDA tensor (which has to live on the library's device)."""
+    global _torch, _device
     if isinstance(a, np.ndarray):
         return HOST_PTRS
     if _torch is None:
@@ -606,8 +609,9 @@ def _side(a):
         _load_views()
     if not (isinstance(a, _torch.Tensor) and a.is_cuda):
         raise TypeError("operands must be numpy arrays (host) or CUDA tensors (device)")
-    if _follow_torch_stream:
-        lib().envg_set_stream(_raw_stream(a.get_device()) or CUDA_STREAM_LEGACY)
+    dev = a.get_device()
+    _check(lib().envg_use_device(dev, _follow_torch_stream, _raw_stream(dev) or CUDA_STREAM_LEGACY if _follow_torch_stream else 0))
+    _device = dev
     return DEVICE_PTRS
 
 
@@ -635,11 +639,11 @@ def _call(name, sync, spec, *operands):
         _ADDRESSES[None] = lib()
     fn = _ADDRESSES.get(name)
     if fn is None:
-        for k in (name, "envg_set_stream"):
+        for k in (name, "envg_use_device"):
             _ADDRESSES[k] = ctypes.cast(getattr(lib(), k), _vp).value
         fn = _ADDRESSES[name]
-    rc = _views.call(fn, _ADDRESSES["envg_set_stream"] if _follow_torch_stream else 0, DEVICE_PTRS if sync else DEVICE_PTRS | ASYNC,
-                     spec, *operands)
+    flags = DEVICE_PTRS if sync else DEVICE_PTRS | ASYNC
+    rc = _views.call(fn, _ADDRESSES["envg_use_device"], flags | _FOLLOW if _follow_torch_stream else flags, spec, *operands)
     if rc:
         _check(rc)
     return rc is not None
@@ -655,6 +659,8 @@ def _on_side(a, mode, name):
     host = isinstance(a, np.ndarray)
     if host != (mode == HOST_PTRS) or not (host or a.is_cuda):
         raise TypeError(f"{name}: operands must be all numpy (host) or all torch CUDA tensors (device)")
+    if not host and a.get_device() != _device:
+        raise ValueError(f"{name}: lives on cuda:{a.get_device()}, the library runs on cuda:{_device}")
     return host
 
 
@@ -664,7 +670,7 @@ def _matrix(a, rows, cols, name, mode, dtype="float32"):
         return 0, 0
     if mode == DEVICE_PTRS and _views is not None:
         got = _views.matrix(a, rows, cols, _CODES[dtype])
-        if got is not None:
+        if got is not None and a.get_device() == _device:
             return got
     host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:
@@ -689,7 +695,7 @@ def _vector(a, n, name, mode, dtype="float32"):
         return 0
     if mode == DEVICE_PTRS and _views is not None:
         got = _views.vector(a, n, _CODES[dtype])
-        if got is not None:
+        if got is not None and a.get_device() == _device:
             return got
     host = _on_side(a, mode, name)
     if a.dtype != (_NP_DTYPES if host else _TORCH_DTYPES)[dtype]:

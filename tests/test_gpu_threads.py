@@ -117,3 +117,10 @@ def test_threads_with_streams_of_their_own_get_their_results(gpu):
         t.join()
     for a, b in zip(alone, got):
         assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
+def test_operands_have_to_live_where_the_library_runs(gpu):
+    L = gpu.lib()
+    assert L.envg_use_device(0, 0, None) == gpu.OK
+    for device in (1, -1):
+        assert L.envg_use_device(device, 1, None) == gpu.ERR_ARG and "device" in gpu.last_error()

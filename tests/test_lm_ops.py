@@ -128,3 +128,52 @@ def test_one_step_calls_leave_other_tensors_to_the_binding():
     with pytest.raises(TypeError):
         call(at, 0, 0, "q" * 40, *range(40))  # more than a structure holds
     assert not calls
+
+
+def _claim(torch, monkeypatch, t, device):
+    """A tensor that says it lives on cuda:`device`; its memory is host memory, which nothing here reads."""
+    import ctypes
+
+    for name in ("init", "_lazy_init"):
+        monkeypatch.setattr(torch.cuda, name, lambda: None)
+    cap = torch.utils.dlpack.to_dlpack(t)
+    get = ctypes.pythonapi.PyCapsule_GetPointer
+    get.restype, get.argtypes = ctypes.c_void_p, [ctypes.py_object, ctypes.c_char_p]
+    where = ctypes.cast(get(cap, b"dltensor") + 8, ctypes.POINTER(ctypes.c_int32))  # DLTensor: data, then device
+    where[0], where[1] = 2, device  # kDLCUDA
+    return torch._C._from_dlpack(cap)
+
+
+def test_operands_of_several_devices_are_refused(monkeypatch):
+    import ctypes
+
+    torch = pytest.importorskip("torch")
+    with pytest.raises(TypeError, match="CUDA"):
+        envg._side(torch.zeros(1))
+    a, b, c = (_claim(torch, monkeypatch, torch.zeros(2, 4), d) for d in (0, 1, 0))
+    n, m = _claim(torch, monkeypatch, torch.zeros(4), 1), _claim(torch, monkeypatch, torch.zeros(4), 0)
+    monkeypatch.setattr(envg, "_device", 0)
+    for views in (envg._views, None):  # the checks of the extension, and those in Python
+        monkeypatch.setattr(envg, "_views", views)
+        assert envg._matrix(a, 2, 4, "x", envg.DEVICE_PTRS) == (a.data_ptr(), 4)
+        assert envg._vector(m, 4, "bias", envg.DEVICE_PTRS) == m.data_ptr()
+        for look in (lambda: envg._matrix(b, 2, 4, "dst", envg.DEVICE_PTRS), lambda: envg._vector(n, 4, "dst", envg.DEVICE_PTRS),
+                     lambda: envg._packed(b, 2, 4, "dst", envg.DEVICE_PTRS)):
+            with pytest.raises(ValueError, match="dst: lives on cuda:1"):
+                look()
+    monkeypatch.undo()
+    if envg._views is None:
+        pytest.skip("the torch extension was not built for this torch")
+    calls, refuse = [], 0
+    fn = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int)(lambda p, f: calls.append(f) or 0)
+    use = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p)(lambda d, s, p: calls.append((d, s, p)) or refuse)
+    at, use_at = (ctypes.cast(f, ctypes.c_void_p).value for f in (fn, use))
+    assert envg._views.call(at, use_at, 3, "MVM", a, 2, 4, m, 4, c, 2, 4) == 0
+    assert calls == [(0, 0, None), 3]
+    calls.clear()
+    for operands in ((a, 2, 4, m, 4, b, 2, 4), (a, 2, 4, n, 4, c, 2, 4), (b, 2, 4, m, 4, c, 2, 4)):
+        assert envg._views.call(at, use_at, 3, "MVM", *operands) is None
+    assert not calls
+    refuse = envg.ERR_ARG  # the library runs on another device
+    assert envg._views.call(at, use_at, 3, "M", a, 2, 4) == envg.ERR_ARG
+    assert calls == [(0, 0, None)]
