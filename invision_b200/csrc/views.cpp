@@ -165,4 +165,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_views", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__views() { return PyModule_Create(&module); }
+// `stamp` says what the module was built from and for; the binding loads no other.
+PyMODINIT_FUNC PyInit__views() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "stamp", ENVG_VIEWS_STAMP) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

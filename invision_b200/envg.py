@@ -617,18 +617,20 @@ def _side(a):
 
 def _load_views():
     global _views, _Tensor
-    path = os.path.join(HERE, "lib", "_views.so")
-    if os.path.exists(path):
+    from . import build
+
+    if os.path.exists(build.VIEWS):
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_loader
 
         try:
-            spec = spec_from_loader("_views", ExtensionFileLoader("_views", path))
+            spec = spec_from_loader("_views", ExtensionFileLoader("_views", build.VIEWS))
             found = module_from_spec(spec)
             spec.loader.exec_module(found)
-            _views, _Tensor = found, _torch.Tensor
-        except ImportError:  # built for another torch: the checks are made attribute by attribute
-            pass
+            if found.stamp == build.views_stamp():
+                _views, _Tensor = found, _torch.Tensor
+        except (ImportError, OSError, AttributeError):
+            pass  # built for another torch, or from another source: the checks are made attribute by attribute
 
 
 def _call(name, sync, spec, *operands):
