@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
     for (int j = 0; j < 16 * G; ++j) top = max(top, __float_as_uint(x[nb][j]) & 0x7fffffffu);
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = fixed_exp(__uint_as_float(top));
+    const int e = min(126, fixed_exp(__uint_as_float(top)));  // scores of a row below 2^-97 are zero to fp32
     const float up = pow2(e);
     const int from = 8 * t;  // a lane whose g / 2 is this thread's t
 #pragma unroll

@@ -91,10 +91,11 @@ ENVG_DEV void mma_s8u8_zero(int (&d)[4], uint32_t a, uint32_t b0, uint32_t b1) {
 // A fixed-point value as four signed digits to the base 256, one to a byte.
 ENVG_DEV uint32_t digits256(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
 // The power of two e that takes a row's largest magnitude to [2^29, 2^30), where it and all smaller
-// fp32 values down to 2^-6 of it are held exactly (at most 2^126: beyond that only denormals round).
+// fp32 values down to 2^-6 of it are held exactly.  At most 149, which makes every fp32 number an
+// integer: below 2^-120 nothing is rounded at all.
 ENVG_DEV int fixed_exp(float top) {
   const int field = (int)(__float_as_uint(top) >> 23);
-  return field == 255 ? 0 : min(126, 156 - field);
+  return field == 255 ? 0 : min(149, 156 - field);
 }
 ENVG_DEV float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -113,7 +114,9 @@ ENVG_DEV int scale_exp(float top) {
   const int field = (int)(__float_as_uint(top) >> 23);
   return field == 255 ? 0 : min(126, 141 - field);
 }
-ENVG_DEV float pow2(int e) { return __int_as_float((127 + e) << 23); }
+ENVG_DEV float pow2(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
+// 2^-e for the e of fixed_exp: from 127 on a denormal, which holds it exactly.
+ENVG_DEV float fixed_unit(int e) { return e <= 126 ? pow2(-e) : __int_as_float(1 << (149 - e)); }
 
 // n / d for 0 <= n < 2^32 by a multiplication (Granlund and Montgomery, PLDI 1994).
 struct FastDiv {

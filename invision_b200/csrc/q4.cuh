@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC;
       if (kb >= kbn) break;
-      const float4 v = in[u];
+      float4 v = in[u];
       // magnitudes as integers order as floats do, and keep a NaN on top
       uint32_t top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
                          max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
@@ -269,7 +269,11 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         if (lane == 0) xs[kb * MC + m] = top >= 0x7f800000u ? nan : pow2(-e);
       } else {
         const int e = fixed_exp(__uint_as_float(top));
-        const float up = pow2(e);
+        float up = pow2(e), wt = pow2(-e);
+        if (e > 126) {  // a row near fp32's end: in two exact steps, and its unit may be a denormal
+          up = pow2(e - 23), wt = fixed_unit(e);
+          v = make_float4(v.x * 8388608.0f, v.y * 8388608.0f, v.z * 8388608.0f, v.w * 8388608.0f);
+        }
         const uint32_t x0 = digits256(__float2int_rn(v.x * up)), x1 = digits256(__float2int_rn(v.y * up));
         const uint32_t x2 = digits256(__float2int_rn(v.z * up)), x3 = digits256(__float2int_rn(v.w * up));
         // A word's columns go in as (0, 2, 4, 6) and (1, 3, 5, 7); lanes 2 i and 2 i + 1 hold columns
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         uint2* out = reinterpret_cast<uint2*>(xf + (((((kb * 2 + (word >> 1)) * MC + m) * 4 + (odd ? 2 : 0)) * 4 + tt) * 2 + (word & 1)) * 8);
         out[0] = make_uint2(__byte_perm(lo0, hi0, 0x5410), __byte_perm(lo1, hi1, 0x5410));
         out[8] = make_uint2(__byte_perm(lo0, hi0, 0x7632), __byte_perm(lo1, hi1, 0x7632));
-        if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? nan : pow2(-e)) * (lane ? 65536.0f : 1.0f);
+        if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? nan : wt) * (lane ? 65536.0f : 1.0f);
       }
     }
   }

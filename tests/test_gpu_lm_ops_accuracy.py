@@ -78,3 +78,24 @@ def test_attention_kv4_seen_nan_comes_through_beside_large_scores(gpu, n, q_len,
             assert np.isfinite(out[..., :64]).all() and np.isnan(out[..., 64:]).all(), (at, big)
         else:
             assert np.isnan(out).all(), (at, big)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 6, 12])
+@pytest.mark.parametrize("size", [1e-25, 1e-30, 1e-33, 1e-36, 3e-38, 1e-40, 1e-43])
+def test_linear_q4_keeps_tiny_rows(gpu, M, size):
+    """Rows whose largest value is near fp32's smallest normal number, or below it, against large
+    scales: x is what fp32 holds, and no bit of it is lost.  One row of ordinary size beside them."""
+    K, N, group = 640, 48, 64
+    rng = np.random.default_rng(M)
+    codes = rng.integers(0, 256, (N, K // 2), dtype=np.uint8)
+    z = rng.integers(0, 16, (N, K // group), dtype=np.uint8)
+    scales = (1e27 * (0.2 + rng.random((N, K // group)))).astype(np.float32)
+    x = (size * rng.standard_normal((M, K))).astype(np.float32)
+    if M > 1:
+        x[M // 2] = rng.standard_normal(K).astype(np.float32)
+    y = np.zeros((M, N), np.float32)
+    gpu.linear_q4(y, x, gpu.Q4Weight(codes, scales, z, K=K, group=group))
+    ref, tol = R.linear(x, R.q4_weight(codes, scales, z, K, group), groups=K // group)
+    assert np.isfinite(y).all()
+    for r in range(M):
+        assert (np.abs(y[r] - ref[r]) <= tol[r]).all() and R.rel(y[r], ref[r]) <= 3e-6, (r, R.rel(y[r], ref[r]))
