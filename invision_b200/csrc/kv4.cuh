@@ -334,7 +334,7 @@ struct KvAttnArgs {
 // tensor cores as 8-bit integer m16n8k32 products, whose 32-bit sums are exact.  The codes are the
 // unsigned 16-row operand (16 tokens of K, 16 channels of V^T), four of them unpacked by one or two
 // logic operations, once for all rows.  The other factor is the 8-column one, a fixed-point number
-// cut into digits to the base 256: q with 31 bits of its row's largest value in four signed
+// cut into digits to the base 256: q with 31 bits of its group's largest value in four signed
 // digits (two products of two adjacent columns a row), p s with 22 bits of its group's largest in the
 // unit in three unsigned ones.  A thread joins its digits' sums, which are one row's, in integers and
 // converts once.  The c - 8 of the output comes from a start of the sums at -8 sum(p s), itself a
@@ -456,29 +456,26 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
   // q: columns g of the two operands are digits g % 2 and 2 + g % 2 of row g / 2, in the order of
   // the K words' nibbles; a thread's scores are those of row t
   uint32_t qb[NB][2 * G][2][2];
-  float qs[NB][G], cq[NB];
+  float qs[NB][G], cq[NB][G];
   int pos[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 16 * G; ++j) top = max(top, __float_as_uint(x[nb][j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = min(126, fixed_exp(__uint_as_float(top)));  // scores of a row below 2^-97 are zero to fp32
-    const float up = pow2(e);
     const int from = 8 * t;  // a lane whose g / 2 is this thread's t
+    float up[G];
 #pragma unroll
-    for (int gi = 0; gi < G; ++gi) {
+    for (int gi = 0; gi < G; ++gi) {  // each group has a unit of its own, as its scores have a scale of their own
+      uint32_t top = 0;
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += x[nb][16 * gi + j];
+      for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(x[nb][16 * gi + j]) & 0x7fffffffu), sum += x[nb][16 * gi + j];
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o)), sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int e = min(126, fixed_exp(__uint_as_float(top)));  // scores of a row below 2^-97 are zero to fp32
+      up[gi] = pow2(e);
       qs[nb][gi] = __shfl_sync(0xffffffffu, sum, from) * a.sl2;
+      // a row with an infinity or a NaN gives NaN
+      cq[nb][gi] = __shfl_sync(0xffffffffu, top >= 0x7f800000u ? __int_as_float(0x7fc00000) : pow2(-e), from) * a.sl2;
     }
-    // a row with an infinity or a NaN gives NaN
-    cq[nb] = __shfl_sync(0xffffffffu, top >= 0x7f800000u ? __int_as_float(0x7fc00000) : pow2(-e), from) * a.sl2;
     const int mr = row0 + 4 * nb + t;
     pos[nb] = mr < rows ? len - a.q_len + mr / per_kv : -1;
     const uint32_t pick[2] = {(g & 1) ? 0x0051u : 0x0040u, (g & 1) ? 0x0073u : 0x0062u};
@@ -486,7 +483,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
     for (int w = 0; w < 2 * G; ++w) {
       uint32_t d[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = digits256(__float2int_rn(x[nb][8 * w + j] * up));
+      for (int j = 0; j < 8; ++j) d[j] = digits256(__float2int_rn(x[nb][8 * w + j] * up[w / 2]));
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -547,9 +544,13 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
           kw[i][0] = k2.x, kw[i][1] = k2.y;
         }
       }
-      float mn[NB][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) x[nb][tt][0] = x[nb][tt][1] = mn[nb][0] = mn[nb][1] = 0.0f;
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[nb][tt][i] = qs[nb][0] * km[i][0];
+          if (G == 2) x[nb][tt][i] = fmaf(qs[nb][G - 1], km[i][G - 1], x[nb][tt][i]);
+        }
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         int d[NB][2][4];
@@ -570,14 +571,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NB == 1 ? 4 : 3) k_kv4_attn(const
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float dot = fmaf((float)(d[nb][1][2 * i + 1] * 256 + d[nb][1][2 * i]), 65536.0f, (float)(d[nb][0][2 * i + 1] * 256 + d[nb][0][2 * i]));
-            x[nb][tt][i] = fmaf(dot, ks[i][gi], x[nb][tt][i]);
-            mn[nb][i] = fmaf(qs[nb][gi], km[i][gi], mn[nb][i]);
+            x[nb][tt][i] = fmaf(dot * cq[nb][gi], ks[i][gi], x[nb][tt][i]);
           }
       }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) x[nb][tt][i] = fmaf(x[nb][tt][i], cq[nb], mn[nb][i]);
     }
     // masks: only where a row of the CTA does not see the whole unit.  A row hides a token by its
     // score; its scale and minimum are dropped where no row sees it (they may hold anything there).

@@ -99,3 +99,26 @@ def test_linear_q4_keeps_tiny_rows(gpu, M, size):
     assert np.isfinite(y).all()
     for r in range(M):
         assert (np.abs(y[r] - ref[r]) <= tol[r]).all() and R.rel(y[r], ref[r]) <= 3e-6, (r, R.rel(y[r], ref[r]))
+
+
+@pytest.mark.parametrize("ratio", [1e2, 1e-3, 1e4, 1e-5, 1e6])
+@pytest.mark.parametrize("lens,q_len,H,KVH,window,sinks", [([700, 333], 1, 8, 2, 0, 0), ([700, 333], 1, 16, 2, 0, 0),
+                                                           ([400], 5, 4, 2, 100, 7)])
+def test_attention_kv4_query_groups_of_different_size(gpu, lens, q_len, H, KVH, window, sinks, ratio):
+    """Channels 0..63 and 64..127 of q differ in size by `ratio`, those of K the other way, so that both
+    count alike in a score: each keeps its own precision."""
+    hd = 128
+    rng = np.random.default_rng(H + q_len)
+    size = np.repeat([ratio ** 0.5, ratio ** -0.5], 64).astype(np.float32)
+    k = [rng.standard_normal((n, KVH, hd)).astype(np.float32) / size for n in lens]
+    v = [rng.standard_normal((n, KVH, hd)).astype(np.float32) for n in lens]
+    c, table = _fill(gpu, rng, lens, 16, k, v)
+    q = (rng.standard_normal((len(lens) * q_len, H, hd)).astype(np.float32) * size).reshape(-1, H * hd)
+    out = np.full_like(q, np.nan)
+    gpu.attention_kv4(out, q, c, table, np.asarray(lens, np.int32), H, q_len=q_len, window=window, sinks=sinks)
+    for b, n in enumerate(lens):
+        rows = slice(b * q_len, (b + 1) * q_len)
+        ref = R.attention_exact(q[rows].reshape(q_len, H, hd), R.kv_hold(k[b]), R.kv_hold(v[b]), n - q_len + np.arange(q_len),
+                                window, sinks, hd ** -0.5)
+        got = out[rows].reshape(q_len, H, hd)
+        assert R.rel(got, ref) <= REL_GROUP, (b, ratio, R.rel(got, ref))
