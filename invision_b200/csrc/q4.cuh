@@ -112,14 +112,15 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
 // the 16-row operand of the tensor cores' products, x the 8-column one, in as many parts as fp32
 // accuracy takes; a group's sum starts from zero and is multiplied by its scale in fp32.  Two forms:
 //   integers (HALF false): codes as unsigned bytes (two logic operations unpack four), x per (row,
-//     block) as a 31-bit fixed-point number in four signed digits to the base 256, a row's digits in
-//     four adjacent columns, two rows to a product.  The 32-bit sums are exact; a thread joins its two
-//     digits, takes off z sum(x) in integers, converts once; a row's two threads are added when the
+//     scale group) as a 31-bit fixed-point number in four signed digits to the base 256, a row's digits
+//     in four adjacent columns, two rows to a product.  The 32-bit sums are exact; a thread joins its
+//     two digits, takes off z sum(x) in integers, converts once; a row's two threads are added when the
 //     tile is left.
 //   halves (HALF true): c - z exact as an fp16 (put into the mantissa of 1024, then one subtraction
 //     or multiply-add; a bare c would be a subnormal, which the cores align by its nominal exponent
 //     and so lose up to ten low bits of x), x in two fp16 parts in adjacent columns, scaled by a power
-//     of two per (row, block), four rows to a product.
+//     of two per (row, block), four rows to a product.  The low part is held 2^11 larger: values down to
+//     2^-29 of the block's largest keep their 22 bits, down to 2^-18 without it.
 // The integer form unpacks a block in 24 operations against 72, the other form spends 4 per group on
 // four rows against 18; the kernel is bound by instruction issue before it is by HBM, so few rows
 // take integers and many rows halves.  Measured, us (integers / halves): 1 x 2560 x 19456, groups of
@@ -155,9 +156,9 @@ struct Q4Smem {
   static constexpr int RECV = R * SUMS;         // [ranks][tiles of the owner], used by clusters
   static constexpr int FIXED = SLOTS + RECV + R * 8;  // and each tile's first and last warp
   static constexpr int X_ROW = 4 * Q4_COLS;     // bytes of x's parts per (row, block)
-  // parts and their weights (one, or one to a pair of digits), digits' sums per group and pair
+  // parts and their weight, or digits with their sum and weight per scale group and pair of digits
   __host__ __device__ static int x_bytes(int kb, int group) {
-    return (int)((kb * MC * (X_ROW + (HALF ? 4 : 8 + 8 * (Q4_COLS / group))) + 15) & ~15);
+    return (int)((kb * MC * (X_ROW + (HALF ? 4 : 16 * (Q4_COLS / group))) + 15) & ~15);
   }
   __host__ __device__ static int total(int kb, int stages, int group) {
     return FIXED + x_bytes(kb, group) + Q4_WARPS * stages * q4_block_bytes(group);
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   int2* ends = reinterpret_cast<int2*>(smem + S::SLOTS + S::RECV);
   // integers: [kb][word pair][row][digit][t][word] 8 bytes; halves: [kb][word][row][part][t] 16 bytes
   uint8_t* xf = smem + S::FIXED;
-  float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // weights: [kb][row][digit pair], [kb][row]
-  int* xt = reinterpret_cast<int*>(xs + p.kb_per * MC * 2);             // sums of digits: [kb][group][row][digit pair]
+  float* xs = reinterpret_cast<float*>(xf + p.kb_per * MC * S::X_ROW);  // halves: weights [kb][row]
+  int2* xt = reinterpret_cast<int2*>(xs);  // integers: (sum of digits, weight as a float) [kb][group][row][digit pair]
   uint8_t* ring = xf + S::x_bytes(p.kb_per, GROUP) + warp * p.stages * BLOCK;
 
   const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0, cl = blockIdx.x >> p.log_splits;
@@ -223,13 +224,16 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
   griddep_wait();
   griddep_launch_dependents();
 
-  // x of this K range in parts: a warp takes 128 columns of a row at a time
+  // x of this K range in parts: a warp takes 128 columns of a row at a time.  A single row goes without
+  // its product's second one, which keeps what shared memory holds: a row's columns of the products are
+  // its own, and those are never stored.
   constexpr int AHEAD = 10;  // loads of a warp under way at a time
-  for (int i0 = warp; i0 < kbn * MC; i0 += AHEAD * Q4_WARPS) {
+  const bool one = MC == 2 && mn == 1;
+  for (int i0 = warp; i0 < (one ? kbn : kbn * MC); i0 += AHEAD * Q4_WARPS) {
     float4 in[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC, k = (kb0 + kb) * Q4_COLS + 4 * lane;
+      const int i = i0 + u * Q4_WARPS, kb = one ? i : i / MC, m = one ? 0 : i % MC, k = (kb0 + kb) * Q4_COLS + 4 * lane;
       in[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (kb < kbn && m < mn) {
         const float* src = a.x + (int64_t)(m0 + m) * a.ldx + k;
@@ -244,13 +248,28 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int i = i0 + u * Q4_WARPS, kb = i / MC, m = i % MC;
+      const int i = i0 + u * Q4_WARPS, kb = one ? i : i / MC, m = one ? 0 : i % MC;
       if (kb >= kbn) break;
       float4 v = in[u];
       // magnitudes as integers order as floats do, and keep a NaN on top
       uint32_t top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
                          max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
-      top = __reduce_max_sync(0xffffffffu, top);
+      // integers: the largest of the scale group, whose sums the digits end in; halves: of the block
+      if (HALF || GROUP == 128) {
+        top = __reduce_max_sync(0xffffffffu, top);
+      } else if (GROUP == 32) {
+#pragma unroll
+        for (int o = 1; o < GROUP / 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      } else {
+        uint32_t all = 0;
+#pragma unroll
+        for (int gi = 0; gi < PER; ++gi) {
+          const bool here = lane / (GROUP / 4) == gi;
+          const uint32_t largest = __reduce_max_sync(0xffffffffu, here ? top : 0u);
+          if (here) all = largest;
+        }
+        top = all;
+      }
       const bool odd = lane & 1;
       const int word = lane >> 3, tt = (lane >> 1) & 3;
       const float nan = __int_as_float(0x7fc00000);  // an infinity or a NaN makes its row's outputs NaN
@@ -259,7 +278,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         const float up = pow2(e), y0 = v.x * up, y1 = v.y * up, y2 = v.z * up, y3 = v.w * up;
         const __half2 h0 = __floats2half2_rn(y0, y1), h1 = __floats2half2_rn(y2, y3);
         const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-        const uint32_t l0 = h2_bits(__floats2half2_rn(y0 - b0.x, y1 - b0.y)), l1 = h2_bits(__floats2half2_rn(y2 - b1.x, y3 - b1.y));
+        const uint32_t l0 = h2_bits(__floats2half2_rn((y0 - b0.x) * 2048.0f, (y1 - b0.y) * 2048.0f));
+        const uint32_t l1 = h2_bits(__floats2half2_rn((y2 - b1.x) * 2048.0f, (y3 - b1.y) * 2048.0f));
         // lanes 2 i and 2 i + 1 hold nibbles 0..3 and 4..7 of a word: the even lane collects the high
         // parts, the odd one the low parts, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
         const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h0) : l0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? h2_bits(h1) : l1, 1);
@@ -285,7 +305,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
         uint2* out = reinterpret_cast<uint2*>(xf + (((((kb * 2 + (word >> 1)) * MC + m) * 4 + (odd ? 2 : 0)) * 4 + tt) * 2 + (word & 1)) * 8);
         out[0] = make_uint2(__byte_perm(lo0, hi0, 0x5410), __byte_perm(lo1, hi1, 0x5410));
         out[8] = make_uint2(__byte_perm(lo0, hi0, 0x7632), __byte_perm(lo1, hi1, 0x7632));
-        if (lane < 2) xs[(kb * MC + m) * 2 + lane] = (top >= 0x7f800000u ? nan : wt) * (lane ? 65536.0f : 1.0f);
+        const int gi = lane / (GROUP / 4), pair = lane % (GROUP / 4);
+        if (pair < 2) xt[((kb * PER + gi) * MC + m) * 2 + pair].y = __float_as_int((top >= 0x7f800000u ? nan : wt) * (pair ? 65536.0f : 1.0f));
       }
     }
   }
@@ -302,7 +323,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
           const uint2 b = *reinterpret_cast<const uint2*>(xf + ((((kb * 2 + (w >> 1)) * MC + 2 * nt) * 4 + g) * 8 + t * 2 + (w & 1)) * 8);
           if (w % (4 / PER) == 0) mma_u8s8<true>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
           else mma_u8s8<false>(d, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, b.x, b.y);
-          if (w % (4 / PER) == 4 / PER - 1 && g == 0) xt[((kb * PER + w / (4 / PER)) * MC + 2 * nt) * 2 + t] = d[1] * 256 + d[0];
+          if (w % (4 / PER) == 4 / PER - 1 && g == 0) xt[((kb * PER + w / (4 / PER)) * MC + 2 * nt) * 2 + t].x = d[1] * 256 + d[0];
         }
       }
     __syncthreads();
@@ -323,8 +344,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
     int row = min(more, (j + 1) * kbn - i);  // of them in this tile
     int kb = i - j * kbn;
     const uint8_t* xk = xf + kb * (MC * S::X_ROW) + lane * 16;
-    const int* xtk = xt + kb * (PER * MC * 2) + t;
-    const float* xsk = xs + kb * (HALF ? MC : MC * 2) + t;
+    const int2* xtk = xt + kb * (PER * MC * 2) + t;
+    const float* xsk = xs + kb * MC + t;
     float acc[NT][2] = {};
     for (; more > 0; --more) {
       if (p.stages == 6) copy_groups_wait<5>();
@@ -334,8 +355,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
       const uint8_t* blk = ring + at;
       const uint4 q0 = *reinterpret_cast<const uint4*>(blk + lane * 16), q1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
       const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w}, w1[4] = {q1.x, q1.y, q1.z, q1.w};
-      float sum[NT][2] = {};
       if constexpr (HALF) {
+        float sum[NT][2] = {};
 #pragma unroll
         for (int gi = 0; gi < PER; ++gi) {
           const float s0 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g) * 4), s1 = *reinterpret_cast<const float*>(blk + 1024 + (gi * 16 + g + 8) * 4);
@@ -369,10 +390,16 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
-              float v = d[0][nt][2 * i2] + d[0][nt][2 * i2 + 1];
-              if (PER < 4) v += d[1][nt][2 * i2] + d[1][nt][2 * i2 + 1];
-              sum[nt][i2] = fmaf(v, i2 ? s1 : s0, sum[nt][i2]);
+              float high = d[0][nt][2 * i2], low = d[0][nt][2 * i2 + 1];
+              if (PER < 4) high += d[1][nt][2 * i2], low += d[1][nt][2 * i2 + 1];
+              sum[nt][i2] = fmaf(fmaf(low, 1.0f / 2048.0f, high), i2 ? s1 : s0, sum[nt][i2]);
             }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float wt = xsk[4 * nt];
+          acc[nt][0] = fmaf(sum[nt][0], wt, acc[nt][0]);
+          acc[nt][1] = fmaf(sum[nt][1], wt, acc[nt][1]);
         }
       } else {
         int d[NT][4];
@@ -395,24 +422,19 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) k_q4(const Q4Args a, const Q4Pl
             const int z0 = blk[1024 + 64 * PER + gi * 16 + g], z1 = blk[1024 + 64 * PER + gi * 16 + g + 8];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const int xsum = xtk[(gi * MC + 2 * nt) * 2];
-              sum[nt][0] = fmaf((float)(d[nt][1] * 256 + d[nt][0] - z0 * xsum), s0, sum[nt][0]);
-              sum[nt][1] = fmaf((float)(d[nt][3] * 256 + d[nt][2] - z1 * xsum), s1, sum[nt][1]);
+              const int2 xw = xtk[(gi * MC + 2 * nt) * 2];
+              const float wt = __int_as_float(xw.y);
+              acc[nt][0] = fmaf((float)(d[nt][1] * 256 + d[nt][0] - z0 * xw.x) * s0, wt, acc[nt][0]);
+              acc[nt][1] = fmaf((float)(d[nt][3] * 256 + d[nt][2] - z1 * xw.x) * s1, wt, acc[nt][1]);
             }
           }
         }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float wt = xsk[4 * nt];
-        acc[nt][0] = fmaf(sum[nt][0], wt, acc[nt][0]);
-        acc[nt][1] = fmaf(sum[nt][1], wt, acc[nt][1]);
       }
       __syncwarp();  // every lane has read the stage
       fetch(at);
       at += BLOCK;
       if (at == stage_end) at = 0;
-      xk += MC * S::X_ROW, xtk += PER * MC * 2, xsk += HALF ? MC : MC * 2;
+      xk += MC * S::X_ROW, xtk += PER * MC * 2, xsk += MC;
       if (--row == 0) {  // the warp leaves the tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {

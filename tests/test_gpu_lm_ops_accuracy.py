@@ -122,3 +122,24 @@ def test_attention_kv4_query_groups_of_different_size(gpu, lens, q_len, H, KVH, 
                                 window, sinks, hd ** -0.5)
         got = out[rows].reshape(q_len, H, hd)
         assert R.rel(got, ref) <= REL_GROUP, (b, ratio, R.rel(got, ref))
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 6, 12])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e8])
+def test_linear_q4_groups_of_different_size(gpu, M, group, ratio):
+    """x differs in size between the scale groups of a row, the scales the other way, so that all groups
+    count alike: each keeps its own precision."""
+    K, N = 1000, 40
+    rng = np.random.default_rng(M + group)
+    codes, scales, z = (rng.integers(0, 256, (N, K // 2), dtype=np.uint8),
+                        (0.01 * (0.2 + rng.random((N, -(-K // group))))).astype(np.float32),
+                        rng.integers(0, 16, (N, -(-K // group)), dtype=np.uint8))
+    size = ratio ** rng.choice([-0.5, 0.0, 0.5], scales.shape[1])
+    scales = (scales / size).astype(np.float32)
+    x = (rng.standard_normal((M, K)) * np.repeat(size, group)[:K]).astype(np.float32)
+    y = np.zeros((M, N), np.float32)
+    gpu.linear_q4(y, x, gpu.Q4Weight(codes, scales, z, K=K, group=group))
+    ref, tol = R.linear(x, R.q4_weight(codes, scales, z, K, group), groups=-(-K // group))
+    for r in range(M):
+        assert (np.abs(y[r] - ref[r]) <= tol[r]).all() and R.rel(y[r], ref[r]) <= 3e-6, (r, R.rel(y[r], ref[r]))
