@@ -681,6 +681,8 @@ def _matrix(a, rows, cols, name, mode, dtype="float32"):
     if len(shape) != 2 or shape[0] != rows or shape[1] < cols:
         raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(shape)}")
     if host:
+        if rows > 1 and a.strides[0] % a.itemsize:
+            raise TypeError(f"{name}: rows {a.strides[0]} bytes apart, not a multiple of the element size")
         st, ptr = [s // a.itemsize for s in a.strides], a.ctypes.data
     else:
         st, ptr = a.stride(), a.data_ptr()

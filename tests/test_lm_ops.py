@@ -177,3 +177,18 @@ def test_operands_of_several_devices_are_refused(monkeypatch):
     refuse = envg.ERR_ARG  # the library runs on another device
     assert envg._views.call(at, use_at, 3, "M", a, 2, 4) == envg.ERR_ARG
     assert calls == [(0, 0, None)]
+
+
+@pytest.mark.parametrize("extra", [1, 2, 3])
+def test_rows_at_odd_byte_distances_are_refused(extra):
+    """Rows of a packed record: their distance in bytes is no multiple of an element, and a stride in
+    elements would name other memory."""
+    records = np.zeros(5, np.dtype([("x", np.float32, (8,)), ("tag", np.uint8, (extra,))]))
+    assert records["x"].shape == (5, 8) and records["x"].strides == (32 + extra, 4)
+    with pytest.raises(TypeError, match="x: rows .* bytes apart"):
+        envg._matrix(records["x"], 5, 8, "x", envg.HOST_PTRS)
+    with pytest.raises(TypeError):
+        envg._packed(records["x"], 5, 8, "x", envg.HOST_PTRS)
+    assert envg._matrix(records["x"][:1], 1, 8, "x", envg.HOST_PTRS)[1] == 8
+    padded = np.zeros(5, np.dtype([("x", np.float32, (8,)), ("tag", np.uint8, (4,))]))
+    assert envg._matrix(padded["x"], 5, 8, "x", envg.HOST_PTRS)[1] == 9
