@@ -362,10 +362,12 @@ int envg_weight_upload_q4(const uint8_t* codes, const float* scales, const uint8
 int envg_q4weight_free(envg_q4weight w);
 
 /* dst = epilogue(x . W^T) for a 4-bit weight, epilogues as envg_linear; x [M, K] of row stride
- * ldx, dst [M, N] (N / 2 for ENVG_EPI_SILU_GATE) of row stride ldd.  The product is an fp32 one:
- * codes are exact in the tensor cores' 16-bit operands, x is carried as two of them, scales are
- * applied to the fp32 sums of their groups (about 1e-7 relative).  Made for few rows (M up to
- * about 64); 0 <= M <= 65535.  A row of x that holds an infinity or a NaN gives non-finite
+ * ldx, dst [M, N] (N / 2 for ENVG_EPI_SILU_GATE) of row stride ldd.  Codes are exact in the tensor
+ * cores' operands and scales are applied to the sums of their groups in fp32.  x is carried, with 1
+ * to 4 rows, as fixed-point numbers in four 8-bit digits, to 2^-30 of the largest value of its scale
+ * group; with more rows in two 16-bit parts, to 2^-22 of each value (and no finer than 2^-50 of the
+ * largest of 128 columns).  Together about 1e-7 relative to the sum of |x| |w|.  Made for few rows:
+ * from 32 on envg_linear on 16-bit weights takes less time; 0 <= M <= 65535.  A row of x that holds an infinity or a NaN gives non-finite
  * outputs in that row.  dst must not overlap x.  The matrices of this and the following calls are
  * many, so each call takes them in a structure. */
 typedef struct envg_linear_q4_args {
@@ -443,8 +445,10 @@ int envg_kv4_read(const envg_kv4_rows* rows, int flags);
  * row b * q_len + i of q and dst ([batch * q_len, heads * head_dim]) stands at position
  * p = ctx_lens[b] - q_len + i and sees the cached tokens j <= p; with window > 0 only those with
  * j > p - window or j < sinks (the first tokens stay visible).  Head h reads kv head
- * h / (heads / kv_heads).  dst = softmax(scale * q . k) . v in fp32 (about 1e-6 relative); a row
- * that sees nothing is zeros.  max_ctx is the largest of ctx_lens where the caller knows it, or 0:
+ * h / (heads / kv_heads).  dst = softmax(scale * q . k) . v; sums and softmax statistics are fp32, q
+ * is held to 2^-30 of the largest of its 64-channel group, the products of softmax weights and V's
+ * scales to 2^-22 of the largest of 32 tokens and a group (about 1e-6 relative in each group).  A row
+ * that sees nothing is zeros, a NaN that is seen comes through whatever its weight.  max_ctx is the largest of ctx_lens where the caller knows it, or 0:
  * it only plans how the work is split.  dst must not overlap q. */
 typedef struct envg_attention_kv4_args {
   float* dst;

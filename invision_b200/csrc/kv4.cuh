@@ -347,10 +347,16 @@ struct KvAttnArgs {
 // with its own ring of bulk copies; the warps' (max, sum, output) are joined in shared memory, the
 // CTAs' through distributed shared memory in rank order: no workspace, no atomics, one launch.
 //
-// Bound: instruction issue in the loop (about 440 instructions a unit and warp for four rows, 70% of
-// the slots at four CTAs per SM), start and join around it (6 us alone).  Measured: 16 sequences of
-// 8192 to 16384 tokens, 32 / 8 heads of 128: 55 us, 4.2 TB/s; fp16 operands with q and p s in two
-// parts took 68 (9 operations to unpack 8 codes against 3).
+// Rounding.  Both fixed-point numbers are relative to the largest of one group of 64 channels, whose
+// sums are the only ones they enter: q to 2^-30 of it, p s to 2^-22, where a step of V's own codes is
+// a fifteenth of the group's span.  One unit for both groups of a 128-channel head lost log2 R bits in
+// a group R times smaller.
+//
+// Bound: the chain of dependent steps of each warp (about 455 instructions a unit and warp for four
+// rows; with four CTAs per SM, as many as registers allow, issue slots are 56% busy, DRAM 47%, the
+// tensor pipe 26%), and start and join around it (6 us alone, a quarter of the instructions below).
+// Measured: 16 sequences of 8192 to 16384 tokens, 32 / 8 heads of 128: 55 to 58 us, 4.1 TB/s; fp16
+// operands with q and p s in two parts took 68 (9 operations to unpack 8 codes against 3).
 constexpr int KVA_WARPS = 4, KVA_THREADS = 32 * KVA_WARPS, KVA_STAGES = 2;
 constexpr int SITE_KVA_RING = 60;  // status[1] of a ring wait that ran out
 

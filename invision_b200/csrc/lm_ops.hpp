@@ -327,8 +327,8 @@ int kv4_rows(const envg_kv4_rows* r, int flags, bool read) {
 // CTAs that share one (sequence, kv head, row tile), a power of two up to 8 (the portable cluster).
 // A CTA costs about as much as eight units of two tiles a warp, so a GPU that is full takes more
 // CTAs only while they keep that (measured, us: 16 sequences of 8192 to 16384 tokens, 128 groups:
-// 122 / 75 / 65 / 59 at 1 / 2 / 4 / 8; 32 windows of 1024, 256 groups: 16.4 / 18 / 24 / 37); one that
-// is not takes them down to one unit a warp (512 tokens, 8 groups: 6.9 / 6.4 / 5.6 / 5.9).
+// 119 / 72 / 63 / 57 at 1 / 2 / 4 / 8; 32 windows of 1024, 256 groups: 15.1 / 15.7 / 22 / 34); one that
+// is not takes them down to one unit a warp (512 tokens, 8 groups: 7.0 / 6.9 / 6.0 / 6.0).
 int kv4_splits(Dev* d, int64_t groups, int64_t tokens) {
   const int64_t units = cdiv(tokens, 2 * KV_TILE);
   int s = 1;

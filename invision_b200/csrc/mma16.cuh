@@ -1,10 +1,10 @@
 // mma16.cuh -- warp-level pieces that the 4-bit kernels share: m16n8k16 products with fp16 operands
-// and fp32 sums, m16n8k32 products of bytes with 32-bit sums, an 8 x 8 transpose in registers, unpacking, untiled bulk copies and reads of a
-// cluster's shared memory.
+// and fp32 sums, m16n8k32 products of bytes with 32-bit sums, an 8 x 8 transpose in registers,
+// unpacking, untiled bulk copies and reads of a cluster's shared memory.
 //
 // mma.sync rather than tcgen05: a code has to be unpacked in registers and its group's scale has to
-// meet the fp32 sum of that group alone, so both operands and accumulators live in registers; the
-// tensor pipe is a fifth busy when these kernels stream from HBM.
+// meet the fp32 sum of that group alone, so both operands and accumulators live in registers.  The
+// tensor pipe is 23 to 26% busy in the linear and in long decodes, 36% in a chunk of 128 queries.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -32,6 +32,7 @@ ENVG_DEV uint32_t transpose_8x8(uint32_t v) {
 }
 ENVG_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 ENVG_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// 2^x for softmax weights: within about 2^-22, and 0 where it would be a denormal.
 ENVG_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

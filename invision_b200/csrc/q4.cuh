@@ -120,13 +120,13 @@ ENVG_DEV void q4_store(const Q4Args& a, int64_t tile, int r, int m, float v0, fl
 //     or multiply-add; a bare c would be a subnormal, which the cores align by its nominal exponent
 //     and so lose up to ten low bits of x), x in two fp16 parts in adjacent columns, scaled by a power
 //     of two per (row, block), four rows to a product.  The low part is held 2^11 larger: values down to
-//     2^-29 of the block's largest keep their 22 bits, down to 2^-18 without it.
+//     2^-28 of the block's largest keep their 22 bits, down to 2^-17 without it.
 // The integer form unpacks a block in 24 operations against 72, the other form spends 4 per group on
-// four rows against 18; the kernel is bound by instruction issue before it is by HBM, so few rows
-// take integers and many rows halves.  Measured, us (integers / halves): 1 x 2560 x 19456, groups of
-// 64: 7.9 / 13.2; 4 x 4096 x 36864, groups of 128: 20.1 / 28.2 (4.0 TB/s; one row: 17.4, 4.6 TB/s,
-// and 6.5 TB/s for every block past the first wave); 4 x 9728 x 2560, groups of 32: 9.6 / 10.2;
-// 16 x 9728 x 2560, groups of 32: 20.0 / 14.1.
+// four rows against 22; the kernel is bound by its warps' own steps (16 warps an SM, issue slots 54%
+// busy, DRAM 40%), so few rows take integers and many rows halves.  Measured, us (integers / halves):
+// 1 x 2560 x 19456, groups of 64: 7.9 / 13.7; 4 x 4096 x 36864, groups of 128: 20.4 / 28.1 (4.0 TB/s);
+// 4 x 9728 x 2560, groups of 32: 9.9 / 10.2; 16 x 9728 x 2560, groups of 32: 21.8 / 14.4.  These
+// weights stay in L2 from call to call; from HBM the first takes 1.2 us more, the second 1.0.
 //
 // Split.  A cluster of CTAs (one CTA of 16 warps per SM) takes a run of row tiles, each CTA a range
 // of K, as many CTAs as fill the GPU when there are few tiles.  Up to R tiles at a time, the CTA's
