@@ -115,7 +115,7 @@ ENVG_DEV int scale_exp(float top) {
   const int field = (int)(__float_as_uint(top) >> 23);
   return field == 255 ? 0 : min(126, 141 - field);
 }
-ENVG_DEV float pow2(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
+ENVG_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 // 2^-e for the e of fixed_exp: from 127 on a denormal, which holds it exactly.
 ENVG_DEV float fixed_unit(int e) { return e <= 126 ? pow2(-e) : __int_as_float(1 << (149 - e)); }
 
