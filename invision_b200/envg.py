@@ -666,7 +666,7 @@ def _on_side(a, mode, name):
     return host
 
 
-def _matrix(a, rows, cols, name, mode, dtype="float32"):
+def _matrix(a, rows, cols, name, mode, dtype="float32", write=False):
     """(pointer, row stride in elements) of a 2-D array [rows, >= cols] whose columns are adjacent."""
     if a is None:
         return 0, 0
@@ -681,6 +681,8 @@ def _matrix(a, rows, cols, name, mode, dtype="float32"):
     if len(shape) != 2 or shape[0] != rows or shape[1] < cols:
         raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(shape)}")
     if host:
+        if write and not a.flags.writeable:
+            raise ValueError(f"{name}: the array is read-only")
         if rows > 1 and a.strides[0] % a.itemsize:
             raise TypeError(f"{name}: rows {a.strides[0]} bytes apart, not a multiple of the element size")
         st, ptr = [s // a.itemsize for s in a.strides], a.ctypes.data
@@ -787,7 +789,7 @@ def linear_q4(dst, x, W, bias=None, epilogue=None, gate=None, sync=True):
     px, ldx = _matrix(x, M, W.K, "x", mode)
     if x.shape[1] != W.K:
         raise ValueError(f"x: expected {W.K} columns, got {x.shape[1]}")
-    py, ldd = _matrix(dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, "dst", mode)
+    py, ldd = _matrix(dst, M, N // 2 if W.layout == LAYOUT_GATE_UP else N, "dst", mode, write=True)
     return _check(lib().envg_linear_q4(
         _LINEAR_Q4.pack(py, ldd, px, ldx, _handle(W), _vector(bias, N, "bias", mode), _vector(gate, N, "gate", mode), M,
                         W.K, N, epilogue), _flags(mode, sync)))
@@ -811,7 +813,7 @@ def qk_norm_rope(q_dst, k_dst, q, k, q_weight, k_weight, cos, sin, heads, kv_hea
     T, wq, wk, half = first.shape[0], heads * head_dim, kv_heads * head_dim, head_dim // 2
     rows = cos.shape[0] if cos is not None else 0
     return _check(lib().envg_qk_norm_rope(
-        _QK_NORM_ROPE.pack(*_matrix(q_dst, T, wq, "q_dst", mode), *_matrix(k_dst, T, wk, "k_dst", mode),
+        _QK_NORM_ROPE.pack(*_matrix(q_dst, T, wq, "q_dst", mode, write=True), *_matrix(k_dst, T, wk, "k_dst", mode, write=True),
                            *_matrix(q, T, wq, "q", mode), *_matrix(k, T, wk, "k", mode),
                            _vector(q_weight, head_dim, "q_weight", mode), _vector(k_weight, head_dim, "k_weight", mode),
                            _packed(cos, rows, half, "cos", mode), _packed(sin, rows, half, "sin", mode), rows,
@@ -848,9 +850,10 @@ class KV4Cache:
                 return OK
         mode = _side(k)
         B, width = ctx_lens.shape[0], self.kv_heads * self.head_dim
-        return _check(getattr(lib(), name)(_KV4_ROWS.pack(_handle(self), *_matrix(k, B * q_len, width, "k", mode),
-                                          *_matrix(v, B * q_len, width, "v", mode), *_table(table, ctx_lens, B, mode),
-                                          B, q_len), _flags(mode, sync)))
+        read = name == "envg_kv4_read"
+        return _check(getattr(lib(), name)(_KV4_ROWS.pack(_handle(self), *_matrix(k, B * q_len, width, "k", mode, write=read),
+                                          *_matrix(v, B * q_len, width, "v", mode, write=read),
+                                          *_table(table, ctx_lens, B, mode), B, q_len), _flags(mode, sync)))
 
     def append(self, k, v, table, ctx_lens, q_len=1, sync=True):
         """Write the newest ``q_len`` tokens of each sequence; k, v [B * q_len, kv_heads * hd]: envg_kv4_append."""
@@ -887,7 +890,7 @@ def attention_kv4(dst, q, cache, table, ctx_lens, heads, q_len=1, max_ctx=0, win
     mode = _side(q)
     B, width = ctx_lens.shape[0], heads * cache.head_dim
     return _check(lib().envg_attention_kv4(
-        _ATTENTION_KV4.pack(*_matrix(dst, B * q_len, width, "dst", mode), *_matrix(q, B * q_len, width, "q", mode),
+        _ATTENTION_KV4.pack(*_matrix(dst, B * q_len, width, "dst", mode, write=True), *_matrix(q, B * q_len, width, "q", mode),
                             _handle(cache), *_table(table, ctx_lens, B, mode), B, q_len, max_ctx, heads, window, sinks,
                             scale), _flags(mode, sync)))
 

@@ -192,3 +192,24 @@ def test_rows_at_odd_byte_distances_are_refused(extra):
     assert envg._matrix(records["x"][:1], 1, 8, "x", envg.HOST_PTRS)[1] == 8
     padded = np.zeros(5, np.dtype([("x", np.float32, (8,)), ("tag", np.uint8, (4,))]))
     assert envg._matrix(padded["x"], 5, 8, "x", envg.HOST_PTRS)[1] == 9
+
+
+def test_read_only_outputs_are_refused():
+    """An output that numpy holds to be read-only (a view of bytes, a file mapped for reading) is refused
+    before any call; the same array is fine as an input."""
+    import types
+
+    ro, rw = np.frombuffer(bytes(4 * 2 * 64), np.float32).reshape(2, 64), np.zeros((2, 64), np.float32)
+    n, table = np.array([2], np.int32), np.zeros((1, 1), np.int32)
+    W = types.SimpleNamespace(N=64, K=64, layout=envg.LAYOUT_PLAIN, h=None)
+    cache = object.__new__(envg.KV4Cache)
+    cache.h, cache.kv_heads, cache.head_dim = None, 1, 64
+    for call in (lambda: envg.linear_q4(ro, rw, W), lambda: envg.qk_norm_rope(ro, None, rw, None, None, None, None, None, 1, 0, 64),
+                 lambda: envg.qk_norm_rope(None, ro, None, rw, None, None, None, None, 0, 1, 64),
+                 lambda: cache.read(ro, rw, table, n, q_len=2), lambda: cache.read(rw, ro, table, n, q_len=2),
+                 lambda: envg.attention_kv4(ro, rw, cache, table, n, 1, q_len=2)):
+        with pytest.raises(ValueError, match="read-only"):
+            call()
+    for call in (lambda: envg.linear_q4(rw, ro, W), lambda: cache.append(ro, ro, table, n, q_len=2)):
+        with pytest.raises(envg.EnvgError):  # as far as the library, which has no weight or cache here
+            call()
