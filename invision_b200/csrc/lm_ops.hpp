@@ -585,6 +585,10 @@ int envg_qk_norm_rope(const envg_qk_norm_rope_args* r, int flags) {
   if ((heads && (!q || !q_dst)) || (kv_heads && (!k || !k_dst))) return fail(ENVG_ERR_ARG, "qk_norm_rope: NULL operand");
   if ((heads && (ldq < wq || ldqd < wq)) || (kv_heads && (ldk < wk || ldkd < wk)))
     return fail(ENVG_ERR_ARG, "qk_norm_rope: a row stride is shorter than its heads x head_dim");
+  // with another stride a token's output would overwrite rows that are still to be read (host pointers: no
+  // matter, the operands are copied)
+  if ((flags & ENVG_DEVICE_PTRS) && tokens > 1 && ((heads && q_dst == q && ldqd != ldq) || (kv_heads && k_dst == k && ldkd != ldk)))
+    return fail(ENVG_ERR_ARG, "qk_norm_rope: in place the row strides have to be equal");
   if (cos_table) {
     if (table_rows <= 0) return fail(ENVG_ERR_ARG, "qk_norm_rope: empty position table");
     if (!positions && (pos0 < 0 || pos0 + tokens > table_rows))

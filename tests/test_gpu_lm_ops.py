@@ -656,3 +656,28 @@ def test_kv4_length_beyond_the_table_leaves_its_sequence_alone(gpu):
             new = R.kv_hold(x.cpu().numpy().reshape(B, 3, KVH, hd)).reshape(B, 3, -1)
             assert np.array_equal(got[[0, 2], 29:], new[[0, 2]])
         before = after
+
+
+def test_qk_norm_rope_in_place_with_another_stride_is_refused(gpu):
+    """On the device the rows of one would be overwritten while they are read; one row, or one stride, is fine."""
+    import torch
+
+    buf = torch.randn(1024, device="cuda")
+    wide, narrow = buf.view(4, 256), buf[:512].view(4, 128)
+    before = buf.clone()
+    for q, k in (((narrow, wide[:, :128]), (None, None)), ((None, None), (wide[:, :128], narrow))):
+        n = [1 if t[0] is not None else 0 for t in (q, k)]
+        with pytest.raises(gpu.EnvgError, match="in place") as e:
+            gpu.qk_norm_rope(q[0], k[0], q[1], k[1], None, None, None, None, *n, 128)
+        assert e.value.code == gpu.ERR_ARG
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    gpu.qk_norm_rope(narrow[:1], None, wide[:1, :128], None, None, None, None, None, 1, 0, 128)
+    gpu.qk_norm_rope(wide[:, 128:], None, wide[:, 128:], None, None, None, None, None, 1, 0, 128)
+    for rows in (buf[:128].view(1, 128), wide[:, 128:]):
+        assert torch.allclose((rows * rows).mean(-1), torch.ones(len(rows), device="cuda"), atol=1e-5)
+    x = np.random.default_rng(0).standard_normal(1024).astype(np.float32)  # host pointers: copied, any strides
+    w, n = x.reshape(4, 256), x[:512].reshape(4, 128)
+    ref, tol = R.norm_rope(w[:, :128].copy(), 1, 128, None, None, None, None, False, 1e-6)
+    gpu.qk_norm_rope(n, None, w[:, :128], None, None, None, None, None, 1, 0, 128)
+    _close(n, ref, tol)
